@@ -145,7 +145,9 @@ __global__ __launch_bounds__(256, 2) void conv_f32_fwd_kernel(F32FwdArgs a) {
           const int gy = y0 + 2 * wave + p;
           const float v = (gy < a.H && gx < a.W) ? acc[c2][p][e16] : 0.f;
           s += v;
-          q += v * v;
+          float vv = v * v;
+          asm("" : "+v"(vv));      // rounded before it is added: no fused multiply-add, whatever the compiler packs
+          q += vv;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
