@@ -446,6 +446,25 @@ int snws_bn_bwd_pack_post(const float* part, int T, int N, int C, const float* p
                           float* dbeta, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Layer normalisation over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias, mean and variance over the C
+ * elements of each row (the channels of one pixel of an NHWC tensor).  No counterpart in the reference: it stands beside
+ * SwitchNorm and BatchNorm for blocks that normalise every position by itself.
+ *
+ * x (rows, C) with row stride ldx, y with row stride ldy (elements; >= C), any alignment; dtype SNWS_F32 | SNWS_BF16;
+ * weight / bias f32 (C) or NULL (ones / zeros).  mean, rstd: f32 (rows), what the backward pass needs of each row, or both
+ * NULL.  Any C >= 1 and rows >= 0; no workspace. */
+int snws_ln_fwd(const void* x, int64_t ldx, const float* weight, const float* bias, void* y, int64_t ldy, int dtype,
+                int64_t rows, int C, float eps, float* mean, float* rstd, void* stream);
+/* With z = (x - mean) rstd and g = dy weight: dx = rstd (g - sum(g)/C - z sum(g z)/C) in dtype (NULL: not wanted);
+ * dweight = sum over rows of dy z, dbias = sum of dy, f32 (C), overwritten (NULL: not wanted; zeros for rows == 0).
+ * workspace: snws_ln_bwd_workspace_floats(...) floats when dweight or dbias is wanted; contents irrelevant.  The sums are
+ * taken in a fixed order. */
+int64_t snws_ln_bwd_workspace_floats(int dtype, int64_t rows, int C);
+int snws_ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* mean, const float* rstd,
+                const float* weight, int dtype, int64_t rows, int C, void* dx, int64_t lddx, float* dweight, float* dbias,
+                float* workspace, int64_t workspace_floats, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Full-scale skip resampling - replaces nn.MaxPool2d(k,k,ceil_mode=True) / nn.Upsample(scale, bilinear,
  * align_corners=False) / torch.cat at modeling/UNet3p_SNws.py:49-55,127-156 and their autograd.
  *

@@ -1,0 +1,341 @@
+// Layer normalisation over the last axis, backward.  With z = (x - mean) * rstd and g = dy * weight, per row
+//   dx = rstd * (g - sum(g) / C - z * sum(g * z) / C),
+// and over all rows dweight = sum(dy * z), dbias = sum(dy).
+//
+// Bound by memory: x and dy are read once and dx is written once.  One sweep does it all: a group of lanes holds a row
+// in registers (ln.h) and walks over rows, so its columns stay the same and their share of the two parameter gradients
+// is summed in registers.  A workgroup folds its groups and stores one partial row; a second, small launch adds the
+// partial rows in a fixed order in float64.  Runs with the same sizes give the same bits.
+#include "ln.h"
+
+namespace {
+using namespace ln;
+
+struct BwdArgs {
+  const void* dy;
+  const void* x;
+  const float* mean;
+  const float* rstd;
+  const float* w;      // nullptr: ones
+  void* dx;            // nullptr: not wanted
+  float* part;         // [blocks][2][C], nullptr: no parameter gradient wanted
+  int64_t lddy, ldx, lddx, rows;
+  int C;
+};
+
+constexpr int64_t MAX_BLOCKS = 512;   // two resident workgroups per CU
+
+template <typename T, int G, int NV, bool TAIL>
+__global__ __launch_bounds__(G <= 256 ? 256 : G) void ln_bwd_kernel(BwdArgs a) {
+  constexpr int VEC = Geo<T>::VEC, BT = G <= 256 ? 256 : G, GB = BT / G, R = Rows<NV>::R;
+  constexpr int NW = BT / 64, WC = (G < 64 ? G : 64) * NV * VEC;       // waves; columns that one wave holds
+  __shared__ float red[2 * NW];
+  __shared__ float fold[G < 256 ? 2 * WC : 1];
+  const int t = threadIdx.x % G, grp = threadIdx.x / G;
+  const T* x = static_cast<const T*>(a.x);
+  const T* dy = static_cast<const T*>(a.dy);
+  T* dx = static_cast<T*>(a.dx);
+  int col[NV], dup[NV];
+  float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c0 = (t + k * G) * VEC;
+    col[k] = TAIL && c0 + VEC > a.C ? a.C - VEC : c0;
+    dup[k] = TAIL ? (c0 - col[k] < VEC ? c0 - col[k] : VEC) : 0;
+    load_param<VEC>(a.w, col[k], 1.f, w[k]);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) dw[k][e] = db[k][e] = 0.f;
+  }
+  const float inv = 1.f / (float)a.C;
+  const int64_t step = (int64_t)gridDim.x * GB * R;
+  for (int64_t r0 = ((int64_t)blockIdx.x * GB + grp) * R; r0 < a.rows; r0 += step) {
+    uint4 vx[R][NV], vg[R][NV];
+    float mean[R], rstd[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = r0 + r < a.rows ? r0 + r : a.rows - 1;
+      mean[r] = a.mean[row];
+      rstd[r] = a.rstd[row];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        vx[r][k] = load_raw(x + row * a.ldx + col[k]);
+        vg[r][k] = load_raw(dy + row * a.lddy + col[k]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool live = R == 1 || r0 + r < a.rows;
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        float f[VEC], g[VEC];
+        unpack(vx[r][k], f);
+        unpack(vg[r][k], g);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float z = (f[e] - mean[r]) * rstd[r];
+          const bool on = (!TAIL || e >= dup[k]) && live;
+          const float d = on ? g[e] : 0.f, dz = on ? g[e] * z : 0.f;
+          db[k][e] += d;
+          dw[k][e] += dz;
+          s1 += d * w[k][e];
+          s2 += dz * w[k][e];
+        }
+      }
+      if (!dx) continue;
+      group_sum2<G>(s1, s2, red);
+      if (!live) continue;
+      const float m1 = s1 * inv, m2 = s2 * inv;
+      T* o = dx + (r0 + r) * a.lddx;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        float f[VEC], g[VEC];
+        unpack(vx[r][k], f);
+        unpack(vg[r][k], g);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float z = (f[e] - mean[r]) * rstd[r];
+          f[e] = rstd[r] * (g[e] * w[k][e] - m1 - z * m2);
+        }
+        if (!TAIL || dup[k] == 0) {
+          store_raw(o + col[k], pack(f));
+        } else {
+#pragma unroll
+          for (int e = 1; e < VEC; ++e)
+            if (e >= dup[k]) o[col[k] + e] = (T)f[e];
+        }
+      }
+    }
+  }
+  if (!a.part) return;
+  float* part = a.part + (int64_t)blockIdx.x * 2 * a.C;
+  if (G >= 256) {               // the workgroup is one group: its sums are the workgroup's
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (!TAIL || e >= dup[k]) {
+          part[col[k] + e] = dw[k][e];
+          part[a.C + col[k] + e] = db[k][e];
+        }
+    return;
+  }
+  // fold the groups of a wave by shuffles, then the waves one after the other through one row of LDS: a fixed order
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+#pragma unroll
+      for (int o = G; o < 64; o <<= 1) {
+        dw[k][e] += __shfl_xor(dw[k][e], o, 64);
+        db[k][e] += __shfl_xor(db[k][e], o, 64);
+      }
+    }
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int q = 0; q < NW; ++q) {
+    if (q == wave && lane < G) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (!TAIL || e >= dup[k]) {
+            const int c = col[k] + e;
+            fold[c] = q ? fold[c] + dw[k][e] : dw[k][e];
+            fold[WC + c] = q ? fold[WC + c] + db[k][e] : db[k][e];
+          }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < 2 * a.C; i += BT) part[i] = fold[i < a.C ? i : WC + i - a.C];
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void ln_bwd_narrow_kernel(BwdArgs a) {
+  constexpr int M = 7;
+  __shared__ float red[16];
+  const T* x = static_cast<const T*>(a.x);
+  const T* dy = static_cast<const T*>(a.dy);
+  T* dx = static_cast<T*>(a.dx);
+  const float inv = 1.f / (float)a.C;
+  float dw[M], db[M];
+#pragma unroll
+  for (int e = 0; e < M; ++e) dw[e] = db[e] = 0.f;
+  for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 256) {
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float z[M], g[M], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+      z[e] = e < a.C ? ((float)x[row * a.ldx + e] - mean) * rstd : 0.f;
+      g[e] = e < a.C ? (float)dy[row * a.lddy + e] : 0.f;
+      db[e] += g[e];
+      dw[e] += g[e] * z[e];
+      g[e] *= e < a.C && a.w ? a.w[e] : 1.f;
+      s1 += g[e];
+      s2 += g[e] * z[e];
+    }
+    if (dx) {
+#pragma unroll
+      for (int e = 0; e < M; ++e)
+        if (e < a.C) dx[row * a.lddx + e] = (T)(rstd * (g[e] - s1 * inv - z[e] * s2 * inv));
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int e = 0; e < M; ++e) {
+    const float sw = block_sum(dw[e], red), sb = block_sum(db[e], red);
+    if (threadIdx.x == 0 && e < a.C) {
+      a.part[(int64_t)blockIdx.x * 2 * a.C + e] = sw;
+      a.part[(int64_t)blockIdx.x * 2 * a.C + a.C + e] = sb;
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(512) void ln_bwd_wide_kernel(BwdArgs a) {
+  __shared__ float red[16];
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
+  T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+  const float mean = a.mean[row], rstd = a.rstd[row];
+  float s1 = 0.f, s2 = 0.f;
+  for (int c = threadIdx.x; c < a.C; c += 512) {
+    const float g = (float)dy[c] * (a.w ? a.w[c] : 1.f);
+    s1 += g;
+    s2 += g * ((float)x[c] - mean) * rstd;
+  }
+  group_sum2<512>(s1, s2, red);
+  const float m1 = s1 / (float)a.C, m2 = s2 / (float)a.C;
+  for (int c = threadIdx.x; c < a.C; c += 512) {
+    const float z = ((float)x[c] - mean) * rstd;
+    dx[c] = (T)(rstd * ((float)dy[c] * (a.w ? a.w[c] : 1.f) - m1 - z * m2));
+  }
+}
+
+// parameter gradients of such rows: a thread per column, rows dealt to gridDim.y slices
+template <typename T>
+__global__ __launch_bounds__(256) void ln_bwd_wide_param_kernel(BwdArgs a) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.C) return;
+  const T* x = static_cast<const T*>(a.x);
+  const T* dy = static_cast<const T*>(a.dy);
+  float dw = 0.f, db = 0.f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const float g = (float)dy[row * a.lddy + c];
+    db += g;
+    dw += g * ((float)x[row * a.ldx + c] - a.mean[row]) * a.rstd[row];
+  }
+  float* part = a.part + (int64_t)blockIdx.y * 2 * a.C;
+  part[c] = dw;
+  part[a.C + c] = db;
+}
+
+// dweight[c] / dbias[c] = sum over the partial rows, in float64 and a fixed order: 32 columns x 32 row lanes
+__global__ __launch_bounds__(1024) void ln_param_sum_kernel(const float* __restrict__ part, int blocks, int C,
+                                                            float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ double red[32][33];
+  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+  const int i = blockIdx.x * 32 + cl;
+  double s = 0.0;
+  if (i < 2 * C)
+    for (int r = rl; r < blocks; r += 32) s += (double)part[(int64_t)r * 2 * C + i];
+  red[rl][cl] = s;
+  __syncthreads();
+  if (rl == 0 && i < 2 * C) {
+    s = 0.0;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) s += red[r][cl];
+    float* o = i < C ? dw : db;
+    if (o) o[i < C ? i : i - C] = (float)s;
+  }
+}
+
+// workgroups of the sweep = partial rows
+template <typename T>
+int64_t bwd_blocks(int64_t rows, int C) {
+  constexpr int VEC = Geo<T>::VEC;
+  int64_t need;
+  if (C < VEC) {
+    need = cdiv64(rows, 256);
+  } else {
+    const int64_t chunks = cdiv64(C, VEC);
+    const int G = pick_group(chunks);
+    if (!G) {
+      need = cdiv64(rows, 16);                       // slices of the column sums
+      const int64_t cb = cdiv64(C, 256);
+      const int64_t most = cdiv64(1024, cb);
+      return need < most ? need : most;
+    }
+    const int nv = (int)cdiv64(chunks, G), R = nv == 1 ? 4 : nv == 2 ? 2 : 1;
+    need = cdiv64(rows, (int64_t)(G <= 256 ? 256 / G : 1) * R);
+  }
+  return need < MAX_BLOCKS ? need : MAX_BLOCKS;
+}
+
+template <typename T>
+struct Bwd {
+  const BwdArgs& a;
+  int64_t blocks;
+  hipStream_t st;
+  template <int G, int NV>
+  int run() {
+    constexpr int VEC = Geo<T>::VEC, BT = G <= 256 ? 256 : G;
+    if (a.C == G * NV * VEC) ln_bwd_kernel<T, G, NV, false><<<(unsigned)blocks, BT, 0, st>>>(a);
+    else ln_bwd_kernel<T, G, NV, true><<<(unsigned)blocks, BT, 0, st>>>(a);
+    SNWS_LAUNCH_CHECK("snws_ln_bwd");
+    return SNWS_OK;
+  }
+  int wide() {
+    if (a.rows > 0x7fffffff) SNWS_UNSUPPORTED("snws_ln_bwd: too many rows of this length");
+    if (a.dx) {
+      ln_bwd_wide_kernel<T><<<(unsigned)a.rows, 512, 0, st>>>(a);
+      SNWS_LAUNCH_CHECK("snws_ln_bwd");
+    }
+    if (a.part) {
+      ln_bwd_wide_param_kernel<T><<<dim3((unsigned)cdiv64(a.C, 256), (unsigned)blocks), 256, 0, st>>>(a);
+      SNWS_LAUNCH_CHECK("snws_ln_bwd");
+    }
+    return SNWS_OK;
+  }
+  int go() {
+    constexpr int VEC = Geo<T>::VEC;
+    if (a.C < VEC) {
+      ln_bwd_narrow_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(a);
+      SNWS_LAUNCH_CHECK("snws_ln_bwd");
+      return SNWS_OK;
+    }
+    return dispatch(cdiv64(a.C, VEC), *this);
+  }
+};
+
+}  // namespace
+
+extern "C" int64_t snws_ln_bwd_workspace_floats(int dtype, int64_t rows, int C) {
+  if (rows < 1 || C < 1) return 0;
+  return 2 * (int64_t)C * (dtype == SNWS_F32 ? bwd_blocks<float>(rows, C) : bwd_blocks<bf16_t>(rows, C));
+}
+
+extern "C" int snws_ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* mean, const float* rstd,
+                           const float* weight, int dtype, int64_t rows, int C, void* dx, int64_t lddx, float* dweight,
+                           float* dbias, float* workspace, int64_t workspace_floats, void* stream) {
+  SNWS_CHECK_ARG(dtype == SNWS_F32 || dtype == SNWS_BF16, "snws_ln_bwd: dtype must be float32 or bfloat16");
+  SNWS_CHECK_ARG(rows >= 0 && C >= 1 && lddy >= C && ldx >= C && (!dx || lddx >= C), "snws_ln_bwd: bad sizes");
+  SNWS_CHECK_ARG(rows == 0 || (dy && x && mean && rstd), "snws_ln_bwd: NULL pointer");
+  const bool params = dweight || dbias;
+  const int64_t need = params ? snws_ln_bwd_workspace_floats(dtype, rows, C) : 0;
+  SNWS_CHECK_ARG(need == 0 || (workspace && workspace_floats >= need), "snws_ln_bwd: workspace of %lld floats needed",
+                 (long long)need);
+  const hipStream_t st = (hipStream_t)stream;
+  int64_t blocks = 0;
+  if (rows > 0 && (dx || params)) {
+    blocks = dtype == SNWS_F32 ? bwd_blocks<float>(rows, C) : bwd_blocks<bf16_t>(rows, C);
+    const BwdArgs a{dy, x, mean, rstd, weight, dx, params ? workspace : nullptr, lddy, ldx, lddx, rows, C};
+    const int rc = dtype == SNWS_F32 ? Bwd<float>{a, blocks, st}.go() : Bwd<bf16_t>{a, blocks, st}.go();
+    if (rc != SNWS_OK) return rc;
+  }
+  if (params) {
+    ln_param_sum_kernel<<<(unsigned)cdiv64(2 * (int64_t)C, 32), 1024, 0, st>>>(workspace, (int)blocks, C, dweight, dbias);
+    SNWS_LAUNCH_CHECK("snws_ln_bwd");
+  }
+  return SNWS_OK;
+}

@@ -142,6 +142,9 @@ _SIGNATURES = {
     "snws_sn_apply_post": (c_int, [P, c_int64, P, c_int64, c_int, P, P, P, c_int, c_int64, c_int, c_int, P]),
     "snws_sn_bwd_apply_post": (c_int, [P, c_int64, P, c_int64, P, c_int64, c_int, P, P, P, P, c_int, c_int64, c_int, c_int, P]),
     "snws_bn_bwd_coeff": (c_int, [P, P, P, c_int, c_int, c_float, c_int, P]),
+    "snws_ln_fwd": (c_int, [P, c_int64, P, P, P, c_int64, c_int, c_int64, c_int, c_float, P, P, P]),
+    "snws_ln_bwd_workspace_floats": (c_int64, [c_int, c_int64, c_int]),
+    "snws_ln_bwd": (c_int, [P, c_int64, P, c_int64, P, P, P, c_int, c_int64, c_int, P, c_int64, P, P, P, c_int64, P]),
     "snws_tile_minmax_blocks": (c_int, [c_int64]),
     "snws_tile_minmax_scale": (c_int, [P, P, c_int, c_int, c_int64, P, P, P]),
     "snws_label_remap": (c_int, [P, c_int, P, c_int64, P]),

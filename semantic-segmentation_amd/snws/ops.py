@@ -4,6 +4,7 @@ torch.autograd.Functions behind Conv2dws / SwitchNorm2d / the fused ConvSnRelu b
 Tensors keep the reference's logical NCHW shape; physically they are NHWC ("channels last"), which is what
 the kernels read.  Everything here requires a GPU tensor: there is no CPU path.
 """
+import contextlib
 import ctypes
 import os
 
@@ -1242,6 +1243,110 @@ class BatchNormFn(torch.autograd.Function):
         ctx.s = None
         return (dx, _view(dg, ctx.shapes[0]) if ctx.has[0] else None, _view(db, ctx.shapes[1]) if ctx.has[1] else None,
                 None, None, None, None, None, None, None, None, None, None)
+
+
+# ------------------------------------------------------------------------------------------------ LayerNorm
+def on_device(t):
+    """Context in which t's device is the current one, so that launches, streams and workspaces belong to it."""
+    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _as_rows(x):
+    """(..., C) tensor -> (tensor read as rows of C consecutive elements, row stride ld, rows).  Leading axes that lie
+    one behind the other - a channel slice of a wider buffer among them - are read in place; anything else is copied."""
+    C = x.shape[-1]
+    rows = x.numel() // C
+    if x.is_contiguous():
+        return x, C, rows
+    ld, span, ok = 0, 1, C == 1 or x.stride(-1) == 1
+    for size, stride in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
+        if size == 1:
+            continue
+        if not ld:
+            ld = stride
+        ok = ok and stride == ld * span
+        span *= size
+    if ok and (rows <= 1 or ld >= C):
+        return x, max(ld, C), rows
+    return x.contiguous(), C, rows
+
+
+def _param32(p, C, what, x):
+    if p is None:
+        return None
+    if p.numel() != C:
+        raise ValueError("layer_norm: %s has %d elements for rows of %d" % (what, p.numel(), C))
+    if p.device != x.device:
+        raise RuntimeError("layer_norm: %s is on %s, the input on %s" % (what, p.device, x.device))
+    return _f32c(p)
+
+
+def _ln_forward(x, w32, b32, eps, keep):
+    """(y, rows x as read, its row stride, mean, rstd); mean and rstd are None unless `keep`."""
+    dt, C = dtype_code(x), x.shape[-1]
+    with on_device(x):
+        xs, ldx, rows = _as_rows(x.detach())
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
+        mp = stats.data_ptr() if keep and rows else None
+        _launch("ln_fwd", 2.0 * x.element_size() * rows * C, "snws_ln_fwd", xs.data_ptr(), ldx, _ptr(w32), _ptr(b32),
+                y.data_ptr(), C, dt, rows, C, eps, mp, mp + 4 * rows if mp else None, _stream())
+    return y, xs, ldx, stats
+
+
+class LayerNormFn(torch.autograd.Function):
+    """layer_norm with its gradients: one sweep over x and dy gives dx and the parameter gradients' partial sums."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, w32, b32, eps):
+        y, xs, ctx.ldx, stats = _ln_forward(x, w32, b32, eps, True)
+        # an input read in place is saved as itself, so that autograd notices a later change of it
+        ctx.save_for_backward(x if xs.data_ptr() == x.data_ptr() else xs, w32, stats)
+        ctx.keys = (grad_key(weight), grad_key(bias))
+        ctx.shapes = (None if weight is None else weight.shape, None if bias is None else bias.shape)
+        ctx.dtypes = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        xs, w32, stats = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        C, dev, dt = xs.shape[-1], xs.device, dtype_code(xs)
+        with on_device(xs):
+            dys, lddy, rows = _as_rows(dy if dy.dtype == xs.dtype else dy.to(xs.dtype))
+            dx = torch.empty(xs.shape, dtype=xs.dtype, device=dev) if need_x else None
+            dw = grad_out(ctx.keys[0], (C,), dev) if need_w else None
+            db = grad_out(ctx.keys[1], (C,), dev) if need_b else None
+            part, n = None, 0
+            if need_w or need_b:
+                n = L.lib().snws_ln_bwd_workspace_floats(dt, rows, C)
+                part = torch.empty(n, dtype=torch.float32, device=dev)
+            mp = stats.data_ptr() if rows else None
+            _launch("ln_bwd", 3.0 * xs.element_size() * rows * C, "snws_ln_bwd", dys.data_ptr(), lddy, xs.data_ptr(), ctx.ldx,
+                    mp, mp + 4 * rows if mp else None, _ptr(w32), dt, rows, C, _ptr(dx), C, _ptr(dw), _ptr(db), _ptr(part),
+                    n, _stream())
+            dw, db = _view(grad_fold(dw), ctx.shapes[0]), _view(grad_fold(db), ctx.shapes[1])
+            dw = dw if dw is None else dw.to(ctx.dtypes[0])
+            db = db if db is None else db.to(ctx.dtypes[1])
+        return dx, dw, db, None, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (..., C), float32 or bfloat16; mean and
+    variance (biased) in float32 over each position's own C elements.  weight / bias: C values (kept in float32) or None.
+    Leading axes may be strided like a channel slice of a wider buffer; the result is contiguous.  Differentiable once
+    in x, weight and bias."""
+    require_gpu(x, "layer_norm")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("layer_norm: a last axis of at least one element expected, got shape %s" % (tuple(x.shape),))
+    dtype_code(x)
+    eps = float(eps)
+    w32, b32 = _param32(weight, x.shape[-1], "weight", x), _param32(bias, x.shape[-1], "bias", x)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        return LayerNormFn.apply(x, weight, bias, w32, b32, eps)
+    return _ln_forward(x, w32, b32, eps, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------ autograd
