@@ -586,6 +586,40 @@ int snws_adamw_step(float* param, const float* grad, float* exp_avg, float* exp_
                     void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Orthogonalisation by Newton-Schulz products, and the Muon update.  No counterpart in the reference: an optimizer for
+ * filters and matrices beside AdamW.  For each matrix G, taken with its shorter side as rows:
+ *   X = G / max(|G|_F, eps);  then for each step's (a, b, c):  A = X X^T,  X <- (a I + b A + c A^2) X.
+ * Products run on the 16-bit matrix cores with every number held as a pair of halves: float32 accuracy.
+ *
+ * Up to SNWS_ORTHO_MAX matrices of any shapes (1 <= rows, cols <= 2^20, the shorter side <= 32768) share the launches of
+ * one call.  coeff: 3 * steps floats in HOST memory, 1 <= steps <= 32; coefficients under which singular values in [0, 1]
+ * can grow beyond 1024 are refused (SNWS_ERR_INVALID).  workspace: snws_ortho_workspace_bytes(...) bytes, 256-byte
+ * aligned, contents irrelevant; calls that may overlap need one each. */
+#define SNWS_ORTHO_MAX 32
+typedef struct snws_ortho_item {
+  const void* x;    /* (rows, cols), row stride ldx */
+  void* out;        /* (rows, cols), row stride ldo; may be x itself */
+  int64_t ldx, ldo; /* elements, >= cols */
+  int rows, cols;
+} snws_ortho_item;
+typedef struct snws_muon_item {
+  float* param;     /* (rows, cols) contiguous */
+  const float* grad;
+  float* momentum;
+  int rows, cols;
+  float lr;         /* learning rate times the matrix's own factor */
+} snws_muon_item;
+int64_t snws_ortho_workspace_bytes(const int* rows, const int* cols, int count); /* -1: sizes that are refused */
+/* x and out of dtype SNWS_F32 | SNWS_BF16 */
+int snws_orthogonalize(const snws_ortho_item* items, int count, int dtype, const float* coeff, int steps, float eps,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+/* m <- momentum m + (1 - momentum) g with g = grad_scale * grad;  u = (1 - momentum) g + momentum m (nesterov) or m;
+ * param <- (1 - weight_decay) param - lr * orthogonalised(u).  (weight_decay: already times the learning rate.) */
+int snws_muon_update(const snws_muon_item* items, int count, float momentum, int nesterov, float grad_scale,
+                     float weight_decay, const float* coeff, int steps, float eps, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Collectives for hosts without their own - the exchange points of the data-parallel path as in-place all-reduces
  * over RCCL, loaded at run time.  Replaces the SyncMaster / SlavePipe rendez-vous of
  * modeling/sync_batchnorm/comm.py:39-43,71-90 (SwitchNorm / BN statistics: the `pack` buffers of snws_sn_mix_a and

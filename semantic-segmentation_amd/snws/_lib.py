@@ -45,7 +45,19 @@ class SnBwdItem(Structure):
                 ("reserved", c_int)]
 
 
+class OrthoItem(Structure):
+    """snws_ortho_item: one matrix of an orthogonalisation call."""
+    _fields_ = [("x", c_void_p), ("out", c_void_p), ("ldx", c_int64), ("ldo", c_int64), ("rows", c_int), ("cols", c_int)]
+
+
+class MuonItem(Structure):
+    """snws_muon_item: one parameter of a Muon update."""
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("momentum", c_void_p), ("rows", c_int), ("cols", c_int),
+                ("lr", c_float)]
+
+
 SN_BATCH_MAX = 8
+ORTHO_MAX = 32
 P = c_void_p
 _SIGNATURES = {
     "snws_version": (c_int, []),
@@ -150,6 +162,10 @@ _SIGNATURES = {
     "snws_label_remap": (c_int, [P, c_int, P, c_int64, P]),
     "snws_nchw_to_nhwc_pad": (c_int, [P, c_int, P, c_int, c_int, c_int, c_int, c_int, c_int, P]),
     "snws_adamw_step": (c_int, [P, P, P, P, c_int64, c_float, c_float, c_float, c_float, c_float, c_int64, c_float, P]),
+    "snws_ortho_workspace_bytes": (c_int64, [POINTER(c_int), POINTER(c_int), c_int]),
+    "snws_orthogonalize": (c_int, [POINTER(OrthoItem), c_int, c_int, POINTER(c_float), c_int, c_float, P, c_int64, P]),
+    "snws_muon_update": (c_int, [POINTER(MuonItem), c_int, c_float, c_int, c_float, c_float, POINTER(c_float), c_int, c_float, P,
+                                 c_int64, P]),
     "snws_comm_unique_id": (c_int, [P]),
     "snws_comm_init": (c_int, [P, c_int, c_int, P]),
     "snws_comm_allreduce_f32": (c_int, [P, P, c_int64, P]),

@@ -1246,9 +1246,18 @@ class BatchNormFn(torch.autograd.Function):
 
 
 # ------------------------------------------------------------------------------------------------ LayerNorm
+_HERE = contextlib.nullcontext()
+
+
 def on_device(t):
     """Context in which t's device is the current one, so that launches, streams and workspaces belong to it."""
-    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def stream_of(t):
+    """The current stream of t's device as a plain number.  (torch.cuda.current_stream() builds an object first: 3 us, as
+    much as a launch.)"""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _as_rows(x):
@@ -1278,19 +1287,24 @@ def _param32(p, C, what, x):
         raise ValueError("layer_norm: %s has %d elements for rows of %d" % (what, p.numel(), C))
     if p.device != x.device:
         raise RuntimeError("layer_norm: %s is on %s, the input on %s" % (what, p.device, x.device))
-    return _f32c(p)
+    return p if p.dtype is torch.float32 and p.is_contiguous() else _f32c(p)
 
 
 def _ln_forward(x, w32, b32, eps, keep):
-    """(y, rows x as read, its row stride, mean, rstd); mean and rstd are None unless `keep`."""
-    dt, C = dtype_code(x), x.shape[-1]
+    """(y, x as read, its row stride, [mean | rstd] or None without `keep`)."""
     with on_device(x):
-        xs, ldx, rows = _as_rows(x.detach())
+        xs, ldx, rows = _as_rows(x)
+        C = xs.shape[-1]
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
-        mp = stats.data_ptr() if keep and rows else None
-        _launch("ln_fwd", 2.0 * x.element_size() * rows * C, "snws_ln_fwd", xs.data_ptr(), ldx, _ptr(w32), _ptr(b32),
-                y.data_ptr(), C, dt, rows, C, eps, mp, mp + 4 * rows if mp else None, _stream())
+        stats = mp = rp = None
+        if keep:
+            stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device)
+            if rows:
+                mp = stats.data_ptr()
+                rp = mp + 4 * rows
+        _launch("ln_fwd", 2.0 * x.element_size() * rows * C, "snws_ln_fwd", xs.data_ptr(), ldx,
+                None if w32 is None else w32.data_ptr(), None if b32 is None else b32.data_ptr(), y.data_ptr(), C, _DT[x.dtype],
+                rows, C, eps, mp, rp, stream_of(x))
     return y, xs, ldx, stats
 
 
@@ -1300,11 +1314,9 @@ class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, w32, b32, eps):
         y, xs, ctx.ldx, stats = _ln_forward(x, w32, b32, eps, True)
-        # an input read in place is saved as itself, so that autograd notices a later change of it
-        ctx.save_for_backward(x if xs.data_ptr() == x.data_ptr() else xs, w32, stats)
-        ctx.keys = (grad_key(weight), grad_key(bias))
-        ctx.shapes = (None if weight is None else weight.shape, None if bias is None else bias.shape)
-        ctx.dtypes = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        ctx.save_for_backward(xs, w32, stats)
+        ctx.weight = None if weight is None else (grad_key(weight), weight.shape, weight.dtype)
+        ctx.bias = None if bias is None else (grad_key(bias), bias.shape, bias.dtype)
         return y
 
     @staticmethod
@@ -1312,24 +1324,32 @@ class LayerNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         xs, w32, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        C, dev, dt = xs.shape[-1], xs.device, dtype_code(xs)
+        C, dev, dt = xs.shape[-1], xs.device, _DT[xs.dtype]
         with on_device(xs):
-            dys, lddy, rows = _as_rows(dy if dy.dtype == xs.dtype else dy.to(xs.dtype))
+            dys, lddy, rows = _as_rows(dy if dy.dtype is xs.dtype else dy.to(xs.dtype))
             dx = torch.empty(xs.shape, dtype=xs.dtype, device=dev) if need_x else None
-            dw = grad_out(ctx.keys[0], (C,), dev) if need_w else None
-            db = grad_out(ctx.keys[1], (C,), dev) if need_b else None
+            dw = grad_out(ctx.weight[0], (C,), dev) if need_w else None
+            db = grad_out(ctx.bias[0], (C,), dev) if need_b else None
             part, n = None, 0
             if need_w or need_b:
                 n = L.lib().snws_ln_bwd_workspace_floats(dt, rows, C)
                 part = torch.empty(n, dtype=torch.float32, device=dev)
             mp = stats.data_ptr() if rows else None
             _launch("ln_bwd", 3.0 * xs.element_size() * rows * C, "snws_ln_bwd", dys.data_ptr(), lddy, xs.data_ptr(), ctx.ldx,
-                    mp, mp + 4 * rows if mp else None, _ptr(w32), dt, rows, C, _ptr(dx), C, _ptr(dw), _ptr(db), _ptr(part),
-                    n, _stream())
-            dw, db = _view(grad_fold(dw), ctx.shapes[0]), _view(grad_fold(db), ctx.shapes[1])
-            dw = dw if dw is None else dw.to(ctx.dtypes[0])
-            db = db if db is None else db.to(ctx.dtypes[1])
-        return dx, dw, db, None, None, None
+                    mp, mp + 4 * rows if rows else None, None if w32 is None else w32.data_ptr(), dt, rows, C,
+                    None if dx is None else dx.data_ptr(), C, None if dw is None else dw.data_ptr(),
+                    None if db is None else db.data_ptr(), None if part is None else part.data_ptr(), n, stream_of(xs))
+            return dx, _param_grad(dw, ctx.weight), _param_grad(db, ctx.bias), None, None, None
+
+
+def _param_grad(g, param):
+    g = grad_fold(g)
+    if g is None:
+        return None
+    _, shape, dtype = param
+    if g.shape != shape:
+        g = g.view(shape)
+    return g if g.dtype is dtype else g.to(dtype)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -2301,3 +2321,152 @@ def max_pool_ceil(x, k):
 
 def upsample_bilinear(x, k):
     return ResampleFn.apply(x, "bilinear", int(k))
+
+
+# ------------------------------------------------------------------------------------------------ orthogonalisation, Muon
+QUINTIC = (3.4445, -4.775, 2.0315)      # slope 3.4 at zero; singular values end within about [0.7, 1.2] after five steps
+
+
+def _ortho_coefficients(coefficients, steps):
+    """One (a, b, c) for every step, or a list of one per step -> (ctypes floats, number of steps)."""
+    steps = int(steps)
+    if steps < 1:
+        raise ValueError("orthogonalize: at least one step expected, got %d" % steps)
+    rows = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else list(coefficients)
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError("orthogonalize: three coefficients, or three for each of the %d steps, expected" % steps)
+    return (ctypes.c_float * (3 * steps))(*[float(v) for r in rows for v in r])
+
+
+def _ortho_workspace(sizes, device):
+    n = len(sizes)
+    nbytes = L.lib().snws_ortho_workspace_bytes((ctypes.c_int * n)(*[r for r, _ in sizes]),
+                                                (ctypes.c_int * n)(*[c for _, c in sizes]), n)
+    if nbytes < 0:
+        raise ValueError(L.lib().snws_last_error().decode("utf-8", "replace"))
+    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+
+
+def _ortho_flops(sizes, steps):
+    return float(sum(steps * (3 * min(s) ** 2 * max(s) + min(s) ** 3) for s in sizes))
+
+
+def _by_size(n, size):
+    """Indices of a list in calls of at most ORTHO_MAX, the largest matrices first: like sizes share launches."""
+    order = sorted(range(n), key=lambda i: -size(i))
+    return [order[i:i + L.ORTHO_MAX] for i in range(0, n, L.ORTHO_MAX)]
+
+
+@torch.no_grad()
+def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
+    """The matrices of g with their singular values pushed towards one, by `steps` Newton-Schulz steps
+    X <- a X + (b A + c A^2) X, A = X X^T, from X = G / max(|G|_F, eps), on the shorter side of each matrix.
+
+    g: a matrix (m, n), a batch (..., m, n) or a list / tuple of matrices of any shapes, float32 or bfloat16 on one
+    device; returns new contiguous tensors in the same arrangement.  coefficients: (a, b, c), or one such triple per
+    step.  A matrix that holds a NaN or an infinity comes out as NaN; the others of the call are not touched by it.  Not
+    differentiable."""
+    if isinstance(g, torch.Tensor):
+        if g.dim() < 2:
+            raise ValueError("orthogonalize: matrices expected, got shape %s" % (tuple(g.shape),))
+        if g.dim() == 2:
+            return orthogonalize([g], steps, coefficients, eps)[0]
+        require_gpu(g, "orthogonalize")
+        flat = g.reshape((-1,) + g.shape[-2:])
+        if not flat.numel():
+            return torch.empty(g.shape, dtype=g.dtype, device=g.device)
+        return torch.stack(orthogonalize(list(flat.unbind(0)), steps, coefficients, eps)).view(g.shape)
+    mats = list(g)
+    coeff = _ortho_coefficients(coefficients, steps)
+    for t in mats:
+        require_gpu(t, "orthogonalize")
+        if t.dim() != 2:
+            raise ValueError("orthogonalize: matrices expected, got shape %s" % (tuple(t.shape),))
+        if t.device != mats[0].device or t.dtype != mats[0].dtype:
+            raise ValueError("orthogonalize: matrices of one type on one device expected")
+    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in mats]
+    live = [i for i, t in enumerate(mats) if t.numel()]
+    if not live:
+        return out
+    dt, dev = dtype_code(mats[0]), mats[0].device
+    with on_device(mats[0]):
+        for part in _by_size(len(live), lambda i: mats[live[i]].numel()):
+            part = [live[i] for i in part]
+            # read in place: rows of consecutive elements, one behind the other at any distance
+            src = [t if (t.shape[1] == 1 or t.stride(1) == 1) and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else
+                   t.contiguous() for t in (mats[i] for i in part)]
+            items = (L.OrthoItem * len(part))()
+            for it, t, i in zip(items, src, part):
+                rows, cols = t.shape
+                it.x, it.out, it.rows, it.cols = t.data_ptr(), out[i].data_ptr(), rows, cols
+                it.ldx, it.ldo = t.stride(0) if rows > 1 else cols, cols
+            sizes = [tuple(t.shape) for t in src]
+            ws, nbytes = _ortho_workspace(sizes, dev)
+            _launch("orthogonalize", _ortho_flops(sizes, int(steps)), "snws_orthogonalize", items, len(part), dt, coeff,
+                    int(steps), float(eps), ws.data_ptr(), nbytes, stream_of(mats[0]))
+    return out
+
+
+def muon_lr_factor(adjust, rows, cols):
+    """Factor on the learning rate of a (rows, cols) matrix: "original" (None): sqrt(max(1, rows / cols));
+    "match_rms_adamw": 0.2 sqrt(max(rows, cols)), which gives updates of the size AdamW's have."""
+    if adjust is None or adjust == "original":
+        return max(1.0, rows / cols) ** 0.5
+    if adjust == "match_rms_adamw":
+        return 0.2 * max(rows, cols) ** 0.5
+    raise ValueError("muon: adjust_lr is None, 'original' or 'match_rms_adamw', got %r" % (adjust,))
+
+
+@torch.no_grad()
+def muon_update(params, grads, momentum_buffers, lr, weight_decay=0.1, momentum=0.95, nesterov=True, coefficients=QUINTIC,
+                eps=1e-7, steps=5, adjust_lr=None, grad_scale=1.0):
+    """One Muon step, in place, for every parameter of the lists (float32, two or more axes; the axes after the first are
+    taken together, so a filter (O, I, kh, kw) is an O x (I kh kw) matrix):
+        m <- momentum m + (1 - momentum) g;  u = (1 - momentum) g + momentum m  (nesterov)  or  m;
+        p <- (1 - lr weight_decay) p - lr factor orthogonalize(u),  factor: see muon_lr_factor.
+    g is grad_scale times the gradient.  Parameters and momentum buffers must be contiguous and all different."""
+    params, grads, bufs = list(params), list(grads), list(momentum_buffers)
+    if not (len(params) == len(grads) == len(bufs)):
+        raise ValueError("muon_update: %d parameters, %d gradients, %d momentum buffers" % (len(params), len(grads), len(bufs)))
+    coeff = _ortho_coefficients(coefficients, steps)
+    lr, weight_decay = float(lr), float(weight_decay)
+    muon_lr_factor(adjust_lr, 1, 1)
+    seen = set()
+    for p, g, m in zip(params, grads, bufs):
+        require_gpu(p, "muon_update")
+        if p.dim() < 2:
+            raise ValueError("muon_update: parameters of two or more axes expected, got shape %s" % (tuple(p.shape),))
+        for t in (g, m):
+            if t.shape != p.shape or t.device != p.device or p.device != params[0].device:
+                raise ValueError("muon_update: parameter, gradient and momentum of one shape on one device expected")
+        if p.dtype != torch.float32 or g.dtype != torch.float32 or m.dtype != torch.float32:
+            raise TypeError("muon_update: float32 tensors expected")
+        if not (p.is_contiguous() and m.is_contiguous()):
+            raise ValueError("muon_update: contiguous parameters and momentum buffers expected")
+        if p.numel():
+            if p.data_ptr() in seen or m.data_ptr() in seen or p.data_ptr() == m.data_ptr():
+                raise ValueError("muon_update: a parameter or momentum buffer is given twice")
+            seen.update((p.data_ptr(), m.data_ptr()))
+    live = [i for i, p in enumerate(params) if p.numel()]
+    if not live:
+        return
+    with on_device(params[0]):
+        for part in _by_size(len(live), lambda i: params[live[i]].numel()):
+            part = [live[i] for i in part]
+            items = (L.MuonItem * len(part))()
+            sizes, keep = [], []
+            for it, i in zip(items, part):
+                p, g = params[i], grads[i]
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    keep.append(g)
+                rows = p.shape[0]
+                cols = p.numel() // rows
+                sizes.append((rows, cols))
+                it.param, it.grad, it.momentum, it.rows, it.cols = p.data_ptr(), g.data_ptr(), bufs[i].data_ptr(), rows, cols
+                it.lr = lr * muon_lr_factor(adjust_lr, rows, cols)
+            ws, nbytes = _ortho_workspace(sizes, params[0].device)
+            _launch("muon_update", _ortho_flops(sizes, int(steps)), "snws_muon_update", items, len(part), float(momentum),
+                    int(bool(nesterov)), float(grad_scale), lr * weight_decay, coeff, int(steps), float(eps), ws.data_ptr(),
+                    nbytes, stream_of(params[0]))
+    weights_changed()       # the kernels do not bump version counters
