@@ -609,7 +609,7 @@ typedef struct snws_muon_item {
   int rows, cols;
   float lr;         /* learning rate times the matrix's own factor */
 } snws_muon_item;
-int64_t snws_ortho_workspace_bytes(const int* rows, const int* cols, int count); /* -1: sizes that are refused */
+int64_t snws_ortho_workspace_bytes(const int* rows, const int* cols, int count, int steps); /* -1: refused */
 /* x and out of dtype SNWS_F32 | SNWS_BF16 */
 int snws_orthogonalize(const snws_ortho_item* items, int count, int dtype, const float* coeff, int steps, float eps,
                        void* workspace, int64_t workspace_bytes, void* stream);

@@ -11,10 +11,9 @@
 // below 2^-22 of it.  The scales s come from bounds on the spectral norms (host, ortho_scales), so hi never overflows.
 //
 // Layout: a matrix with rows of K numbers is stored as rows of 32-number blocks [hi x 32 | lo x 32]: one block is one
-// 128-byte line, a k-step of 32 is 8 rows x 128 bytes per LDS-DMA instruction, and both halves of a fragment come from
-// the same line.  Every product here is D[p][q] = sum_k P[p][k] Q[q][k], both operands contiguous along k:
-//   A = X X^T from X;   A^2 from A (symmetric);   (B X)^T = X^T B from Y = X^T and B (symmetric),
-// so X and its transpose Y are both kept, and the epilogues store a tile twice, once through a transposing read of LDS.
+// 128-byte line, an LDS-DMA instruction copies 8 rows x 128 bytes, and both halves of a fragment come from the same line.
+// X X^T and the m x m products read both operands along their rows (all m x m matrices here are symmetric); B X reads
+// X down its columns, through the transposing LDS read, so X is kept in one orientation only.
 //
 // All matrices of a list share each launch: a workgroup finds its matrix and tile from its index.
 #include "common.h"
@@ -26,15 +25,14 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 
 constexpr int MAXM = SNWS_ORTHO_MAX;
-constexpr int NORM_CHUNK = 16384;    // elements per partial sum of squares
+constexpr int NORM_CHUNK = 8192;    // elements per partial sum of squares
 
 struct Mat {
   const void* x;       // (rows, cols), row stride ldx: the matrix, or the gradient of a Muon item
   void* out;           // (rows, cols), row stride ldo: the result, or the parameter of a Muon item
   float* mom;          // momentum of a Muon item
   int64_t ldx, ldo;
-  int64_t X, Y, A;     // byte offsets into the workspace; the second Y lies behind the first, B behind A
-  int64_t part;        // split-K partial tiles of A
+  int64_t at;          // its part of the workspace (bytes): X, a second X, the slots, partial tiles of A
   int m, n;            // m <= n
   int flip;            // rows > cols: X is the transpose
   int ks, kc;          // splits of the contraction over n and 32-blocks in each
@@ -42,11 +40,27 @@ struct Mat {
   float step;          // learning rate of a Muon item
 };
 
+enum Phase { NORM, START, GRAM, JOIN, SQUARE, APPLY, PHASES };
+
+// The first kernel of a call gets this by value and leaves a copy at the start of the workspace for the others: kernel
+// arguments lie in host memory, where each dependent read costs a microsecond.
 struct Mats {
   Mat mat[MAXM];
-  int end[MAXM];       // first workgroup index behind each matrix, for the launch at hand
+  int end[PHASES][MAXM];      // first workgroup index behind each matrix, by the kind of launch
   int count;
   unsigned char* ws;
+};
+
+// D = ca I + cb C + cc P Q on the slots of every matrix (see square_tile), or a product with X
+enum Kind { K_GRAM, K_SQUARE, K_APPLY };
+struct Op {
+  unsigned char kind, sp, sq, sc, sd, last, pad[2];
+  float ca, cb, cc;
+};
+constexpr int MAX_OPS = 24;    // of a program that one kernel runs: six steps in groups take at most 22
+struct Program {
+  int n;
+  Op op[MAX_OPS];
 };
 
 struct MuonArgs {
@@ -56,9 +70,26 @@ struct MuonArgs {
 
 __host__ __device__ __forceinline__ int up32(int v) { return (v + 31) & ~31; }
 
-__device__ __forceinline__ void glds16(const void* gsrc, unsigned char* lds_wave_base) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gsrc,
-                                   (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
+// parts of a matrix's workspace; every one is a whole number of 128-byte blocks
+constexpr int SLOTS = 6;
+__host__ __device__ __forceinline__ int64_t size_x(const Mat& t) { return (int64_t)t.m * up32(t.n) * 4; }
+__host__ __device__ __forceinline__ int64_t size_slot(const Mat& t) { return (int64_t)t.m * up32(t.m) * 4; }
+__device__ __forceinline__ unsigned char* x_of(const Mat& t, unsigned char* ws, int odd) { return ws + t.at + (odd ? size_x(t) : 0); }
+__device__ __forceinline__ unsigned char* slot_of(const Mat& t, unsigned char* ws, int k) {
+  return ws + t.at + 2 * size_x(t) + k * size_slot(t);
+}
+__device__ __forceinline__ f32x4* part_of(const Mat& t, unsigned char* ws) {
+  return reinterpret_cast<f32x4*>(slot_of(t, ws, SLOTS));
+}
+
+// 16 bytes per lane from global memory into LDS, lane after lane from byte `lds` on (the same for the whole wave).  Written
+// out because the compiler would wait for every copy in flight before a transposing read; it has no result registers, and
+// the waits for it stand in product().  Nothing else here uses m0.
+__device__ __forceinline__ void glds16(const void* gsrc, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gsrc), "s"(lds));
+}
+__device__ __forceinline__ unsigned lds_offset(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
 
 // blocks dealt to the same XCD (bid % 8) get consecutive logical ids
@@ -67,24 +98,41 @@ __device__ __forceinline__ unsigned xcd_order(unsigned bid, unsigned nblk) {
   return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
 }
 
-// matrix of workgroup id, and the id within it
-__device__ __forceinline__ int find_mat(const Mats& a, int id, int& local) {
-  const int lane = threadIdx.x & 63;
-  const bool past = lane < a.count && id >= a.end[lane];
+// Matrix of this workgroup and its index there.  Workgroups of one XCD (every eighth) get neighbouring indices within each
+// matrix: they share operands in its L2, and every XCD gets its share of every matrix.
+__device__ __forceinline__ int find_mat(const Mats& a, int phase, int& local) {
+  const int lane = threadIdx.x & 63, id = blockIdx.x;
+  const bool past = lane < a.count && id >= a.end[phase][lane];
   const int i = __builtin_amdgcn_readfirstlane(__popcll(__ballot(past)));
-  local = i ? id - a.end[i - 1] : id;
+  const int from = i ? a.end[phase][i - 1] : 0;
+  local = xcd_order(id - from, a.end[phase][i] - from);
   return i;
 }
 
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+
+// v = hi + lo: two numbers at a time through the packed conversions, the remainder by one mixed multiply-add
+__device__ __forceinline__ void split2(float a, float b, f16x2& hi, f16x2& lo) {
+  hi = __builtin_convertvector((f32x2{a, b}), f16x2);
+  lo = __builtin_convertvector((f32x2{fmaf((float)hi[0], -1.f, a), fmaf((float)hi[1], -1.f, b)}), f16x2);
+}
+__device__ __forceinline__ void split4(const float (&v)[4], f16x4& hi, f16x4& lo) {
+  f16x2 h0, h1, l0, l1;
+  split2(v[0], v[1], h0, l0);
+  split2(v[2], v[3], h1, l1);
+  hi = f16x4{h0[0], h0[1], h1[0], h1[1]};
+  lo = f16x4{l0[0], l0[1], l1[0], l1[1]};
+}
 __device__ __forceinline__ void split8(const float (&v)[8], uint4& hi, uint4& lo) {
-  f16x8 h, l;
+  f16x2 h[4], l[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    h[e] = (_Float16)v[e];
-    l[e] = (_Float16)(v[e] - (float)h[e]);
-  }
-  hi = __builtin_bit_cast(uint4, h);
-  lo = __builtin_bit_cast(uint4, l);
+  for (int e = 0; e < 4; ++e) split2(v[2 * e], v[2 * e + 1], h[e], l[e]);
+  hi = make_uint4(__builtin_bit_cast(unsigned, h[0]), __builtin_bit_cast(unsigned, h[1]), __builtin_bit_cast(unsigned, h[2]),
+                  __builtin_bit_cast(unsigned, h[3]));
+  lo = make_uint4(__builtin_bit_cast(unsigned, l[0]), __builtin_bit_cast(unsigned, l[1]), __builtin_bit_cast(unsigned, l[2]),
+                  __builtin_bit_cast(unsigned, l[3]));
 }
 // eight numbers of a row from column c (a multiple of 8), `row` its first byte
 __device__ __forceinline__ void store8(unsigned char* row, int c, const float (&v)[8]) {
@@ -103,9 +151,6 @@ __device__ __forceinline__ void load8(const unsigned char* row, int c, float (&v
 }
 
 // ------------------------------------------------------------------------------------------------ start
-template <typename T>
-__device__ __forceinline__ float elem(const T* p, int64_t i) { return (float)p[i]; }
-
 // the matrix itself, or a Muon item's update direction from gradient and momentum (already advanced)
 __device__ __forceinline__ float direction(float g, float m, const MuonArgs& u) {
   return u.nesterov ? (1.f - u.momentum) * g + u.momentum * m : m;
@@ -114,18 +159,13 @@ __device__ __forceinline__ float direction(float g, float m, const MuonArgs& u) 
 // Partial sums of squares in float64 (no overflow or underflow over float32's range, a fixed order); a Muon item's
 // momentum is advanced on the way: m <- momentum m + (1 - momentum) grad_scale g.
 template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void ortho_norm_kernel(Mats a, MuonArgs u, double* __restrict__ partial) {
-  __shared__ double red[16];
-  int chunk;
-  const Mat& t = a.mat[find_mat(a, blockIdx.x, chunk)];
+__device__ __forceinline__ double norm_chunk(const Mat& t, int chunk, const MuonArgs& u) {
+  constexpr int VEC = MUON ? 4 : 16 / (int)sizeof(T);
   const int rows = t.flip ? t.n : t.m, cols = t.flip ? t.m : t.n;
   const int64_t total = (int64_t)rows * cols, lo = (int64_t)chunk * NORM_CHUNK;
-  const int64_t hi = lo + NORM_CHUNK < total ? lo + NORM_CHUNK : total;
   const T* x = static_cast<const T*>(t.x);
   double s = 0.0;
-  const bool flat = t.ldx == cols;
-  for (int64_t i = lo + threadIdx.x; i < hi; i += 256) {
-    float v = elem(x, flat ? i : (i / cols) * t.ldx + i % cols);
+  auto one = [&](int64_t i, float v) {
     if (MUON) {
       v *= u.grad_scale;
       const float m = u.momentum * t.mom[i] + (1.f - u.momentum) * v;
@@ -133,132 +173,330 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(Mats a, MuonArgs u, dou
       v = direction(v, m, u);
     }
     s += (double)v * (double)v;
+  };
+  const bool flat = t.ldx == cols && (((uintptr_t)x | (MUON ? (uintptr_t)t.mom : 0)) & 15) == 0;
+  const int64_t hi = lo + NORM_CHUNK < total ? lo + NORM_CHUNK : total;
+  if (flat) {       // chunks start at multiples of 16 bytes: all loads of a thread in flight at once
+    constexpr int NL = NORM_CHUNK / (256 * VEC);
+    uint4 v[NL];
+    float4 m[MUON ? NL : 1];
+#pragma unroll
+    for (int k = 0; k < NL; ++k) {
+      const int64_t i = lo + (int64_t)(k * 256 + threadIdx.x) * VEC;
+      v[k] = make_uint4(0, 0, 0, 0);
+      if (MUON) m[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i + VEC <= hi) {
+        v[k] = *reinterpret_cast<const uint4*>(x + i);
+        if (MUON) m[k] = *reinterpret_cast<const float4*>(t.mom + i);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < NL; ++k) {
+      const T* e8 = reinterpret_cast<const T*>(&v[k]);
+      float d[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) d[e] = (float)e8[e];
+      if (MUON) {
+        float* me = &m[k].x;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          d[e] *= u.grad_scale;
+          me[e] = u.momentum * me[e] + (1.f - u.momentum) * d[e];
+          d[e] = direction(d[e], me[e], u);
+        }
+        const int64_t i = lo + (int64_t)(k * 256 + threadIdx.x) * VEC;
+        if (i + VEC <= hi) *reinterpret_cast<float4*>(t.mom + i) = m[k];
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s += (double)d[e] * (double)d[e];
+    }
+    const int64_t tail = hi - (hi - lo) % VEC + threadIdx.x;
+    if (tail < hi) one(tail, (float)x[tail]);
+  } else {
+    int64_t i = lo + threadIdx.x;
+    if (i < hi) {
+      int64_t r = i / cols;
+      int c = (int)(i - r * cols);
+#pragma unroll 8
+      for (; i < hi; i += 256) {
+        one(i, (float)x[r * t.ldx + c]);
+        for (c += 256; c >= cols; c -= cols) ++r;
+      }
+    }
   }
-  s = block_sum(s, red);
+  return s;
+}
+
+template <typename T, bool MUON>
+__global__ __launch_bounds__(256) void ortho_norm_kernel(Mats a, MuonArgs u, double* __restrict__ partial) {
+  __shared__ double red[16];
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < (int)(sizeof(Mats) / 4); i += 256)
+      reinterpret_cast<int*>(a.ws)[i] = reinterpret_cast<const int*>(&a)[i];
+  int chunk;
+  const Mat& t = a.mat[find_mat(a, NORM, chunk)];
+  const double s = block_sum(norm_chunk<T, MUON>(t, chunk, u), red);
   if (threadIdx.x == 0) partial[t.norm0 + chunk] = s;
 }
 
-// X_0 and its transpose from 64 x 64 tiles of the source, normalised
-template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void ortho_start_kernel(Mats a, MuonArgs u, const double* __restrict__ partial, float eps,
-                                                          float scale) {
-  constexpr int LP = 66;
-  __shared__ float tile[64 * LP];
-  __shared__ double red[16];
-  int local;
-  const Mat& t = a.mat[find_mat(a, blockIdx.x, local)];
-  const int rows = t.flip ? t.n : t.m, cols = t.flip ? t.m : t.n;
-  const int tc = (cols + 63) >> 6, r0 = (local / tc) * 64, c0 = (local % tc) * 64;
-  double s = 0.0;
-  for (int i = threadIdx.x; i < t.normc; i += 256) s += partial[t.norm0 + i];
-  const double norm = sqrt(block_sum(s, red));
-  const float f = (float)((double)scale / (norm < (double)eps ? (double)eps : norm));      // a NaN stays one
-  const T* x = static_cast<const T*>(t.x);
-#pragma unroll 4
-  for (int k = 0; k < 16; ++k) {
-    const int r = k * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
-    float v = 0.f;
-    if (r0 + r < rows && c0 + c < cols) {
-      v = elem(x, (int64_t)(r0 + r) * t.ldx + c0 + c);
-      if (MUON) v = direction(v * u.grad_scale, t.mom[(int64_t)(r0 + r) * cols + c0 + c], u);
-      v *= f;
-    }
-    tile[r * LP + c] = v;
+
+struct __attribute__((packed, aligned(4))) F4 { float f[4]; };
+struct __attribute__((packed, aligned(2))) H8 { unsigned u[4]; };
+
+// eight consecutive elements of any alignment
+__device__ __forceinline__ void read8(const float* p, float (&v)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const F4 w = *reinterpret_cast<const F4*>(p + 4 * h);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[4 * h + e] = w.f[e];
   }
-  __syncthreads();
-  unsigned char* direct = a.ws + (t.flip ? t.Y : t.X);      // rows x up32(cols)
-  unsigned char* across = a.ws + (t.flip ? t.X : t.Y);      // cols x up32(rows)
+}
+__device__ __forceinline__ void read8(const bf16_t* p, float (&v)[8]) {
+  const H8 w = *reinterpret_cast<const H8*>(p);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int id = k * 256 + threadIdx.x;
-    float v[8];
-    const int r = id >> 3, c = (id & 7) * 8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tile[r * LP + c + e];
-    if (r0 + r < rows && c0 + c < up32(cols)) store8(direct + (int64_t)(r0 + r) * up32(cols) * 4, c0 + c, v);
-    const int q = (id >> 2 & 15) + (id >> 7) * 16, p = ((id & 3) + (id >> 6 & 1) * 4) * 8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tile[(p + e) * LP + q];
-    if (c0 + q < cols && r0 + p < up32(rows)) store8(across + (int64_t)(c0 + q) * up32(rows) * 4, r0 + p, v);
+  for (int e = 0; e < 4; ++e) {
+    v[2 * e] = __uint_as_float(w.u[e] << 16);
+    v[2 * e + 1] = __uint_as_float(w.u[e] & 0xffff0000u);
   }
 }
 
+// A 64 x 64 tile of the source, times f, into X: 16-byte reads to 16-byte stores, row by row, or - where X is the
+// transpose - through LDS.
+template <typename T, bool MUON>
+__device__ __forceinline__ void start_tile(const Mat& t, unsigned char* ws, int local, float f, const MuonArgs& u, float* tile) {
+  constexpr int LP = 66;
+  const int rows = t.flip ? t.n : t.m, cols = t.flip ? t.m : t.n;
+  const int tc = (cols + 63) >> 6, r0 = (local / tc) * 64, c0 = (local % tc) * 64;
+  const T* x = static_cast<const T*>(t.x);
+  unsigned char* X = x_of(t, ws, 0);
+  float v[2][8];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = r0 + k * 32 + (threadIdx.x >> 3), c = c0 + (threadIdx.x & 7) * 8;
+    float m[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[k][e] = m[e] = 0.f;
+    if (r < rows) {
+      const T* p = x + (int64_t)r * t.ldx + c;
+      const float* q = MUON ? t.mom + (int64_t)r * cols + c : nullptr;
+      if (c + 8 <= cols) {
+        read8(p, v[k]);
+        if (MUON) read8(q, m);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < cols) {
+            v[k][e] = (float)p[e];
+            if (MUON) m[e] = q[e];
+          }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[k][e] = f * (MUON ? direction(v[k][e] * u.grad_scale, m[e], u) : v[k][e]);
+  }
+  if (!t.flip) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = r0 + k * 32 + (threadIdx.x >> 3), c = c0 + (threadIdx.x & 7) * 8;
+      if (r < rows && c < up32(cols)) store8(X + (int64_t)r * up32(cols) * 4, c, v[k]);
+    }
+    return;
+  }
+  __syncthreads();                    // the previous tile has been read
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tile[(k * 32 + (threadIdx.x >> 3)) * LP + (threadIdx.x & 7) * 8 + e] = v[k][e];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int id = k * 256 + threadIdx.x;
+    float w[8];
+    const int q = (id >> 2 & 15) + (id >> 7) * 16, p = ((id & 3) + (id >> 6 & 1) * 4) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = tile[(p + e) * LP + q];
+    if (c0 + q < cols && r0 + p < up32(rows)) store8(X + (int64_t)(c0 + q) * up32(rows) * 4, r0 + p, w);
+  }
+}
+
+// scale / max(norm, eps): a NaN stays one
+__device__ __forceinline__ float start_factor(double sum, float eps, float scale) {
+  const double norm = sqrt(sum);
+  return (float)((double)scale / (norm < (double)eps ? (double)eps : norm));
+}
+
+// X_0: the matrices, normalised
+template <typename T, bool MUON>
+__global__ __launch_bounds__(256) void ortho_start_kernel(const Mats* __restrict__ a, unsigned char* ws, MuonArgs u,
+                                                          const double* __restrict__ partial, float eps, float scale) {
+  __shared__ float tile[64 * 66];
+  __shared__ double red[16];
+  int local;
+  const Mat& t = a->mat[find_mat(*a, START, local)];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < t.normc; i += 256) s += partial[t.norm0 + i];
+  start_tile<T, MUON>(t, ws, local, start_factor(block_sum(s, red), eps, scale), u, tile);
+}
+
 // ------------------------------------------------------------------------------------------------ products
-// A workgroup of 4 waves (2 x 2), each WT x WT of a T x T tile, T = 2 WT; k advances by 32 through two LDS stages.
-template <int WT>
+// A workgroup of 4 waves (2 x 2), each WT x WT of a T x T tile, T = 2 WT; k advances by 32 through a ring of S stages, of
+// which S - 1 are on their way while one is multiplied.  128 x 128 tiles take two stages of 32 KB, two workgroups to a
+// CU: the other one's products hide the rest of the latency.  64 x 64 tiles, taken where there are few of them, wait for
+// their operands instead: what a CU has in flight over the latency of 0.7 us is their rate, so they take four stages of
+// 16 KB, or eight (DEEP) where a launch has at most one workgroup for a CU anyway.
+template <int WT, bool DEEP = false>
 struct Tile {
-  static constexpr int T = 2 * WT, MR = WT / 16, LP = T + 2;
+  static constexpr int T = 2 * WT, MR = WT / 16, LP = T + 2, S = WT == 64 ? 2 : DEEP ? 8 : 4;
   static constexpr int PIECES = 2 * T / 8, LOADS = PIECES / 4;          // 1 KB LDS-DMA pieces of a stage; per wave
   static constexpr int STAGE = 2 * T * 128;
-  static constexpr int LDS = 2 * STAGE > T * LP * 4 ? 2 * STAGE : T * LP * 4;
+  static constexpr int LDS = S * STAGE > T * LP * 4 ? S * STAGE : T * LP * 4;
 };
 
-// acc[mr][nr] += P rows p0.. x Q rows q0.. over the k-blocks [kb0, kb1); rows past the last are read as the last.
-// Entered and left with the LDS free for anyone's use after a barrier.
-template <int WT>
+typedef __attribute__((ext_vector_type(4))) short short4v;
+
+// acc[mr][nr] += P rows p0.. x Q over the k-blocks [kb0, kb1).  P: M rows of KB blocks.  Q: N rows of KB blocks like it,
+// rows q0..; or, DOWN, K rows of N numbers in QB blocks each, columns q0...  What lies past the last row or block is read
+// as the last one (its results are not stored, and k past the end meets zeros of P).  Entered and left with the LDS free.
+template <int WT, bool DEEP = false, bool DOWN = false>
 __device__ __forceinline__ void product(f32x4 (&acc)[WT / 16][WT / 16], const unsigned char* P, const unsigned char* Q, int p0,
-                                        int q0, int M, int N, int KB, int kb0, int kb1, unsigned char* smem) {
-  using G = Tile<WT>;
-  constexpr int MR = G::MR;
+                                        int q0, int M, int N, int KB, int kb0, int kb1, unsigned char* smem, int K = 0, int QB = 0) {
+  using G = Tile<WT, DEEP>;
+  constexpr int MR = G::MR, HALF = G::LOADS / 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-  // LDS-DMA: piece w + 4 j holds rows 8 (w + 4 j) .. + 7; lane -> row lane >> 3, slot lane & 7, which receives the 16-byte
-  // chunk slot ^ ((row >> 1) & 7), so that the 16 lanes of a fragment read hit distinct banks
+  // LDS-DMA of rows: piece w + 4 j holds rows 8 (w + 4 j) .. + 7; lane -> row lane >> 3, slot lane & 7, which receives the
+  // 16-byte chunk slot ^ ((row >> 1) & 7), so that the 16 lanes of a fragment read hit distinct banks
   const int chunk = (lane & 7) ^ ((4 * (wave & 1) + (lane >> 4)) & 7);
   const unsigned char* src[G::LOADS];
 #pragma unroll
-  for (int j = 0; j < G::LOADS; ++j) {
+  for (int j = 0; j < (DOWN ? HALF : G::LOADS); ++j) {
     const int r = 8 * (wave + 4 * j) + (lane >> 3);
-    const bool isq = j >= G::LOADS / 2;                    // the first half of the pieces is P, the second Q
+    const bool isq = j >= HALF;                            // the first half of the pieces is P, the second Q
     int row = isq ? q0 + r - G::T : p0 + r;
     const int last = (isq ? N : M) - 1;
     if (row > last) row = last;
     src[j] = (isq ? Q : P) + ((int64_t)row * KB + kb0) * 128 + chunk * 16;
   }
-  auto stage = [&](int kb, int buf) {
+  // DOWN: piece w + 4 j of Q is column block j, k-rows 8 w .. 8 w + 7 of the stage.  A transposing read takes 32 bytes from
+  // each of 16 rows 8 g + t (g, t < 4): pairs of chunks trade places by (t >> 1) + 2 (g & 1), so that they meet in twos.
+  const int krow = 8 * wave + (lane >> 3);
+  const int64_t pitch = (int64_t)QB * 128;
+  int down[HALF];
+  if (DOWN) {
+    const int dchunk = (lane & 7) ^ (((lane >> 4 & 1) + 2 * (wave & 1)) << 1);
 #pragma unroll
-    for (int j = 0; j < G::LOADS; ++j) glds16(src[j] + (int64_t)(kb - kb0) * 128, smem + buf * G::STAGE + (wave + 4 * j) * 1024);
+    for (int j = 0; j < HALF; ++j) {
+      const int blk = (q0 >> 5) + j;
+      down[j] = (blk < QB ? blk : QB - 1) * 128 + dchunk * 16;
+    }
+  }
+  const unsigned base = __builtin_amdgcn_readfirstlane(lds_offset(smem)) + wave * 1024;
+  auto stage = [&](int kb, int buf) {
+    const int64_t k128 = (int64_t)(kb - kb0) * 128;
+#pragma unroll
+    for (int j = 0; j < (DOWN ? HALF : G::LOADS); ++j) glds16(src[j] + k128, base + buf * G::STAGE + j * 4096);
+    if (DOWN) {
+      const int k = kb * 32 + krow;
+      const unsigned char* row = Q + (int64_t)(k < K ? k : K - 1) * pitch;
+#pragma unroll
+      for (int j = 0; j < HALF; ++j) glds16(row + down[j], base + buf * G::STAGE + G::T * 128 + j * 4096);
+    }
   };
   int fro[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) fro[h] = (lane & 15) * 128 + (((h * 4 + (lane >> 4)) ^ ((lane >> 1) & 7)) * 16);
-  stage(kb0, 0);
-  int buf = 0;
-  for (int kb = kb0; kb < kb1; ++kb) {
-    if (kb + 1 < kb1) {
-      stage(kb + 1, buf ^ 1);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(G::LOADS) : "memory");       // this stage landed, the next in flight
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
+  // transposing reads: lane -> k-row 8 g + t of the eight 8 g .. (the upper four follow 512 bytes on), four columns 4 c ..
+  int tro[4];      // [half][16-column side of the block]
+  if (DOWN) {
+    const int g = lane >> 4, t = lane >> 2 & 3, c = lane & 3, turn = (t >> 1) + 2 * (g & 1);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) tro[v] = (8 * g + t) * 128 + ((v ^ turn) * 2 + (c >> 1)) * 16 + (c & 1) * 8;
+  }
+  struct Frags { f16x8 ph[MR], pl[MR], qh[MR], ql[MR]; };
+  auto fetch = [&](Frags& f, int buf) {
     const unsigned char* pb = smem + buf * G::STAGE + wm * WT * 128;
     const unsigned char* qb = smem + buf * G::STAGE + (G::T + wn * WT) * 128;
-    f16x8 ph[MR], pl[MR], qh[MR], ql[MR];
+    auto q_of = [&](int r, int half) {
+      if (!DOWN) return *reinterpret_cast<const f16x8*>(qb + r * 2048 + fro[half]);
+      typedef __attribute__((ext_vector_type(8))) short short8v;
+      const unsigned char* at = qb + (r >> 1) * 4096 + tro[half * 2 + (r & 1)];
+      const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)at);
+      const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(at + 512));
+      return __builtin_bit_cast(f16x8, short8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+    };
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
-      ph[r] = *reinterpret_cast<const f16x8*>(pb + r * 2048 + fro[0]);
-      qh[r] = *reinterpret_cast<const f16x8*>(qb + r * 2048 + fro[0]);
+      f.ph[r] = *reinterpret_cast<const f16x8*>(pb + r * 2048 + fro[0]);
+      f.qh[r] = q_of(r, 0);
     }
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
-      pl[r] = *reinterpret_cast<const f16x8*>(pb + r * 2048 + fro[1]);
-      ql[r] = *reinterpret_cast<const f16x8*>(qb + r * 2048 + fro[1]);
+      f.pl[r] = *reinterpret_cast<const f16x8*>(pb + r * 2048 + fro[1]);
+      f.ql[r] = q_of(r, 1);
     }
+  };
+  auto multiply = [&](const Frags& f) {
 #pragma unroll
     for (int i = 0; i < MR; ++i)
 #pragma unroll
-      for (int j = 0; j < MR; ++j) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
-      }
+      for (int j = 0; j < MR; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.ph[i], f.qh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < MR; ++i)
+#pragma unroll
+      for (int j = 0; j < MR; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.ph[i], f.ql[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < MR; ++i)
+#pragma unroll
+      for (int j = 0; j < MR; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.pl[i], f.qh[j], acc[i][j], 0, 0, 0);
+  };
+  // The loop has no branches: the last stages are fetched again where there are no more, so that the number in flight,
+  // and with it every wait, is a constant.
+  const int nk = kb1 - kb0;
+  auto issue = [&](int k) { stage(kb0 + (k < nk ? k : nk - 1), k & (G::S - 1)); };
+  // the oldest stage in flight has landed for every wave, and every wave holds its fragments of the one before
+  auto landed = [&] {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((G::S - 2) * G::LOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();                          // every wave is done with this stage before it is refilled
-    buf ^= 1;
+  };
+  Frags f[2];
+#pragma unroll
+  for (int d = 0; d < G::S - 1; ++d) issue(d);
+  landed();
+  fetch(f[0], 0);
+  issue(G::S - 1);
+  // while stage k is multiplied from registers, the fragments of k + 1 are read and stage k + S is on its way
+  auto step = [&](int k, const Frags& now, Frags& next) {
+    landed();
+    issue(k + G::S);
+    fetch(next, (k + 1) & (G::S - 1));
+    multiply(now);
+    // order: the copies, a first product (its operands are there: no wait), then reads and products in turn
+    __builtin_amdgcn_sched_group_barrier(0x008, MR / 2, 0);
+#pragma unroll
+    for (int q = 0; q < 2 * MR; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, MR / 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, DOWN ? 2 : 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, MR / 2, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int k = 0;
+  for (; k + 2 < nk; k += 2) {
+    step(k, f[0], f[1]);
+    step(k + 1, f[1], f[0]);
   }
+  if (k + 1 < nk) {
+    step(k, f[0], f[1]);
+    multiply(f[1]);
+  } else {
+    multiply(f[0]);
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // the stages are free for other use
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // the accumulators, times f, as a T x LP float tile in LDS; zeros outside M x N
@@ -267,15 +505,24 @@ __device__ __forceinline__ void to_lds(const f32x4 (&acc)[WT / 16][WT / 16], flo
   using G = Tile<WT>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int pr = (wave >> 1) * WT + 4 * (lane >> 4), qc = (wave & 1) * WT + (lane & 15);
+  if (p0 + G::T <= M && q0 + G::T <= N) {
 #pragma unroll
-  for (int i = 0; i < G::MR; ++i)
+    for (int i = 0; i < G::MR; ++i)
 #pragma unroll
-    for (int j = 0; j < G::MR; ++j)
+      for (int j = 0; j < G::MR; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int p = pr + i * 16 + r, q = qc + j * 16;
-        tile[p * G::LP + q] = p0 + p < M && q0 + q < N ? acc[i][j][r] * f : 0.f;
-      }
+        for (int r = 0; r < 4; ++r) tile[(pr + i * 16 + r) * G::LP + qc + j * 16] = acc[i][j][r] * f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < G::MR; ++i)
+#pragma unroll
+      for (int j = 0; j < G::MR; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int p = pr + i * 16 + r, q = qc + j * 16;
+          tile[p * G::LP + q] = p0 + p < M && q0 + q < N ? acc[i][j][r] * f : 0.f;
+        }
+  }
   __syncthreads();
 }
 // f(p, q, v): eight columns q .. q + 7 of row p, for every row and octet of the tile
@@ -316,32 +563,58 @@ __device__ __forceinline__ void clear(f32x4 (&acc)[WT / 16][WT / 16]) {
     for (int j = 0; j < WT / 16; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
-// tile number t of a lower triangle -> (i, j), j <= i
-__device__ __forceinline__ void triangle(int t, int& i, int& j) {
-  i = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-  while ((i + 1) * (i + 2) / 2 <= t) ++i;
-  while (i * (i + 1) / 2 > t) --i;
-  j = t - i * (i + 1) / 2;
+// Tile number t of a lower triangle of nt tiles a side -> (i, j), j <= i, counted through blocks of 4 x 4 tiles: sixteen
+// neighbours read eight rows of tiles, where a row of the triangle would read the whole matrix - in every XCD's L2.
+__device__ __forceinline__ void triangle(int t, int nt, int& i, int& j) {
+  int I = (int)((sqrtf(2.f + 16.f * (float)t) - 1.f) * 0.125f);          // 8 I^2 + 2 I tiles lie before block row I
+  while (8 * (I + 1) * (I + 1) + 2 * (I + 1) <= t) ++I;
+  while (8 * I * I + 2 * I > t) --I;
+  const int rem = t - 8 * I * I - 2 * I, r = nt - 4 * I < 4 ? nt - 4 * I : 4;
+  const int J = rem / (4 * r) < I ? rem / (4 * r) : I;
+  const int at = rem - J * 4 * r;
+  if (J < I) {
+    i = 4 * I + at % r;
+    j = 4 * J + at / r;
+  } else {
+    const int d = at >= 6 ? 3 : at >= 3 ? 2 : at >= 1 ? 1 : 0;
+    i = 4 * I + d;
+    j = 4 * I + at - d * (d + 1) / 2;
+  }
 }
 
-// A = X X^T, one triangle of tiles, stored on both sides of the diagonal.  The contraction over n is split where the tiles
-// alone would not fill the chip: partial tiles go to the workspace as they lie in the accumulators.
+// a tile, times f, into the symmetric matrix D: rows i .. and, off the diagonal, their mirror image
 template <int WT>
-__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Mats a, float f) {
+__device__ __forceinline__ void put_symmetric(const f32x4 (&acc)[WT / 16][WT / 16], float f, const Mat& t, unsigned char* D, int i,
+                                              int j, unsigned char* smem) {
   using G = Tile<WT>;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  int local, i, j;
-  const Mat& t = a.mat[find_mat(a, xcd_order(blockIdx.x, gridDim.x), local)];
+  float* tile = reinterpret_cast<float*>(smem);
+  const int mp = up32(t.m);
+  to_lds<WT>(acc, f, i * G::T, j * G::T, t.m, t.m, tile);
+  by_rows<WT>(tile, [&](int p, int q, const float (&v)[8]) {
+    if (i * G::T + p < t.m && j * G::T + q < mp) store8(D + (int64_t)(i * G::T + p) * mp * 4, j * G::T + q, v);
+  });
+  if (i != j)
+    by_cols<WT>(tile, [&](int q, int p, const float (&v)[8]) {
+      if (j * G::T + q < t.m && i * G::T + p < mp) store8(D + (int64_t)(j * G::T + q) * mp * 4, i * G::T + p, v);
+    });
+}
+
+// A = X X^T in slot 0, one triangle of tiles, stored on both sides of the diagonal.  The contraction over n is split where
+// the tiles alone would not fill the chip: partial tiles go to the workspace as they lie in the accumulators.
+template <int WT>
+__device__ __forceinline__ void gram_tile(const Mat& t, unsigned char* ws, int local, float f, int odd, unsigned char* smem) {
+  using G = Tile<WT>;
   const int nt = (t.m + G::T - 1) / G::T, tiles = nt * (nt + 1) / 2;
   const int split = local / tiles, tl = local % tiles;      // tiles of one split are neighbours: they share its columns of X
-  triangle(tl, i, j);
+  int i, j;
+  triangle(tl, nt, i, j);
   const int KB = up32(t.n) >> 5, kb0 = split * t.kc, kb1 = kb0 + t.kc < KB ? kb0 + t.kc : KB;
-  const unsigned char* X = a.ws + t.X;
+  const unsigned char* X = x_of(t, ws, odd);
   f32x4 acc[G::MR][G::MR];
   clear<WT>(acc);
   product<WT>(acc, X, X, i * G::T, j * G::T, t.m, t.m, KB, kb0, kb1, smem);
   if (t.ks > 1) {
-    f32x4* part = reinterpret_cast<f32x4*>(a.ws + t.part) + (int64_t)(tl * t.ks + split) * (G::T * G::T / 4);
+    f32x4* part = part_of(t, ws) + (int64_t)(tl * t.ks + split) * (G::T * G::T / 4);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int r = 0; r < G::MR; ++r)
@@ -349,35 +622,33 @@ __global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Mats a, float f) {
       for (int c = 0; c < G::MR; ++c) part[((wave * G::MR + r) * G::MR + c) * 64 + lane] = acc[r][c];
     return;
   }
-  float* tile = reinterpret_cast<float*>(smem);
-  to_lds<WT>(acc, f, i * G::T, j * G::T, t.m, t.m, tile);
-  unsigned char* A = a.ws + t.A;
-  const int mp = up32(t.m);
-  by_rows<WT>(tile, [&](int p, int q, const float (&v)[8]) {
-    if (i * G::T + p < t.m && j * G::T + q < mp) store8(A + (int64_t)(i * G::T + p) * mp * 4, j * G::T + q, v);
-  });
-  if (i != j)
-    by_cols<WT>(tile, [&](int q, int p, const float (&v)[8]) {
-      if (j * G::T + q < t.m && i * G::T + p < mp) store8(A + (int64_t)(j * G::T + q) * mp * 4, i * G::T + p, v);
-    });
+  put_symmetric<WT>(acc, f, t, slot_of(t, ws, 0), i, j, smem);
+}
+
+template <int WT>
+__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(const Mats* __restrict__ a, unsigned char* ws, float f, int odd) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  int local;
+  const Mat& t = a->mat[find_mat(*a, GRAM, local)];
+  gram_tile<WT>(t, ws, local, f, odd, smem);
 }
 
 // adds the partial tiles of A, a workgroup per 32 x 32 block, in the order of the splits
 template <int WT>
-__global__ __launch_bounds__(256) void ortho_join_kernel(Mats a, float f) {
+__global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict__ a, unsigned char* ws, float f) {
   using G = Tile<WT>;
   constexpr int B = G::T / 32;
   __shared__ float tile[32 * 34];
   int local, i, j;
-  const Mat& t = a.mat[find_mat(a, blockIdx.x, local)];
+  const Mat& t = a->mat[find_mat(*a, JOIN, local)];
   const int tl = local / (B * B), sub = local % (B * B);
-  triangle(tl, i, j);
+  triangle(tl, (t.m + G::T - 1) / G::T, i, j);
   const int p0 = i * G::T + (sub / B) * 32, q0 = j * G::T + (sub % B) * 32, mp = up32(t.m);
   if (p0 >= mp || q0 >= mp) return;
   // 16 x 16 accumulator blocks (r, c) of the tile's waves that make up this block
   const int r16 = (sub / B) * 2 + (threadIdx.x >> 7), c16 = (sub % B) * 2 + (threadIdx.x >> 6 & 1), lane = threadIdx.x & 63;
   const int wave = (r16 / G::MR) * 2 + c16 / G::MR;
-  const f32x4* part = reinterpret_cast<const f32x4*>(a.ws + t.part) + (int64_t)tl * t.ks * (G::T * G::T / 4) +
+  const f32x4* part = part_of(t, ws) + (int64_t)tl * t.ks * (G::T * G::T / 4) +
                       ((wave * G::MR + r16 % G::MR) * G::MR + c16 % G::MR) * 64 + lane;
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
@@ -386,7 +657,7 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(Mats a, float f) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) tile[(pr + e) * 34 + qc] = p0 + pr + e < t.m && q0 + qc < t.m ? s[e] * f : 0.f;
   __syncthreads();
-  unsigned char* A = a.ws + t.A;
+  unsigned char* A = slot_of(t, ws, 0);
   const int id = threadIdx.x & 127, r = id >> 2, c = (id & 3) * 8;
   float v[8];
   if (threadIdx.x < 128) {
@@ -400,38 +671,70 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(Mats a, float f) {
   }
 }
 
-// B = ca I + cb A + cc A^2 of the stored (scaled) numbers, one triangle of tiles; the host has folded the scales in
-template <int WT>
-__global__ __launch_bounds__(256, 2) void ortho_poly_kernel(Mats a, float ca, float cb, float cc) {
+// The m x m matrices of one group of steps live in slots of the workspace; all are polynomials in A, so they are symmetric
+// and commute, and one triangle of tiles is computed and stored on both sides.
+//   D = ca I + cb C + cc P Q of the stored (scaled) numbers; C is not read where ca and cb are 0.  D is none of the others.
+template <int WT, bool DEEP = false>
+__device__ __forceinline__ void square_tile(const Mat& t, unsigned char* ws, int local, const Op& op, unsigned char* smem) {
   using G = Tile<WT>;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  int local, i, j;
-  const Mat& t = a.mat[find_mat(a, xcd_order(blockIdx.x, gridDim.x), local)];
-  triangle(local, i, j);
+  int i, j;
+  triangle(local, (t.m + G::T - 1) / G::T, i, j);
   const int mp = up32(t.m), KB = mp >> 5;
-  const unsigned char* A = a.ws + t.A;
-  unsigned char* Bm = a.ws + t.A + (int64_t)t.m * mp * 4;
+  const unsigned char* C = slot_of(t, ws, op.sc);
+  unsigned char* D = slot_of(t, ws, op.sd);
   f32x4 acc[G::MR][G::MR];
   clear<WT>(acc);
-  product<WT>(acc, A, A, i * G::T, j * G::T, t.m, t.m, KB, 0, KB, smem);
+  product<WT, DEEP>(acc, slot_of(t, ws, op.sp), slot_of(t, ws, op.sq), i * G::T, j * G::T, t.m, t.m, KB, 0, KB, smem);
+  if (op.ca == 0.f && op.cb == 0.f) {
+    put_symmetric<WT>(acc, op.cc, t, D, i, j, smem);
+    return;
+  }
   float* tile = reinterpret_cast<float*>(smem);
-  to_lds<WT>(acc, cc, i * G::T, j * G::T, t.m, t.m, tile);
+  to_lds<WT>(acc, op.cc, i * G::T, j * G::T, t.m, t.m, tile);
   auto put = [&](int r, int c, const float (&v)[8]) {        // eight numbers of row r from column c on
     if (r >= t.m || c >= mp) return;
     float w[8];
-    load8(A + (int64_t)r * mp * 4, c, w);
+    load8(C + (int64_t)r * mp * 4, c, w);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = v[e] + cb * w[e] + (r == c + e ? ca : 0.f);
-    store8(Bm + (int64_t)r * mp * 4, c, w);
+    for (int e = 0; e < 8; ++e) w[e] = v[e] + op.cb * w[e] + (r == c + e ? op.ca : 0.f);
+    store8(D + (int64_t)r * mp * 4, c, w);
   };
   by_rows<WT>(tile, [&](int p, int q, const float (&v)[8]) { put(i * G::T + p, j * G::T + q, v); });
   if (i != j) by_cols<WT>(tile, [&](int q, int p, const float (&v)[8]) { put(j * G::T + q, i * G::T + p, v); });
 }
 
-// eight consecutive results at (r, c) of the source's orientation, as many as lie within `cols`
+// one or two operations that do not depend on each other: gridDim.y of them
+template <int WT, bool DEEP>
+__global__ __launch_bounds__(256, DEEP ? 1 : 2) void ortho_square_kernel(const Mats* __restrict__ a, unsigned char* ws, Op first, Op second) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  int local;
+  const Mat& t = a->mat[find_mat(*a, SQUARE, local)];
+  square_tile<WT, DEEP>(t, ws, local, blockIdx.y ? second : first, smem);
+}
+
+// eight consecutive results at (r, c) of the source's orientation, as many as lie within `cols`: 16-byte accesses of any
+// alignment, single elements at the row's end
 template <typename T, bool MUON>
 __device__ __forceinline__ void finish8(const Mat& t, int r, int c, int cols, const float (&v)[8], const MuonArgs& u) {
   T* o = static_cast<T*>(t.out) + (int64_t)r * t.ldo + c;
+  if (c + 8 <= cols) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        F4 w;
+        if (MUON) w = *reinterpret_cast<const F4*>(o + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.f[e] = MUON ? w.f[e] * u.decay - t.step * v[4 * h + e] : v[4 * h + e];
+        *reinterpret_cast<F4*>(o + 4 * h) = w;
+      }
+    } else {
+      H8 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w.u[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+      *reinterpret_cast<H8*>(o) = w;
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     if (c + e < cols) {
@@ -440,42 +743,403 @@ __device__ __forceinline__ void finish8(const Mat& t, int r, int c, int cols, co
     }
 }
 
-// Y' = Y B (= (B X)^T): the next step's Y and X, or the result
+// Q X with Q from slot sq: the next group's X, or the result.  Tiles of a column panel of X are neighbours.
 template <int WT, typename T, bool LAST, bool MUON>
-__global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Mats a, MuonArgs u, float f, int odd) {
+__device__ __forceinline__ void apply_tile(const Mat& t, unsigned char* ws, int local, const MuonArgs& u, int sq, float f, int odd,
+                                           unsigned char* smem) {
   using G = Tile<WT>;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  int local;
-  const Mat& t = a.mat[find_mat(a, xcd_order(blockIdx.x, gridDim.x), local)];
-  const int mp = up32(t.m), np = up32(t.n), KB = mp >> 5;
-  const int tq = (t.m + G::T - 1) / G::T, p0 = (local / tq) * G::T, q0 = (local % tq) * G::T;
-  const int64_t ysz = (int64_t)t.n * mp * 4;
-  const unsigned char* Yin = a.ws + t.Y + (odd ? ysz : 0);
-  unsigned char* Yout = a.ws + t.Y + (odd ? 0 : ysz);
-  const unsigned char* Bm = a.ws + t.A + (int64_t)t.m * mp * 4;
+  const int np = up32(t.n), KB = up32(t.m) >> 5;
+  const int tp = (t.m + G::T - 1) / G::T, p0 = (local % tp) * G::T, q0 = (local / tp) * G::T;
   f32x4 acc[G::MR][G::MR];
   clear<WT>(acc);
-  product<WT>(acc, Yin, Bm, p0, q0, t.n, t.m, KB, 0, KB, smem);
+  product<WT, false, true>(acc, slot_of(t, ws, sq), x_of(t, ws, odd), p0, q0, t.m, t.n, KB, 0, KB, smem, t.m, np >> 5);
   float* tile = reinterpret_cast<float*>(smem);
-  to_lds<WT>(acc, f, p0, q0, t.n, t.m, tile);
+  to_lds<WT>(acc, f, p0, q0, t.m, t.n, tile);
   if (LAST) {
-    if (t.flip)
+    if (!t.flip)
       by_rows<WT>(tile, [&](int p, int q, const float (&v)[8]) {
-        if (p0 + p < t.n && q0 + q < t.m) finish8<T, MUON>(t, p0 + p, q0 + q, t.m, v, u);
+        if (p0 + p < t.m && q0 + q < t.n) finish8<T, MUON>(t, p0 + p, q0 + q, t.n, v, u);
       });
     else
       by_cols<WT>(tile, [&](int q, int p, const float (&v)[8]) {
-        if (q0 + q < t.m && p0 + p < t.n) finish8<T, MUON>(t, q0 + q, p0 + p, t.n, v, u);
+        if (q0 + q < t.n && p0 + p < t.m) finish8<T, MUON>(t, q0 + q, p0 + p, t.m, v, u);
       });
     return;
   }
+  unsigned char* X = x_of(t, ws, odd ^ 1);
   by_rows<WT>(tile, [&](int p, int q, const float (&v)[8]) {
-    if (p0 + p < t.n && q0 + q < mp) store8(Yout + (int64_t)(p0 + p) * mp * 4, q0 + q, v);
+    if (p0 + p < t.m && q0 + q < np) store8(X + (int64_t)(p0 + p) * np * 4, q0 + q, v);
   });
-  unsigned char* X = a.ws + t.X;
-  by_cols<WT>(tile, [&](int q, int p, const float (&v)[8]) {
-    if (q0 + q < t.m && p0 + p < np) store8(X + (int64_t)(q0 + q) * np * 4, p0 + p, v);
-  });
+}
+
+template <int WT, typename T, bool LAST, bool MUON>
+__global__ __launch_bounds__(256, 2) void ortho_apply_kernel(const Mats* __restrict__ a, unsigned char* ws, MuonArgs u, int sq, float f,
+                                                             int odd) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  int local;
+  const Mat& t = a->mat[find_mat(*a, APPLY, local)];
+  apply_tile<WT, T, LAST, MUON>(t, ws, local, u, sq, f, odd, smem);
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// What one workgroup wrote to the workspace is there for all its waves: its stores have left, and its CU has one L1.
+__device__ __forceinline__ void phase_done() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// a value that lies in LDS, the same for all lanes, in scalar registers
+template <typename V>
+__device__ __forceinline__ V uniform(const V* p) {
+  static_assert(sizeof(V) % 4 == 0, "whole words");
+  union { V v; int w[sizeof(V) / 4]; } u;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(V) / 4); ++i) u.w[i] = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(p)[i]);
+  return u.v;
+}
+// kernel arguments into LDS, all at once
+template <typename V>
+__device__ __forceinline__ void keep(V* lds, const V& arg) {
+  for (int i = threadIdx.x; i < (int)(sizeof(V) / 4); i += 256) reinterpret_cast<int*>(lds)[i] = reinterpret_cast<const int*>(&arg)[i];
+}
+
+// the sum of a matrix's partial tiles of A, in the order of the splits
+template <int WT>
+__device__ __forceinline__ void add_parts(f32x4 (&acc)[WT / 16][WT / 16], const Mat& t, unsigned char* ws) {
+  using G = Tile<WT>;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const f32x4* part = part_of(t, ws);
+  clear<WT>(acc);
+  for (int k = 0; k < t.ks; ++k)
+#pragma unroll
+    for (int r = 0; r < G::MR; ++r)
+#pragma unroll
+      for (int c = 0; c < G::MR; ++c)
+        acc[r][c] += part[(int64_t)k * (G::T * G::T / 4) + ((wave * G::MR + r) * G::MR + c) * 64 + lane];
+}
+
+// The m x m operations of a group for matrices of 65 to 128 rows, a workgroup each, instead of a launch for every operation;
+// the partial tiles of A are added up on the way.
+__global__ __launch_bounds__(256) void ortho_chain128_kernel(const Mats* __restrict__ a, unsigned char* ws, float f, Program prog) {
+  using G = Tile<64>;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ Program kept;
+  keep(&kept, prog);
+  const Mat& t = a->mat[blockIdx.x];
+  __syncthreads();
+  if (t.ks > 1) {
+    f32x4 acc[G::MR][G::MR];
+    add_parts<64>(acc, t, ws);
+    put_symmetric<64>(acc, f, t, slot_of(t, ws, 0), 0, 0, smem);
+    phase_done();
+  }
+  for (int k = 0; k < prog.n; ++k) {
+    square_tile<64>(t, ws, 0, uniform(&kept.op[k]), smem);
+    phase_done();
+  }
+}
+
+// Up to 64 rows the m x m matrices stay in LDS, 16 KB each: slot k, 32-column block b, row r, 16-byte chunks as in the
+// stages of product().  A workgroup computes the whole 64 x 64 product, and a lane's four rows of one column are, by
+// symmetry, four columns of one row: they go back without any transposition.  An operation takes 0.4 us this way,
+// 2.7 us through global memory.
+constexpr int SLOT64 = 64 * 2 * 128;
+
+struct Lane64 {
+  int wm, wn, r, g, fro[2];
+  int at[2][2];      // byte of this lane's four numbers of accumulator (i, j = 0), [i][half], within a slot; j adds 2048
+  __device__ __forceinline__ Lane64() {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), turn = (lane >> 1) & 7;
+    wm = wave >> 1; wn = wave & 1; r = lane & 15; g = lane >> 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      fro[h] = r * 128 + (((h * 4 + g) ^ turn) * 16);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        at[i][h] = wm * 8192 + wn * 4096 + r * 128 + (((i * 2 + (g >> 1)) + 4 * h) ^ turn) * 16 + (g & 1) * 8;
+    }
+  }
+};
+
+// D = ca I + cb C + cc acc into slot D.  What lies outside m x m is zero in C and in acc, and stays zero.
+__device__ __forceinline__ void put64(const f32x4 (&acc)[2][2], float ca, float cb, float cc, int m, unsigned char* D,
+                                      const unsigned char* C, const Lane64& L) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = cc * acc[i][j][e];
+      f16x4 hi, lo;
+      if (cb != 0.f) {
+        hi = *reinterpret_cast<const f16x4*>(C + L.at[i][0] + j * 2048);
+        lo = *reinterpret_cast<const f16x4*>(C + L.at[i][1] + j * 2048);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = fmaf((float)lo[e], cb, fmaf((float)hi[e], cb, v[e]));
+      }
+      const int c = L.wm * 32 + i * 16 + 4 * L.g, r = L.wn * 32 + j * 16 + L.r;
+      if (ca != 0.f && L.wm == L.wn && i == j) {         // a block on the diagonal
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += r == c + e && r < m ? ca : 0.f;
+      }
+      split4(v, hi, lo);
+      *reinterpret_cast<f16x4*>(D + L.at[i][0] + j * 2048) = hi;
+      *reinterpret_cast<f16x4*>(D + L.at[i][1] + j * 2048) = lo;
+    }
+}
+__device__ __forceinline__ void lds_done() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+// acc += P Q^T over nb 32-column blocks of two matrices of 64 rows in LDS
+__device__ __forceinline__ void product64(f32x4 (&acc)[2][2], const unsigned char* P, const unsigned char* Q, int nb, const Lane64& L) {
+  P += L.wm * 4096;
+  Q += L.wn * 4096;
+  for (int b = 0; b < nb; ++b) {
+    f16x8 p[2][2], q[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        p[h][i] = *reinterpret_cast<const f16x8*>(P + b * 8192 + i * 2048 + L.fro[h]);
+        q[h][i] = *reinterpret_cast<const f16x8*>(Q + b * 8192 + i * 2048 + L.fro[h]);
+      }
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[w == 2][i], q[w == 1][j], acc[i][j], 0, 0, 0);
+  }
+}
+__device__ __forceinline__ void square64(const Op& op, int m, unsigned char* slots, const Lane64& L) {
+  f32x4 acc[2][2];
+  clear<32>(acc);
+  product64(acc, slots + op.sp * SLOT64, slots + op.sq * SLOT64, up32(m) >> 5, L);
+  put64(acc, op.ca, op.cb, op.cc, m, slots + op.sd * SLOT64, slots + op.sc * SLOT64, L);
+  lds_done();
+}
+
+// The m x m operations of a group for matrices of up to 64 rows; the last slot written is Q, which goes to global memory.
+__global__ __launch_bounds__(256) void ortho_chain64_kernel(const Mats* __restrict__ a, unsigned char* ws, float f, Program prog) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ Program kept;
+  keep(&kept, prog);
+  const Mat& t = a->mat[blockIdx.x];
+  const Lane64 L;
+  const int m = t.m, nb = up32(m) >> 5;
+  unsigned char* A = slot_of(t, ws, 0);
+  if (t.ks > 1) {
+    f32x4 acc[2][2];
+    add_parts<32>(acc, t, ws);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)      // rows past the last repeat it in the partial tiles
+          if (L.wm * 32 + i * 16 + 4 * L.g + e >= m || L.wn * 32 + j * 16 + L.r >= m) acc[i][j][e] = 0.f;
+    put64(acc, 0.f, 0.f, f, m, smem, smem, L);
+  } else {
+    for (int id = threadIdx.x; id < 64 * nb * 8; id += 256) {
+      const int r = id / (nb * 8), b = (id >> 3) % nb, c = id & 7;
+      const uint4 v = r < m ? *reinterpret_cast<const uint4*>(A + ((int64_t)r * nb + b) * 128 + c * 16) : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(smem + b * 8192 + r * 128 + (c ^ ((r >> 1) & 7)) * 16) = v;
+    }
+  }
+  __syncthreads();
+  int last = 0;
+  for (int k = 0; k < prog.n; ++k) {
+    const Op op = uniform(&kept.op[k]);
+    square64(op, m, smem, L);
+    last = op.sd;
+  }
+  unsigned char* Q = slot_of(t, ws, last);
+  for (int id = threadIdx.x; id < m * nb * 8; id += 256) {
+    const int r = id / (nb * 8), b = (id >> 3) % nb, c = id & 7;
+    *reinterpret_cast<uint4*>(Q + ((int64_t)r * nb + b) * 128 + c * 16) =
+        *reinterpret_cast<const uint4*>(smem + last * SLOT64 + b * 8192 + r * 128 + (c ^ ((r >> 1) & 7)) * 16);
+  }
+}
+
+// The whole call for small matrices, a workgroup each and a single launch: here the time of a launch, and of the latencies
+// behind it, is all there is to save.  X lives in LDS too, as 32-column blocks of 64 rows in the layout of the slots; Q X
+// replaces it 64 columns at a time, each depending on themselves only.
+constexpr int SMALL_N = 192, SMALL_LDS = (SLOTS + SMALL_N / 64) * SLOT64;
+
+// columns 64 c .. of X <- f Q X, or the result.  The operands trade sides, D[j][i] = sum_k X[k][j] Q[i][k]: a lane then has
+// four columns of one row of the result.
+template <typename T, bool MUON>
+__device__ __forceinline__ void apply64(const Mat& t, unsigned char* X, const unsigned char* Q, int c, float f, bool last,
+                                        const MuonArgs& u, const Lane64& L) {
+  const int lane = threadIdx.x & 63, m = t.m, n = t.n, nb = up32(m) >> 5, KB = up32(n) >> 5;
+  X += c * SLOT64;
+  // transposing reads: k-row 8 g + t (+ 4), columns 4 q ..; the chunk a row holds them in: base ^ 4 half ^ 2 (side ^ upper four)
+  const int tt = lane >> 2 & 3, cq = lane & 3, base = (cq >> 1) ^ (4 * (L.g & 1) + (tt >> 1));
+  const unsigned char* row = X + (2 * c + L.wm < KB ? L.wm : 0) * 8192 + (8 * L.g + tt) * 128 + (cq & 1) * 8;
+  f32x4 acc[2][2];
+  clear<32>(acc);
+  for (int b = 0; b < nb; ++b) {
+    f16x8 x[2][2], q[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        typedef __attribute__((ext_vector_type(8))) short short8v;
+        const unsigned char* at = row + b * 4096;
+        const short4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) short4v*)(at + (base ^ (4 * h) ^ (2 * i)) * 16));
+        const short4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) short4v*)(at + 512 + (base ^ (4 * h) ^ (2 * (i ^ 1))) * 16));
+        x[h][i] = __builtin_bit_cast(f16x8, short8v{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]});
+        q[h][i] = *reinterpret_cast<const f16x8*>(Q + b * 8192 + L.wn * 4096 + i * 2048 + L.fro[h]);
+      }
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[w == 2][i], q[w == 1][j], acc[i][j], 0, 0, 0);
+  }
+  if (2 * c + L.wm >= KB) return lds_done();                  // this wave's block lies past the end
+  if (!last) {
+    lds_done();                                               // every wave has read the old columns
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float v[4];
+        f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f;
+        split4(v, hi, lo);
+        *reinterpret_cast<f16x4*>(X + L.at[i][0] + j * 2048) = hi;
+        *reinterpret_cast<f16x4*>(X + L.at[i][1] + j * 2048) = lo;
+      }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int col = c * 64 + L.wm * 32 + i * 16 + 4 * L.g, r = L.wn * 32 + j * 16 + L.r;
+      if (r >= m) continue;
+      T* o = static_cast<T*>(t.out) + (t.flip ? (int64_t)col * t.ldo + r : (int64_t)r * t.ldo + col);
+      const int64_t next = t.flip ? t.ldo : 1;
+      float old[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) old[e] = MUON && col + e < n ? (float)o[e * next] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = acc[i][j][e] * f;
+        if (col + e < n) o[e * next] = MUON ? (T)(old[e] * u.decay - t.step * v) : (T)v;
+      }
+    }
+  lds_done();
+}
+
+template <typename T, bool MUON>
+__global__ __launch_bounds__(256) void ortho_small_kernel(Mats a, MuonArgs u, float eps, float scale, Program prog) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ double red[16];
+  __shared__ Program kept;
+  __shared__ Mat mine;
+  keep(&kept, prog);
+  keep(&mine, a.mat[blockIdx.x]);
+  __syncthreads();
+  const Mat t = uniform(&mine);
+  unsigned char* X = smem + SLOTS * SLOT64;
+  const Lane64 L;
+  const int m = t.m, n = t.n, KB = up32(n) >> 5;
+  // the matrix, eight elements at a time, stays in registers until its norm is known
+  constexpr int MOST = 64 * SMALL_N / 8 / 256;
+  const int rows = t.flip ? n : m, cols = t.flip ? m : n, c8 = (cols + 7) >> 3, chunks = rows * c8;
+  const T* x = static_cast<const T*>(t.x);
+  float v[MOST][8];
+#pragma unroll
+  for (int k = 0; k < MOST; ++k) {
+    const int id = k * 256 + threadIdx.x, r = id / c8, c = (id - r * c8) * 8;
+    float mo[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[k][e] = mo[e] = 0.f;
+    if (id < chunks) {
+      const T* p = x + (int64_t)r * t.ldx + c;
+      float* q = MUON ? t.mom + (int64_t)r * cols + c : nullptr;
+      if (c + 8 <= cols) {
+        read8(p, v[k]);
+        if (MUON) read8(q, mo);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < cols) {
+            v[k][e] = (float)p[e];
+            if (MUON) mo[e] = q[e];
+          }
+      }
+      if (MUON) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[k][e] *= u.grad_scale;
+          mo[e] = u.momentum * mo[e] + (1.f - u.momentum) * v[k][e];
+          if (c + e < cols) q[e] = mo[e];
+          v[k][e] = direction(v[k][e], mo[e], u);
+        }
+      }
+    }
+  }
+  double s = 0.0;
+#pragma unroll
+  for (int k = 0; k < MOST; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (double)v[k][e] * (double)v[k][e];
+  const float f = start_factor(block_sum(s, red), eps, scale);
+  for (int i = threadIdx.x; i < KB * 512; i += 256) reinterpret_cast<uint4*>(X)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < MOST; ++k) {
+    const int id = k * 256 + threadIdx.x, r = id / c8, c = (id - r * c8) * 8;
+    if (id >= chunks) continue;
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = v[k][e] * f;
+    uint4 hi, lo;
+    split8(w, hi, lo);
+    if (!t.flip) {      // row r, columns c ..: two chunks of 16 bytes (zeros past the end)
+      unsigned char* p = X + (c >> 5) * 8192 + r * 128;
+      const int turn = (r >> 1) & 7, q = (c & 31) >> 3;
+      *reinterpret_cast<uint4*>(p + (q ^ turn) * 16) = hi;
+      *reinterpret_cast<uint4*>(p + ((q + 4) ^ turn) * 16) = lo;
+    } else {            // rows c .., column r
+      const unsigned hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < cols) {
+          unsigned char* p = X + (r >> 5) * 8192 + (c + e) * 128 + (r & 7) * 2;
+          const int turn = ((c + e) >> 1) & 7, q = (r & 31) >> 3;
+          *reinterpret_cast<unsigned short*>(p + (q ^ turn) * 16) = (unsigned short)(hs[e >> 1] >> (16 * (e & 1)));
+          *reinterpret_cast<unsigned short*>(p + ((q + 4) ^ turn) * 16) = (unsigned short)(ls[e >> 1] >> (16 * (e & 1)));
+        }
+    }
+  }
+  __syncthreads();
+  const int ops = uniform(&kept.n);
+  for (int k = 0; k < ops; ++k) {
+    const Op op = uniform(&kept.op[k]);
+    if (op.kind == K_GRAM) {
+      f32x4 acc[2][2];
+      clear<32>(acc);
+      product64(acc, X, X, KB, L);
+      put64(acc, 0.f, 0.f, op.cc, m, smem, smem, L);
+      lds_done();
+    } else if (op.kind == K_SQUARE) {
+      square64(op, m, smem, L);
+    } else {
+      for (int c = 0; c * 64 < n; ++c) apply64<T, MUON>(t, X, smem + op.sq * SLOT64, c, op.cc, op.last, u, L);
+      lds_done();
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -483,9 +1147,9 @@ constexpr int MAX_STEPS = 32;
 
 // Powers of two for the stored numbers of each step, from bounds on the spectral norms: |X_0| <= 1, and over singular values
 // s in [0, r] the next bound is max |s p(s^2)| with p(l) = a + b l + c l^2; A's numbers are within r^2, B's within max |p|.
-struct Scales { float x[MAX_STEPS + 1], a[MAX_STEPS], b[MAX_STEPS]; };
+struct Scales { double x[MAX_STEPS + 1], a[MAX_STEPS], pa[MAX_STEPS], p[MAX_STEPS], pmax[MAX_STEPS]; };
 
-float pow2_for(double bound) { return (float)ldexp(1.0, (int)floor(log2(60000.0 / bound))); }
+double pow2_for(double bound) { return ldexp(1.0, (int)floor(log2(60000.0 / bound))); }
 
 bool ortho_scales(const float* coeff, int steps, Scales* s) {
   double r = 1.0;
@@ -495,87 +1159,118 @@ bool ortho_scales(const float* coeff, int steps, Scales* s) {
     s->x[k] = pow2_for(r);
     if (k == steps) break;
     const double a = coeff[3 * k], b = coeff[3 * k + 1], c = coeff[3 * k + 2];
-    double pm = 1e-3, xm = 0.0;
-    for (int i = 0; i <= 4096; ++i) {
-      const double v = r * i / 4096.0, p = a + b * v * v + c * v * v * v * v;
-      if (!(fabs(p) < 1e9)) return false;
-      if (fabs(p) > pm) pm = fabs(p);
-      if (fabs(v * p) > xm) xm = fabs(v * p);
-    }
+    // p(l), s p(s^2) and l p(l) over l = s^2 in [0, r^2]: the ends, and where their derivatives vanish
+    double pm = 1e-3, xm = 0.0, am = 1e-3;
+    auto look = [&](double l) {
+      if (!(l >= 0.0 && l <= r * r)) return;
+      const double p = fabs(a + b * l + c * l * l);
+      pm = fmax(pm, p);
+      xm = fmax(xm, sqrt(l) * p);
+      am = fmax(am, l * p);
+    };
+    auto roots = [&](double q, double h, double w) {       // q l^2 + h l + w = 0
+      if (q == 0.0) {
+        if (h != 0.0) look(-w / h);
+        return;
+      }
+      const double d = h * h - 4.0 * q * w;
+      if (d < 0.0) return;
+      look((-h + sqrt(d)) / (2.0 * q));
+      look((-h - sqrt(d)) / (2.0 * q));
+    };
+    if (!(fabs(a) + fabs(b) + fabs(c) < 1e6)) return false;
+    look(0.0);
+    look(r * r);
+    roots(0.0, 2.0 * c, b);
+    roots(5.0 * c, 3.0 * b, a);
+    roots(3.0 * c, 2.0 * b, a);
+    if (!(pm <= 4096.0)) return false;
+    s->pmax[k] = pm * 1.01;
     s->a[k] = pow2_for(r * r);
-    s->b[k] = pow2_for(pm * 1.01);
-    if (pm > 4096.0) return false;
+    s->pa[k] = pow2_for(am * 1.01);
+    s->p[k] = pow2_for(s->pmax[k]);
     r = xm * 1.01;
   }
   return true;
 }
 
+// How a call is run.  GENERAL: every product a launch over all its tiles.  CHAIN (all m <= 128): one launch for the m x m
+// products of a group.  SMALL: one launch for everything.
+enum Mode { GENERAL, CHAIN, SMALL };
+
 struct Plan {
-  int wg, wp, wa;              // wave tiles of the three products: 64 or 32
-  int64_t bytes;
-  int norms;
-  bool split;
+  Mode mode;
+  int wg, wp, wa;              // wave tiles of the three kinds of products: 64 or 32
+  int group;                   // steps taken together
+  int64_t bytes, norms;        // of the workspace; where the partial sums of squares begin
 };
 
 int tri(int m, int T) { const int n = cdiv(m, T); return n * (n + 1) / 2; }
 
-// Places the workspace and chooses tiles and splits.  128 x 128 tiles read each operand half as often as 64 x 64 ones, but
-// need 256 of them to give every CU one.
-int make_plan(Mats& a, Plan& p) {
-  int64_t poly = 0, apply = 0, work = 0;
-  int mmax = 0;
+// Places the workspace, chooses mode, tiles and splits, and counts workgroups.
+//
+// Steps in groups: with A = X X^T a step multiplies X by P = a I + b A + c A^2, and the next A is P A P.  Two steps then cost
+// one product each way with X and five with m x m matrices instead of two each way and two; three steps 1 + 1 and nine.
+// That pays where n >= 2 m.  Its price is rounding: A is not taken anew from X, so directions far below the largest lose
+// digits.  Measured against float64 on 12 kinds of spectra, 64 x 126 to 1024 x 9216, the error of groups of two stays within
+// 0.6 to 1.9 of what float32 products of single steps have (median 1.0), of groups of three within 0.6 to 3.9, but within
+// 1.0 from m = 512 on, where long float32 sums dominate; groups of five lose up to 100 times.  So: three from m = 512
+// on and for results that carry less (bfloat16; an update added to a parameter), else two.
+void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
+  int64_t apply = 0, poly = 0;
+  double long_ops = 0.0, square_ops = 0.0;
+  int mmax = 0, mmin = 1 << 30, nmax = 0;
   for (int i = 0; i < a.count; ++i) {
     const Mat& t = a.mat[i];
     poly += tri(t.m, 128);
     apply += (int64_t)cdiv(t.m, 128) * cdiv(t.n, 128);
-    if (t.m > mmax) mmax = t.m;
+    mmax = t.m > mmax ? t.m : mmax;
+    mmin = t.m < mmin ? t.m : mmin;
+    nmax = t.n > nmax ? t.n : nmax;
+    square_ops += (double)t.m * t.m * t.m;
+    long_ops += (double)t.m * t.m * t.n;
   }
+  p.group = long_ops < 2.0 * square_ops ? 1 : coarse || mmin >= 512 ? 3 : 2;
+  p.mode = GENERAL;
+  if (steps <= 6) {
+    if (mmax <= 64 && nmax <= SMALL_N) p.mode = SMALL;
+    else if (mmax <= 128) p.mode = CHAIN;
+  }
+  // 128 x 128 tiles read each operand half as often as 64 x 64 ones, but need 256 of them to give every CU one
   p.wg = mmax > 64 ? 64 : 32;
-  p.wp = poly >= 256 ? 64 : 32;
+  p.wp = p.mode == CHAIN ? p.wg : poly >= 256 ? 64 : 32;
   p.wa = apply >= 256 ? 64 : 32;
   const int T = 2 * p.wg;
+  int64_t work = 0;
   for (int i = 0; i < a.count; ++i) work += (int64_t)tri(a.mat[i].m, T) * (up32(a.mat[i].n) >> 5);
-  // k-blocks per workgroup so that 512 of them, two per CU, share the whole contraction evenly; at least 8
+  // k-blocks per workgroup so that 512 of them, two per CU, share the whole contraction evenly; at least 8.  A chain adds
+  // the partial tiles by itself: at most eight of them.
   int64_t kc = cdiv64(work, 512);
   if (kc < 8) kc = 8;
-  int64_t off = 0;
-  auto take = [&](int64_t bytes) {
-    const int64_t at = off;
-    off += (bytes + 255) & ~(int64_t)255;
-    return at;
-  };
-  p.norms = 0;
-  p.split = false;
+  int64_t off = (sizeof(Mats) + 255) & ~(int64_t)255;
+  int norms = 0;
   for (int i = 0; i < a.count; ++i) {
     Mat& t = a.mat[i];
-    const int64_t mp = up32(t.m), np = up32(t.n), KB = np >> 5;
+    const int64_t KB = up32(t.n) >> 5;
     t.normc = (int)cdiv64((int64_t)t.m * t.n, NORM_CHUNK);
-    t.norm0 = p.norms;
-    p.norms += t.normc;
-    t.X = take(t.m * np * 4);
-    t.Y = take(2 * t.n * mp * 4);
-    t.A = take(2 * t.m * mp * 4);
-    t.kc = (int)(kc < KB ? kc : KB);
+    t.norm0 = norms;
+    norms += t.normc;
+    int64_t k = kc;
+    if (p.mode == CHAIN && k < cdiv64(KB, 8)) k = cdiv64(KB, 8);
+    t.kc = (int)(p.mode == SMALL || k > KB ? KB : k);
     t.ks = (int)cdiv64(KB, t.kc);
-    t.part = 0;
-    if (t.ks > 1) {
-      t.part = take((int64_t)tri(t.m, T) * t.ks * T * T * 4);
-      p.split = true;
-    }
+    t.at = off;
+    off += 2 * size_x(t) + SLOTS * size_slot(t);
+    if (t.ks > 1) off += (int64_t)tri(t.m, T) * t.ks * T * T * 4;
+    off = (off + 255) & ~(int64_t)255;
+    const int B = T / 32;
+    const int64_t n[PHASES] = {t.normc, (int64_t)cdiv(t.m, 64) * cdiv(t.n, 64), (int64_t)tri(t.m, T) * t.ks,
+                               t.ks > 1 ? (int64_t)tri(t.m, T) * B * B : 0, tri(t.m, 2 * p.wp),
+                               (int64_t)cdiv(t.m, 2 * p.wa) * cdiv(t.n, 2 * p.wa)};
+    for (int k2 = 0; k2 < PHASES; ++k2) a.end[k2][i] = (int)n[k2] + (i ? a.end[k2][i - 1] : 0);
   }
-  p.bytes = off + 8 * (int64_t)p.norms;
-  return SNWS_OK;
-}
-
-// grid of a launch: f(mat) workgroups per matrix
-template <typename F>
-unsigned grid_of(Mats& a, F&& f) {
-  int64_t n = 0;
-  for (int i = 0; i < a.count; ++i) {
-    n += f(a.mat[i]);
-    a.end[i] = (int)n;
-  }
-  return (unsigned)n;
+  p.norms = off;
+  p.bytes = off + 8 * (int64_t)norms;
 }
 
 // one instance per kernel, so that each has its own flag
@@ -599,64 +1294,145 @@ int ready(int bytes, const char* what) {
     if (rc__ != SNWS_OK) return rc__;      \
   } while (0)
 
-template <int WT>
-int run_gram(Mats& a, const Plan& p, float f, const char* what, hipStream_t st) {
-  ORTHO_TRY((ready<&ortho_gram_kernel<WT>>(Tile<WT>::LDS, what)));
-  const unsigned grid = grid_of(a, [](const Mat& t) { return (int64_t)tri(t.m, 2 * WT) * t.ks; });
-  ortho_gram_kernel<WT><<<grid, 256, Tile<WT>::LDS, st>>>(a, f);
-  SNWS_LAUNCH_CHECK(what);
-  if (p.split) {
-    constexpr int B = 2 * WT / 32;
-    const unsigned blocks = grid_of(a, [](const Mat& t) { return t.ks > 1 ? (int64_t)tri(t.m, 2 * WT) * B * B : 0; });
-    ortho_join_kernel<WT><<<blocks, 256, 0, st>>>(a, f);
+// A call in flight: the copy of the matrices in the workspace, grid sizes and the stream
+struct Run {
+  const Mats& a;
+  const Plan& p;
+  const MuonArgs& u;
+  const char* what;
+  hipStream_t st;
+  unsigned grid(Phase k) const { return (unsigned)a.end[k][a.count - 1]; }
+  const Mats* table() const { return reinterpret_cast<const Mats*>(a.ws); }
+
+  template <int WT>
+  int gram(float f, int odd) const {
+    ORTHO_TRY((ready<&ortho_gram_kernel<WT>>(Tile<WT>::LDS, what)));
+    ortho_gram_kernel<WT><<<grid(GRAM), 256, Tile<WT>::LDS, st>>>(table(), a.ws, f, odd);
     SNWS_LAUNCH_CHECK(what);
+    if (p.mode == GENERAL && grid(JOIN)) {
+      ortho_join_kernel<WT><<<grid(JOIN), 256, 0, st>>>(table(), a.ws, f);
+      SNWS_LAUNCH_CHECK(what);
+    }
+    return SNWS_OK;
   }
-  return SNWS_OK;
-}
+  template <int WT, bool DEEP>
+  int squares(const Op& first, const Op* second) const {
+    ORTHO_TRY((ready<&ortho_square_kernel<WT, DEEP>>(Tile<WT, DEEP>::LDS, what)));
+    ortho_square_kernel<WT, DEEP><<<dim3(grid(SQUARE), second ? 2 : 1), 256, Tile<WT, DEEP>::LDS, st>>>(table(), a.ws, first,
+                                                                                                     second ? *second : first);
+    SNWS_LAUNCH_CHECK(what);
+    return SNWS_OK;
+  }
+  int chain(float f, const Program& prog) const {
+    if (p.wg == 64) {
+      ORTHO_TRY((ready<&ortho_chain128_kernel>(Tile<64>::LDS, what)));
+      ortho_chain128_kernel<<<(unsigned)a.count, 256, Tile<64>::LDS, st>>>(table(), a.ws, f, prog);
+    } else {
+      ORTHO_TRY((ready<&ortho_chain64_kernel>(SLOTS * SLOT64, what)));
+      ortho_chain64_kernel<<<(unsigned)a.count, 256, SLOTS * SLOT64, st>>>(table(), a.ws, f, prog);
+    }
+    SNWS_LAUNCH_CHECK(what);
+    return SNWS_OK;
+  }
+  template <int WT, typename T, bool LAST, bool MUON>
+  int apply(const Op& op, int odd) const {
+    ORTHO_TRY((ready<&ortho_apply_kernel<WT, T, LAST, MUON>>(Tile<WT>::LDS, what)));
+    ortho_apply_kernel<WT, T, LAST, MUON><<<grid(APPLY), 256, Tile<WT>::LDS, st>>>(table(), a.ws, u, op.sq, op.cc, odd);
+    SNWS_LAUNCH_CHECK(what);
+    return SNWS_OK;
+  }
+  template <typename T, bool MUON>
+  int small(const Program& prog, float eps, float scale) const {
+    ORTHO_TRY((ready<&ortho_small_kernel<T, MUON>>(SMALL_LDS, what)));
+    ortho_small_kernel<T, MUON><<<(unsigned)a.count, 256, SMALL_LDS, st>>>(a, u, eps, scale, prog);
+    SNWS_LAUNCH_CHECK(what);
+    return SNWS_OK;
+  }
+};
 
-template <int WT>
-int run_poly(Mats& a, float ca, float cb, float cc, const char* what, hipStream_t st) {
-  ORTHO_TRY((ready<&ortho_poly_kernel<WT>>(Tile<WT>::LDS, what)));
-  const unsigned grid = grid_of(a, [](const Mat& t) { return (int64_t)tri(t.m, 2 * WT); });
-  ortho_poly_kernel<WT><<<grid, 256, Tile<WT>::LDS, st>>>(a, ca, cb, cc);
-  SNWS_LAUNCH_CHECK(what);
-  return SNWS_OK;
-}
-
-template <int WT, typename T, bool LAST, bool MUON>
-int run_apply(Mats& a, const MuonArgs& u, float f, int odd, const char* what, hipStream_t st) {
-  ORTHO_TRY((ready<&ortho_apply_kernel<WT, T, LAST, MUON>>(Tile<WT>::LDS, what)));
-  const unsigned grid = grid_of(a, [](const Mat& t) { return (int64_t)cdiv(t.m, 2 * WT) * cdiv(t.n, 2 * WT); });
-  ortho_apply_kernel<WT, T, LAST, MUON><<<grid, 256, Tile<WT>::LDS, st>>>(a, u, f, odd);
-  SNWS_LAUNCH_CHECK(what);
-  return SNWS_OK;
+// The operations of steps k .. k + g - 1; returns how many.  Stored numbers are true ones times a power of two: the factors
+// turn a product of stored numbers into stored ones.
+int group_ops(const float* coeff, const Scales& s, int k, int g, bool last, Op* op) {
+  int n = 0;
+  auto square = [&](int sp, int sq, int sd, double ca, double cb, double cc) {
+    op[n++] = Op{K_SQUARE, (unsigned char)sp, (unsigned char)sq, (unsigned char)sp, (unsigned char)sd, 0, {0, 0}, (float)ca, (float)cb,
+                 (float)cc};
+  };
+  op[n++] = Op{K_GRAM, 0, 0, 0, 0, 0, {0, 0}, 0.f, 0.f, (float)(s.a[k] / (s.x[k] * s.x[k]))};
+  int A = 0, Q = 1, spare[4] = {2, 3, 4, 5};
+  double qs = s.p[k], qmax = s.pmax[k];                  // scale of Q, bound of its numbers
+  for (int j = k; j < k + g; ++j) {
+    const int P = j == k ? Q : spare[0];
+    square(A, A, P, (double)coeff[3 * j] * s.p[j], (double)coeff[3 * j + 1] * s.p[j] / s.a[j],
+           (double)coeff[3 * j + 2] * s.p[j] / (s.a[j] * s.a[j]));
+    const bool more = j + 1 < k + g;
+    if (more) square(P, A, spare[2], 0.0, 0.0, s.pa[j] / (s.p[j] * s.a[j]));      // P A, and beside it
+    if (j > k) {                                                                  // Q <- P Q
+      qmax *= s.pmax[j];
+      const double to = pow2_for(qmax);
+      square(P, Q, spare[1], 0.0, 0.0, to / (s.p[j] * qs));
+      const int old = Q;
+      Q = spare[1];
+      spare[1] = old;
+      qs = to;
+    }
+    if (more) {                                                                   // A <- P (P A), the next X X^T
+      square(P, spare[2], spare[3], 0.0, 0.0, s.a[j + 1] / (s.p[j] * s.pa[j]));
+      const int old = A;
+      A = spare[3];
+      spare[3] = old;
+    }
+  }
+  op[n++] = Op{K_APPLY, 0, (unsigned char)Q, 0, 0, last, {0, 0}, 0.f, 0.f, (float)((last ? 1.0 : s.x[k + g]) / (s.x[k] * qs))};
+  return n;
 }
 
 template <typename T, bool MUON>
-int run_all(Mats& a, const Plan& p, const MuonArgs& u, const float* coeff, int steps, float eps, const Scales& s,
+int run_all(const Mats& a, const Plan& p, const MuonArgs& u, const float* coeff, int steps, float eps, const Scales& s,
             const char* what, hipStream_t st) {
-  double* norms = reinterpret_cast<double*>(a.ws + (p.bytes - 8 * (int64_t)p.norms));
-  unsigned grid = grid_of(a, [](const Mat& t) { return (int64_t)t.normc; });
-  ortho_norm_kernel<T, MUON><<<grid, 256, 0, st>>>(a, u, norms);
+  const Run run{a, p, u, what, st};
+  if (p.mode == SMALL) {
+    Program prog{};
+    for (int k = 0; k < steps;) {
+      const int g = p.group < steps - k ? p.group : steps - k;
+      prog.n += group_ops(coeff, s, k, g, k + g == steps, prog.op + prog.n);
+      k += g;
+    }
+    return run.small<T, MUON>(prog, eps, (float)s.x[0]);
+  }
+  double* partial = reinterpret_cast<double*>(a.ws + p.norms);
+  ortho_norm_kernel<T, MUON><<<run.grid(NORM), 256, 0, st>>>(a, u, partial);
   SNWS_LAUNCH_CHECK(what);
-  grid = grid_of(a, [](const Mat& t) { return (int64_t)cdiv(t.m, 64) * cdiv(t.n, 64); });
-  ortho_start_kernel<T, MUON><<<grid, 256, 0, st>>>(a, u, norms, eps, s.x[0]);
+  ortho_start_kernel<T, MUON><<<run.grid(START), 256, 0, st>>>(run.table(), a.ws, u, partial, eps, (float)s.x[0]);
   SNWS_LAUNCH_CHECK(what);
-  for (int k = 0; k < steps; ++k) {
-    // stored numbers are true ones times a scale: the factors turn a product of stored numbers into the next stored ones
-    const float fa = (float)((double)s.a[k] / ((double)s.x[k] * s.x[k]));
-    ORTHO_TRY(p.wg == 64 ? run_gram<64>(a, p, fa, what, st) : run_gram<32>(a, p, fa, what, st));
-    const float ca = (float)((double)coeff[3 * k] * s.b[k]), cb = (float)((double)coeff[3 * k + 1] * s.b[k] / s.a[k]);
-    const float cc = (float)((double)coeff[3 * k + 2] * s.b[k] / ((double)s.a[k] * s.a[k]));
-    ORTHO_TRY(p.wp == 64 ? run_poly<64>(a, ca, cb, cc, what, st) : run_poly<32>(a, ca, cb, cc, what, st));
-    const bool last = k + 1 == steps;
-    const float fx = (float)((last ? 1.0 : (double)s.x[k + 1]) / ((double)s.x[k] * s.b[k]));
-    if (last)
-      ORTHO_TRY((p.wa == 64 ? run_apply<64, T, true, MUON>(a, u, fx, k & 1, what, st)
-                            : run_apply<32, T, true, MUON>(a, u, fx, k & 1, what, st)));
+  int odd = 0;
+  for (int k = 0; k < steps;) {
+    const int g = p.group < steps - k ? p.group : steps - k;
+    Op op[MAX_OPS];
+    const int n = group_ops(coeff, s, k, g, k + g == steps, op);
+    ORTHO_TRY(p.wg == 64 ? run.gram<64>(op[0].cc, odd) : run.gram<32>(op[0].cc, odd));
+    if (p.mode == CHAIN) {
+      Program prog{};
+      for (int i = 1; i + 1 < n; ++i) prog.op[prog.n++] = op[i];
+      ORTHO_TRY(run.chain(op[0].cc, prog));
+    } else {
+      for (int i = 1; i + 1 < n; ++i) {
+        // P A and P Q read the same matrices and write different ones: one launch for both
+        const bool both = i + 2 < n && op[i].cb == 0.f && op[i + 1].cb == 0.f && op[i + 1].sp != op[i].sd && op[i + 1].sq != op[i].sd;
+        const Op* second = both ? &op[i + 1] : nullptr;
+        const bool deep = run.grid(SQUARE) * (both ? 2 : 1) <= 256;
+        ORTHO_TRY(p.wp == 64 ? (run.squares<64, false>(op[i], second))
+                             : deep ? (run.squares<32, true>(op[i], second)) : (run.squares<32, false>(op[i], second)));
+        if (both) ++i;
+      }
+    }
+    k += g;
+    const Op& ap = op[n - 1];
+    if (ap.last)
+      ORTHO_TRY((p.wa == 64 ? run.apply<64, T, true, MUON>(ap, odd) : run.apply<32, T, true, MUON>(ap, odd)));
     else
-      ORTHO_TRY((p.wa == 64 ? run_apply<64, float, false, false>(a, u, fx, k & 1, what, st)
-                            : run_apply<32, float, false, false>(a, u, fx, k & 1, what, st)));
+      ORTHO_TRY((p.wa == 64 ? run.apply<64, float, false, false>(ap, odd) : run.apply<32, float, false, false>(ap, odd)));
+    odd ^= 1;
   }
   return SNWS_OK;
 }
@@ -684,8 +1460,11 @@ int check_common(const float* coeff, int steps, float eps, Scales* s, const char
 
 }  // namespace
 
-extern "C" int64_t snws_ortho_workspace_bytes(const int* rows, const int* cols, int count) {
-  if (!rows || !cols || count < 1 || count > MAXM) return -1;
+extern "C" int64_t snws_ortho_workspace_bytes(const int* rows, const int* cols, int count, int steps) {
+  if (!rows || !cols || count < 1 || count > MAXM || steps < 1 || steps > MAX_STEPS) {
+    snws_set_error("snws_ortho_workspace_bytes: 1 to %d matrices, 1 to %d steps", MAXM, MAX_STEPS);
+    return -1;
+  }
   Mats a{};
   Plan p;
   a.count = count;
@@ -693,7 +1472,7 @@ extern "C" int64_t snws_ortho_workspace_bytes(const int* rows, const int* cols, 
     if (check_size(rows[i], cols[i], "snws_ortho_workspace_bytes") != SNWS_OK) return -1;
     set_shape(a.mat[i], rows[i], cols[i]);
   }
-  make_plan(a, p);
+  make_plan(a, p, steps, false);      // (the group size takes no room)
   return p.bytes;
 }
 
@@ -718,7 +1497,7 @@ extern "C" int snws_orthogonalize(const snws_ortho_item* items, int count, int d
     a.mat[i].ldx = t.ldx;
     a.mat[i].ldo = t.ldo;
   }
-  make_plan(a, p);
+  make_plan(a, p, steps, dtype == SNWS_BF16);
   SNWS_CHECK_ARG(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
                  "%s: workspace of %lld bytes, 256-byte aligned, needed", what, (long long)p.bytes);
   a.ws = static_cast<unsigned char*>(workspace);
@@ -749,7 +1528,7 @@ extern "C" int snws_muon_update(const snws_muon_item* items, int count, float mo
     a.mat[i].ldx = a.mat[i].ldo = t.cols;
     a.mat[i].step = t.lr;
   }
-  make_plan(a, p);
+  make_plan(a, p, steps, true);
   SNWS_CHECK_ARG(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
                  "%s: workspace of %lld bytes, 256-byte aligned, needed", what, (long long)p.bytes);
   a.ws = static_cast<unsigned char*>(workspace);

@@ -162,7 +162,7 @@ _SIGNATURES = {
     "snws_label_remap": (c_int, [P, c_int, P, c_int64, P]),
     "snws_nchw_to_nhwc_pad": (c_int, [P, c_int, P, c_int, c_int, c_int, c_int, c_int, c_int, P]),
     "snws_adamw_step": (c_int, [P, P, P, P, c_int64, c_float, c_float, c_float, c_float, c_float, c_int64, c_float, P]),
-    "snws_ortho_workspace_bytes": (c_int64, [POINTER(c_int), POINTER(c_int), c_int]),
+    "snws_ortho_workspace_bytes": (c_int64, [POINTER(c_int), POINTER(c_int), c_int, c_int]),
     "snws_orthogonalize": (c_int, [POINTER(OrthoItem), c_int, c_int, POINTER(c_float), c_int, c_float, P, c_int64, P]),
     "snws_muon_update": (c_int, [POINTER(MuonItem), c_int, c_float, c_int, c_float, c_float, POINTER(c_float), c_int, c_float, P,
                                  c_int64, P]),

@@ -2327,37 +2327,47 @@ def upsample_bilinear(x, k):
 QUINTIC = (3.4445, -4.775, 2.0315)      # slope 3.4 at zero; singular values end within about [0.7, 1.2] after five steps
 
 
+_COEFFICIENTS = {}
+
+
 def _ortho_coefficients(coefficients, steps):
-    """One (a, b, c) for every step, or a list of one per step -> (ctypes floats, number of steps)."""
-    steps = int(steps)
-    if steps < 1:
+    """One (a, b, c) for every step, or a list of one per step -> ctypes floats (kept for the next call)."""
+    try:
+        known = _COEFFICIENTS.get((coefficients, steps))
+    except TypeError:           # lists: not hashable
+        known = None
+    if known is not None:
+        return known
+    if int(steps) < 1:
         raise ValueError("orthogonalize: at least one step expected, got %d" % steps)
-    rows = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else list(coefficients)
-    if len(rows) != steps or any(len(r) != 3 for r in rows):
-        raise ValueError("orthogonalize: three coefficients, or three for each of the %d steps, expected" % steps)
-    return (ctypes.c_float * (3 * steps))(*[float(v) for r in rows for v in r])
+    rows = [coefficients] * int(steps) if not hasattr(coefficients[0], "__len__") else list(coefficients)
+    if len(rows) != int(steps) or any(len(r) != 3 for r in rows):
+        raise ValueError("orthogonalize: three coefficients, or three for each of the %d steps, expected" % int(steps))
+    known = (ctypes.c_float * (3 * len(rows)))(*[float(v) for r in rows for v in r])
+    if isinstance(coefficients, tuple) and isinstance(coefficients[0], float) and len(_COEFFICIENTS) < 64:
+        _COEFFICIENTS[(coefficients, steps)] = known
+    return known
 
 
-def _ortho_workspace(sizes, device):
-    n = len(sizes)
-    nbytes = L.lib().snws_ortho_workspace_bytes((ctypes.c_int * n)(*[r for r, _ in sizes]),
-                                                (ctypes.c_int * n)(*[c for _, c in sizes]), n)
+def _ortho_workspace(rows, cols, steps, device):
+    n = len(rows)
+    ints = ctypes.c_int * n
+    nbytes = L.lib().snws_ortho_workspace_bytes(ints(*rows), ints(*cols), n, steps)
     if nbytes < 0:
         raise ValueError(L.lib().snws_last_error().decode("utf-8", "replace"))
     return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
 
 
-def _ortho_flops(sizes, steps):
-    return float(sum(steps * (3 * min(s) ** 2 * max(s) + min(s) ** 3) for s in sizes))
+def _ortho_flops(rows, cols, steps):
+    return float(sum(steps * (3 * min(s) ** 2 * max(s) + min(s) ** 3) for s in zip(rows, cols)))
 
 
-def _by_size(n, size):
+def _by_size(sizes):
     """Indices of a list in calls of at most ORTHO_MAX, the largest matrices first: like sizes share launches."""
-    order = sorted(range(n), key=lambda i: -size(i))
-    return [order[i:i + L.ORTHO_MAX] for i in range(0, n, L.ORTHO_MAX)]
+    order = sorted(range(len(sizes)), key=sizes.__getitem__, reverse=True)
+    return [order[i:i + L.ORTHO_MAX] for i in range(0, len(order), L.ORTHO_MAX)]
 
 
-@torch.no_grad()
 def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
     """The matrices of g with their singular values pushed towards one, by `steps` Newton-Schulz steps
     X <- a X + (b A + c A^2) X, A = X X^T, from X = G / max(|G|_F, eps), on the shorter side of each matrix.
@@ -2367,43 +2377,56 @@ def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
     step.  A matrix that holds a NaN or an infinity comes out as NaN; the others of the call are not touched by it.  Not
     differentiable."""
     if isinstance(g, torch.Tensor):
+        if g.dim() == 2:
+            return _orthogonalize([g], steps, coefficients, eps)[0]
         if g.dim() < 2:
             raise ValueError("orthogonalize: matrices expected, got shape %s" % (tuple(g.shape),))
-        if g.dim() == 2:
-            return orthogonalize([g], steps, coefficients, eps)[0]
         require_gpu(g, "orthogonalize")
-        flat = g.reshape((-1,) + g.shape[-2:])
-        if not flat.numel():
-            return torch.empty(g.shape, dtype=g.dtype, device=g.device)
-        return torch.stack(orthogonalize(list(flat.unbind(0)), steps, coefficients, eps)).view(g.shape)
-    mats = list(g)
+        flat = g.detach().reshape((-1,) + g.shape[-2:])
+        out = torch.empty(flat.shape, dtype=g.dtype, device=g.device)
+        _orthogonalize(list(flat.unbind(0)), steps, coefficients, eps, list(out.unbind(0)))
+        return out.view(g.shape)
+    return _orthogonalize(list(g), steps, coefficients, eps)
+
+
+def _orthogonalize(mats, steps, coefficients, eps, out=None):
     coeff = _ortho_coefficients(coefficients, steps)
+    if not mats:
+        return []
+    first = mats[0]
+    device, dtype = first.device, first.dtype
     for t in mats:
         require_gpu(t, "orthogonalize")
         if t.dim() != 2:
             raise ValueError("orthogonalize: matrices expected, got shape %s" % (tuple(t.shape),))
-        if t.device != mats[0].device or t.dtype != mats[0].dtype:
+        if t.device != device or t.dtype is not dtype:
             raise ValueError("orthogonalize: matrices of one type on one device expected")
-    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in mats]
+    dt = dtype_code(first)
+    if out is None:
+        out = [torch.empty(t.shape, dtype=dtype, device=device) for t in mats]
     live = [i for i, t in enumerate(mats) if t.numel()]
     if not live:
         return out
-    dt, dev = dtype_code(mats[0]), mats[0].device
-    with on_device(mats[0]):
-        for part in _by_size(len(live), lambda i: mats[live[i]].numel()):
-            part = [live[i] for i in part]
-            # read in place: rows of consecutive elements, one behind the other at any distance
-            src = [t if (t.shape[1] == 1 or t.stride(1) == 1) and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else
-                   t.contiguous() for t in (mats[i] for i in part)]
-            items = (L.OrthoItem * len(part))()
-            for it, t, i in zip(items, src, part):
-                rows, cols = t.shape
-                it.x, it.out, it.rows, it.cols = t.data_ptr(), out[i].data_ptr(), rows, cols
-                it.ldx, it.ldo = t.stride(0) if rows > 1 else cols, cols
-            sizes = [tuple(t.shape) for t in src]
-            ws, nbytes = _ortho_workspace(sizes, dev)
-            _launch("orthogonalize", _ortho_flops(sizes, int(steps)), "snws_orthogonalize", items, len(part), dt, coeff,
-                    int(steps), float(eps), ws.data_ptr(), nbytes, stream_of(mats[0]))
+    steps = int(steps)
+    with on_device(first):
+        for part in _by_size([mats[i].numel() for i in live]):
+            n = len(part)
+            items, rows, cols, keep = (L.OrthoItem * n)(), [], [], []
+            for it, k in zip(items, part):
+                t = mats[live[k]]
+                r, c = t.shape
+                ld, inner = t.stride()
+                # read in place: rows of consecutive elements, one behind the other at any distance
+                if not ((c == 1 or inner == 1) and (r == 1 or ld >= c)):
+                    t = t.detach().contiguous()
+                    keep.append(t)
+                    ld = c
+                it.x, it.out, it.ldx, it.ldo, it.rows, it.cols = t.data_ptr(), out[live[k]].data_ptr(), ld if r > 1 else c, c, r, c
+                rows.append(r)
+                cols.append(c)
+            ws, nbytes = _ortho_workspace(rows, cols, steps, device)
+            _launch("orthogonalize", 0.0 if PROFILE is None else _ortho_flops(rows, cols, steps), "snws_orthogonalize", items, n,
+                    dt, coeff, steps, float(eps), ws.data_ptr(), nbytes, stream_of(first))
     return out
 
 
@@ -2417,56 +2440,52 @@ def muon_lr_factor(adjust, rows, cols):
     raise ValueError("muon: adjust_lr is None, 'original' or 'match_rms_adamw', got %r" % (adjust,))
 
 
-@torch.no_grad()
 def muon_update(params, grads, momentum_buffers, lr, weight_decay=0.1, momentum=0.95, nesterov=True, coefficients=QUINTIC,
                 eps=1e-7, steps=5, adjust_lr=None, grad_scale=1.0):
     """One Muon step, in place, for every parameter of the lists (float32, two or more axes; the axes after the first are
     taken together, so a filter (O, I, kh, kw) is an O x (I kh kw) matrix):
         m <- momentum m + (1 - momentum) g;  u = (1 - momentum) g + momentum m  (nesterov)  or  m;
         p <- (1 - lr weight_decay) p - lr factor orthogonalize(u),  factor: see muon_lr_factor.
-    g is grad_scale times the gradient.  Parameters and momentum buffers must be contiguous and all different."""
+    g is grad_scale times the gradient.  Parameters and momentum buffers must be contiguous, and none may overlap another."""
     params, grads, bufs = list(params), list(grads), list(momentum_buffers)
     if not (len(params) == len(grads) == len(bufs)):
         raise ValueError("muon_update: %d parameters, %d gradients, %d momentum buffers" % (len(params), len(grads), len(bufs)))
     coeff = _ortho_coefficients(coefficients, steps)
-    lr, weight_decay = float(lr), float(weight_decay)
+    lr, weight_decay, steps = float(lr), float(weight_decay), int(steps)
     muon_lr_factor(adjust_lr, 1, 1)
-    seen = set()
+    if not params:
+        return
+    device, f32 = params[0].device, torch.float32
+    live, spans, keep = [], [], []
     for p, g, m in zip(params, grads, bufs):
         require_gpu(p, "muon_update")
-        if p.dim() < 2:
-            raise ValueError("muon_update: parameters of two or more axes expected, got shape %s" % (tuple(p.shape),))
-        for t in (g, m):
-            if t.shape != p.shape or t.device != p.device or p.device != params[0].device:
-                raise ValueError("muon_update: parameter, gradient and momentum of one shape on one device expected")
-        if p.dtype != torch.float32 or g.dtype != torch.float32 or m.dtype != torch.float32:
+        shape = p.shape
+        if len(shape) < 2:
+            raise ValueError("muon_update: parameters of two or more axes expected, got shape %s" % (tuple(shape),))
+        if g.shape != shape or m.shape != shape or p.device != device or g.device != device or m.device != device:
+            raise ValueError("muon_update: parameter, gradient and momentum of one shape on one device expected")
+        if p.dtype is not f32 or g.dtype is not f32 or m.dtype is not f32:
             raise TypeError("muon_update: float32 tensors expected")
         if not (p.is_contiguous() and m.is_contiguous()):
             raise ValueError("muon_update: contiguous parameters and momentum buffers expected")
-        if p.numel():
-            if p.data_ptr() in seen or m.data_ptr() in seen or p.data_ptr() == m.data_ptr():
-                raise ValueError("muon_update: a parameter or momentum buffer is given twice")
-            seen.update((p.data_ptr(), m.data_ptr()))
-    live = [i for i, p in enumerate(params) if p.numel()]
-    if not live:
-        return
+        n = p.numel()
+        if n:
+            if not g.is_contiguous():
+                g = g.contiguous()
+                keep.append(g)
+            pp, mp = p.data_ptr(), m.data_ptr()
+            live.append((n, shape[0], n // shape[0], pp, g.data_ptr(), mp))
+            spans += ((pp, pp + 4 * n), (mp, mp + 4 * n))
+    spans.sort()
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("muon_update: a parameter or momentum buffer is given twice, or overlaps another")
     with on_device(params[0]):
-        for part in _by_size(len(live), lambda i: params[live[i]].numel()):
+        for part in _by_size([t[0] for t in live]):
             part = [live[i] for i in part]
-            items = (L.MuonItem * len(part))()
-            sizes, keep = [], []
-            for it, i in zip(items, part):
-                p, g = params[i], grads[i]
-                if not g.is_contiguous():
-                    g = g.contiguous()
-                    keep.append(g)
-                rows = p.shape[0]
-                cols = p.numel() // rows
-                sizes.append((rows, cols))
-                it.param, it.grad, it.momentum, it.rows, it.cols = p.data_ptr(), g.data_ptr(), bufs[i].data_ptr(), rows, cols
-                it.lr = lr * muon_lr_factor(adjust_lr, rows, cols)
-            ws, nbytes = _ortho_workspace(sizes, params[0].device)
-            _launch("muon_update", _ortho_flops(sizes, int(steps)), "snws_muon_update", items, len(part), float(momentum),
-                    int(bool(nesterov)), float(grad_scale), lr * weight_decay, coeff, int(steps), float(eps), ws.data_ptr(),
-                    nbytes, stream_of(params[0]))
+            items = (L.MuonItem * len(part))(*[(pp, gp, mp, r, c, lr * muon_lr_factor(adjust_lr, r, c)) for _, r, c, pp, gp, mp in part])
+            rows, cols = [t[1] for t in part], [t[2] for t in part]
+            ws, nbytes = _ortho_workspace(rows, cols, steps, device)
+            _launch("muon_update", 0.0 if PROFILE is None else _ortho_flops(rows, cols, steps), "snws_muon_update", items,
+                    len(part), float(momentum), int(bool(nesterov)), float(grad_scale), lr * weight_decay, coeff, steps,
+                    float(eps), ws.data_ptr(), nbytes, stream_of(params[0]))
     weights_changed()       # the kernels do not bump version counters

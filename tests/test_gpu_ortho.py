@@ -43,12 +43,14 @@ def test_refuses_cpu_tensors_and_bad_arguments():
 def test_entry_points_refuse_bad_arguments():
     P = 4096        # never dereferenced: every refusal comes before a launch
     coeff = (ctypes.c_float * 3)(*ops.QUINTIC)
-    n = L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(4), (ctypes.c_int * 1)(9), 1)
+    n = L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(4), (ctypes.c_int * 1)(9), 1, 1)
     assert n > 0
-    assert L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(0), (ctypes.c_int * 1)(9), 1) == -1
-    assert L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(4), (ctypes.c_int * 1)((1 << 20) + 1), 1) == -1
-    assert L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(40000), (ctypes.c_int * 1)(40000), 1) == -1
-    assert L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(4), (ctypes.c_int * 1)(9), L.ORTHO_MAX + 1) == -1
+    assert L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(0), (ctypes.c_int * 1)(9), 1, 1) == -1
+    assert L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(4), (ctypes.c_int * 1)((1 << 20) + 1), 1, 1) == -1
+    assert L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(40000), (ctypes.c_int * 1)(40000), 1, 1) == -1
+    assert L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(4), (ctypes.c_int * 1)(9), L.ORTHO_MAX + 1, 1) == -1
+
+    assert L.lib().snws_ortho_workspace_bytes((ctypes.c_int * 1)(4), (ctypes.c_int * 1)(9), 1, 33) == -1
 
     def item(**kw):
         d = dict(x=P, out=P, ldx=9, ldo=9, rows=4, cols=9)
@@ -83,7 +85,7 @@ def test_entry_points_refuse_bad_arguments():
 
 
 def test_calls_hold_the_largest_first():
-    parts = ops._by_size(70, lambda i: i % 7)
+    parts = ops._by_size([i % 7 for i in range(70)])
     assert [len(p) for p in parts] == [32, 32, 6] and sorted(sum(parts, [])) == list(range(70))
     assert parts[0][0] % 7 == 6 and parts[-1][-1] % 7 == 0
 
