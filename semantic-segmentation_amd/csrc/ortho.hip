@@ -340,54 +340,59 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(const Mats* __restrict
 }
 
 // ------------------------------------------------------------------------------------------------ products
-// A workgroup of 4 waves (2 x 2), each WT x WT of a T x T tile, T = 2 WT; k advances by 32 through a ring of S stages, of
-// which S - 1 are on their way while one is multiplied.  128 x 128 tiles take two stages of 32 KB, two workgroups to a
-// CU: the other one's products hide the rest of the latency.  64 x 64 tiles, taken where there are few of them, wait for
-// their operands instead: what a CU has in flight over the latency of 0.7 us is their rate, so they take four stages of
-// 16 KB, or eight (DEEP) where a launch has at most one workgroup for a CU anyway.
-template <int WT, bool DEEP = false>
+// A workgroup of WM x WN waves on a T x T tile; k advances by 32 through a ring of S stages, of which S - 1 are on their
+// way while one is multiplied.
+template <int T_, int WM_, int WN_, int S_>
 struct Tile {
-  static constexpr int T = 2 * WT, MR = WT / 16, LP = T + 2, S = WT == 64 ? 2 : DEEP ? 8 : 4;
-  static constexpr int PIECES = 2 * T / 8, LOADS = PIECES / 4;          // 1 KB LDS-DMA pieces of a stage; per wave
+  static constexpr int T = T_, WM = WM_, WN = WN_, S = S_, W = WM * WN, THREADS = 64 * W;
+  static constexpr int MR = T / WM / 16, NR = T / WN / 16, LP = T + 2;   // 16 x 16 products of a wave; LDS row of the epilogue
+  static constexpr int LOADS = 2 * T / 8 / W;                            // 1 KB LDS-DMA pieces of a stage, per wave
   static constexpr int STAGE = 2 * T * 128;
   static constexpr int LDS = S * STAGE > T * LP * 4 ? S * STAGE : T * LP * 4;
+  static constexpr int PER_CU = 2 * LDS <= 160 * 1024 && 2 * W <= 16 ? 2 : 1;
+  static_assert((S & (S - 1)) == 0 && LOADS % 2 == 0 && W % 4 == 0, "ring, halves and piece order");
 };
+// 128 x 128, four waves of 64 x 64, two workgroups to a CU: one's products hide the other's waits
+typedef Tile<128, 2, 2, 2> Big;
+// 64 x 64, where there are few tiles and a CU holds one workgroup: eight waves, so that each SIMD has two to alternate
+typedef Tile<64, 2, 4, 4> Fine;
+// 128 x 128 by one workgroup alone
+typedef Tile<128, 2, 4, 2> Alone;
 
 typedef __attribute__((ext_vector_type(4))) short short4v;
 
 // acc[mr][nr] += P rows p0.. x Q over the k-blocks [kb0, kb1).  P: M rows of KB blocks.  Q: N rows of KB blocks like it,
 // rows q0..; or, DOWN, K rows of N numbers in QB blocks each, columns q0...  What lies past the last row or block is read
 // as the last one (its results are not stored, and k past the end meets zeros of P).  Entered and left with the LDS free.
-template <int WT, bool DEEP = false, bool DOWN = false>
-__device__ __forceinline__ void product(f32x4 (&acc)[WT / 16][WT / 16], const unsigned char* P, const unsigned char* Q, int p0,
+template <typename G, bool DOWN = false>
+__device__ __forceinline__ void product(f32x4 (&acc)[G::MR][G::NR], const unsigned char* P, const unsigned char* Q, int p0,
                                         int q0, int M, int N, int KB, int kb0, int kb1, unsigned char* smem, int K = 0, int QB = 0) {
-  using G = Tile<WT, DEEP>;
-  constexpr int MR = G::MR, HALF = G::LOADS / 2;
+  constexpr int MR = G::MR, NR = G::NR, W = G::W, HALF = G::LOADS / 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
-  // LDS-DMA of rows: piece w + 4 j holds rows 8 (w + 4 j) .. + 7; lane -> row lane >> 3, slot lane & 7, which receives the
+  const int wm = wave / G::WN, wn = wave % G::WN;
+  // LDS-DMA of rows: piece w + W j holds its rows 8 (w + W j) .. + 7; lane -> row lane >> 3, slot lane & 7, which receives the
   // 16-byte chunk slot ^ ((row >> 1) & 7), so that the 16 lanes of a fragment read hit distinct banks
   const int chunk = (lane & 7) ^ ((4 * (wave & 1) + (lane >> 4)) & 7);
   const unsigned char* src[G::LOADS];
 #pragma unroll
   for (int j = 0; j < (DOWN ? HALF : G::LOADS); ++j) {
-    const int r = 8 * (wave + 4 * j) + (lane >> 3);
+    const int r = 8 * (wave + W * j) + (lane >> 3);
     const bool isq = j >= HALF;                            // the first half of the pieces is P, the second Q
     int row = isq ? q0 + r - G::T : p0 + r;
     const int last = (isq ? N : M) - 1;
     if (row > last) row = last;
     src[j] = (isq ? Q : P) + ((int64_t)row * KB + kb0) * 128 + chunk * 16;
   }
-  // DOWN: piece w + 4 j of Q is column block j, k-rows 8 w .. 8 w + 7 of the stage.  A transposing read takes 32 bytes from
+  // DOWN: piece c of Q is column block c / 4, k-rows 8 (c % 4) .. + 7 of the stage.  A transposing read takes 32 bytes from
   // each of 16 rows 8 g + t (g, t < 4): pairs of chunks trade places by (t >> 1) + 2 (g & 1), so that they meet in twos.
-  const int krow = 8 * wave + (lane >> 3);
+  const int krow = 8 * (wave & 3) + (lane >> 3);
   const int64_t pitch = (int64_t)QB * 128;
   int down[HALF];
   if (DOWN) {
     const int dchunk = (lane & 7) ^ (((lane >> 4 & 1) + 2 * (wave & 1)) << 1);
 #pragma unroll
     for (int j = 0; j < HALF; ++j) {
-      const int blk = (q0 >> 5) + j;
+      const int blk = (q0 >> 5) + (wave >> 2) + (W / 4) * j;
       down[j] = (blk < QB ? blk : QB - 1) * 128 + dchunk * 16;
     }
   }
@@ -395,12 +400,12 @@ __device__ __forceinline__ void product(f32x4 (&acc)[WT / 16][WT / 16], const un
   auto stage = [&](int kb, int buf) {
     const int64_t k128 = (int64_t)(kb - kb0) * 128;
 #pragma unroll
-    for (int j = 0; j < (DOWN ? HALF : G::LOADS); ++j) glds16(src[j] + k128, base + buf * G::STAGE + j * 4096);
+    for (int j = 0; j < (DOWN ? HALF : G::LOADS); ++j) glds16(src[j] + k128, base + buf * G::STAGE + j * (W * 1024));
     if (DOWN) {
       const int k = kb * 32 + krow;
       const unsigned char* row = Q + (int64_t)(k < K ? k : K - 1) * pitch;
 #pragma unroll
-      for (int j = 0; j < HALF; ++j) glds16(row + down[j], base + buf * G::STAGE + G::T * 128 + j * 4096);
+      for (int j = 0; j < HALF; ++j) glds16(row + down[j], base + buf * G::STAGE + G::T * 128 + j * (W * 1024));
     }
   };
   int fro[2];
@@ -413,42 +418,37 @@ __device__ __forceinline__ void product(f32x4 (&acc)[WT / 16][WT / 16], const un
 #pragma unroll
     for (int v = 0; v < 4; ++v) tro[v] = (8 * g + t) * 128 + ((v ^ turn) * 2 + (c >> 1)) * 16 + (c & 1) * 8;
   }
-  struct Frags { f16x8 ph[MR], pl[MR], qh[MR], ql[MR]; };
+  struct Frags { f16x8 ph[MR], pl[MR], qh[NR], ql[NR]; };
   auto fetch = [&](Frags& f, int buf) {
-    const unsigned char* pb = smem + buf * G::STAGE + wm * WT * 128;
-    const unsigned char* qb = smem + buf * G::STAGE + (G::T + wn * WT) * 128;
+    const unsigned char* pb = smem + buf * G::STAGE + wm * (MR * 2048);
+    const unsigned char* qb = smem + buf * G::STAGE + G::T * 128;
     auto q_of = [&](int r, int half) {
-      if (!DOWN) return *reinterpret_cast<const f16x8*>(qb + r * 2048 + fro[half]);
+      const int c16 = wn * NR + r;                           // 16 columns of the tile
+      if (!DOWN) return *reinterpret_cast<const f16x8*>(qb + c16 * 2048 + fro[half]);
       typedef __attribute__((ext_vector_type(8))) short short8v;
-      const unsigned char* at = qb + (r >> 1) * 4096 + tro[half * 2 + (r & 1)];
+      const int side = NR >= 2 ? r & 1 : wn & 1;             // (a wave with one block has the same side throughout)
+      const unsigned char* at = qb + (c16 >> 1) * 4096 + (NR >= 2 ? tro[half * 2 + side] : side ? tro[half * 2 + 1] : tro[half * 2]);
       const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)at);
       const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(at + 512));
       return __builtin_bit_cast(f16x8, short8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
     };
 #pragma unroll
-    for (int r = 0; r < MR; ++r) {
-      f.ph[r] = *reinterpret_cast<const f16x8*>(pb + r * 2048 + fro[0]);
-      f.qh[r] = q_of(r, 0);
-    }
+    for (int r = 0; r < MR; ++r) f.ph[r] = *reinterpret_cast<const f16x8*>(pb + r * 2048 + fro[0]);
 #pragma unroll
-    for (int r = 0; r < MR; ++r) {
-      f.pl[r] = *reinterpret_cast<const f16x8*>(pb + r * 2048 + fro[1]);
-      f.ql[r] = q_of(r, 1);
-    }
+    for (int r = 0; r < NR; ++r) f.qh[r] = q_of(r, 0);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) f.ql[r] = q_of(r, 1);
+#pragma unroll
+    for (int r = 0; r < MR; ++r) f.pl[r] = *reinterpret_cast<const f16x8*>(pb + r * 2048 + fro[1]);
   };
   auto multiply = [&](const Frags& f) {
 #pragma unroll
-    for (int i = 0; i < MR; ++i)
+    for (int w = 0; w < 3; ++w)
 #pragma unroll
-      for (int j = 0; j < MR; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.ph[i], f.qh[j], acc[i][j], 0, 0, 0);
+      for (int i = 0; i < MR; ++i)
 #pragma unroll
-    for (int i = 0; i < MR; ++i)
-#pragma unroll
-      for (int j = 0; j < MR; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.ph[i], f.ql[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < MR; ++i)
-#pragma unroll
-      for (int j = 0; j < MR; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.pl[i], f.qh[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < NR; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w == 2 ? f.pl[i] : f.ph[i], w == 1 ? f.ql[j] : f.qh[j], acc[i][j], 0, 0, 0);
   };
   // The loop has no branches: the last stages are fetched again where there are no more, so that the number in flight,
   // and with it every wait, is a constant.
@@ -473,13 +473,12 @@ __device__ __forceinline__ void product(f32x4 (&acc)[WT / 16][WT / 16], const un
     fetch(next, (k + 1) & (G::S - 1));
     multiply(now);
     // order: the copies, a first product (its operands are there: no wait), then reads and products in turn
-    __builtin_amdgcn_sched_group_barrier(0x008, MR / 2, 0);
+    constexpr int READS = 2 * MR + (DOWN ? 4 : 2) * NR, PRODUCTS = 3 * MR * NR, EACH = (PRODUCTS - 2) / READS > 0 ? (PRODUCTS - 2) / READS : 1;
+    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS > 12 ? 2 : 1, 0);
 #pragma unroll
-    for (int q = 0; q < 2 * MR; ++q) {
+    for (int q = 0; q < READS; ++q) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, MR / 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, DOWN ? 2 : 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, MR / 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -500,23 +499,22 @@ __device__ __forceinline__ void product(f32x4 (&acc)[WT / 16][WT / 16], const un
 }
 
 // the accumulators, times f, as a T x LP float tile in LDS; zeros outside M x N
-template <int WT>
-__device__ __forceinline__ void to_lds(const f32x4 (&acc)[WT / 16][WT / 16], float f, int p0, int q0, int M, int N, float* tile) {
-  using G = Tile<WT>;
+template <typename G>
+__device__ __forceinline__ void to_lds(const f32x4 (&acc)[G::MR][G::NR], float f, int p0, int q0, int M, int N, float* tile) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int pr = (wave >> 1) * WT + 4 * (lane >> 4), qc = (wave & 1) * WT + (lane & 15);
+  const int pr = (wave / G::WN) * (16 * G::MR) + 4 * (lane >> 4), qc = (wave % G::WN) * (16 * G::NR) + (lane & 15);
   if (p0 + G::T <= M && q0 + G::T <= N) {
 #pragma unroll
     for (int i = 0; i < G::MR; ++i)
 #pragma unroll
-      for (int j = 0; j < G::MR; ++j)
+      for (int j = 0; j < G::NR; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) tile[(pr + i * 16 + r) * G::LP + qc + j * 16] = acc[i][j][r] * f;
   } else {
 #pragma unroll
     for (int i = 0; i < G::MR; ++i)
 #pragma unroll
-      for (int j = 0; j < G::MR; ++j)
+      for (int j = 0; j < G::NR; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int p = pr + i * 16 + r, q = qc + j * 16;
@@ -526,12 +524,11 @@ __device__ __forceinline__ void to_lds(const f32x4 (&acc)[WT / 16][WT / 16], flo
   __syncthreads();
 }
 // f(p, q, v): eight columns q .. q + 7 of row p, for every row and octet of the tile
-template <int WT, typename F>
+template <typename G, typename F>
 __device__ __forceinline__ void by_rows(const float* tile, F&& f) {
-  using G = Tile<WT>;
   constexpr int C8 = G::T / 8;
 #pragma unroll 2
-  for (int id = threadIdx.x; id < G::T * C8; id += 256) {
+  for (int id = threadIdx.x; id < G::T * C8; id += G::THREADS) {
     const int p = id / C8, q = (id % C8) * 8;
     float v[8];
 #pragma unroll
@@ -541,12 +538,11 @@ __device__ __forceinline__ void by_rows(const float* tile, F&& f) {
 }
 // f(q, p, v): eight rows p .. p + 7 of column q.  Four lanes take the 32 rows of a block, sixteen the next columns: the
 // reads of a wave spread over all banks (8 LP = 16 mod 32) and the stores of four lanes share a line.
-template <int WT, typename F>
+template <typename G, typename F>
 __device__ __forceinline__ void by_cols(const float* tile, F&& f) {
-  using G = Tile<WT>;
   constexpr int B = G::T / 32;
 #pragma unroll 2
-  for (int id = threadIdx.x; id < G::T * G::T / 8; id += 256) {
+  for (int id = threadIdx.x; id < G::T * G::T / 8; id += G::THREADS) {
     const int g = id >> 6, p = ((g % B) * 4 + (id & 3)) * 8, q = (g / B) * 16 + (id >> 2 & 15);
     float v[8];
 #pragma unroll
@@ -555,12 +551,12 @@ __device__ __forceinline__ void by_cols(const float* tile, F&& f) {
   }
 }
 
-template <int WT>
-__device__ __forceinline__ void clear(f32x4 (&acc)[WT / 16][WT / 16]) {
+template <int M, int N>
+__device__ __forceinline__ void clear(f32x4 (&acc)[M][N]) {
 #pragma unroll
-  for (int i = 0; i < WT / 16; ++i)
+  for (int i = 0; i < M; ++i)
 #pragma unroll
-    for (int j = 0; j < WT / 16; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < N; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
 // Tile number t of a lower triangle of nt tiles a side -> (i, j), j <= i, counted through blocks of 4 x 4 tiles: sixteen
@@ -583,60 +579,58 @@ __device__ __forceinline__ void triangle(int t, int nt, int& i, int& j) {
 }
 
 // a tile, times f, into the symmetric matrix D: rows i .. and, off the diagonal, their mirror image
-template <int WT>
-__device__ __forceinline__ void put_symmetric(const f32x4 (&acc)[WT / 16][WT / 16], float f, const Mat& t, unsigned char* D, int i,
+template <typename G>
+__device__ __forceinline__ void put_symmetric(const f32x4 (&acc)[G::MR][G::NR], float f, const Mat& t, unsigned char* D, int i,
                                               int j, unsigned char* smem) {
-  using G = Tile<WT>;
   float* tile = reinterpret_cast<float*>(smem);
   const int mp = up32(t.m);
-  to_lds<WT>(acc, f, i * G::T, j * G::T, t.m, t.m, tile);
-  by_rows<WT>(tile, [&](int p, int q, const float (&v)[8]) {
+  to_lds<G>(acc, f, i * G::T, j * G::T, t.m, t.m, tile);
+  by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) {
     if (i * G::T + p < t.m && j * G::T + q < mp) store8(D + (int64_t)(i * G::T + p) * mp * 4, j * G::T + q, v);
   });
   if (i != j)
-    by_cols<WT>(tile, [&](int q, int p, const float (&v)[8]) {
+    by_cols<G>(tile, [&](int q, int p, const float (&v)[8]) {
       if (j * G::T + q < t.m && i * G::T + p < mp) store8(D + (int64_t)(j * G::T + q) * mp * 4, i * G::T + p, v);
     });
 }
 
 // A = X X^T in slot 0, one triangle of tiles, stored on both sides of the diagonal.  The contraction over n is split where
 // the tiles alone would not fill the chip: partial tiles go to the workspace as they lie in the accumulators.
-template <int WT>
+template <typename G>
 __device__ __forceinline__ void gram_tile(const Mat& t, unsigned char* ws, int local, float f, int odd, unsigned char* smem) {
-  using G = Tile<WT>;
   const int nt = (t.m + G::T - 1) / G::T, tiles = nt * (nt + 1) / 2;
   const int split = local / tiles, tl = local % tiles;      // tiles of one split are neighbours: they share its columns of X
   int i, j;
   triangle(tl, nt, i, j);
   const int KB = up32(t.n) >> 5, kb0 = split * t.kc, kb1 = kb0 + t.kc < KB ? kb0 + t.kc : KB;
   const unsigned char* X = x_of(t, ws, odd);
-  f32x4 acc[G::MR][G::MR];
-  clear<WT>(acc);
-  product<WT>(acc, X, X, i * G::T, j * G::T, t.m, t.m, KB, kb0, kb1, smem);
+  f32x4 acc[G::MR][G::NR];
+  clear(acc);
+  product<G>(acc, X, X, i * G::T, j * G::T, t.m, t.m, KB, kb0, kb1, smem);
   if (t.ks > 1) {
     f32x4* part = part_of(t, ws) + (int64_t)(tl * t.ks + split) * (G::T * G::T / 4);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int r = 0; r < G::MR; ++r)
 #pragma unroll
-      for (int c = 0; c < G::MR; ++c) part[((wave * G::MR + r) * G::MR + c) * 64 + lane] = acc[r][c];
+      for (int c = 0; c < G::NR; ++c)      // by 16 x 16 blocks of the tile, row by row
+        part[(((wave / G::WN) * G::MR + r) * (G::T / 16) + (wave % G::WN) * G::NR + c) * 64 + lane] = acc[r][c];
     return;
   }
-  put_symmetric<WT>(acc, f, t, slot_of(t, ws, 0), i, j, smem);
+  put_symmetric<G>(acc, f, t, slot_of(t, ws, 0), i, j, smem);
 }
 
-template <int WT>
-__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(const Mats* __restrict__ a, unsigned char* ws, float f, int odd) {
+template <typename G>
+__global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_gram_kernel(const Mats* __restrict__ a, unsigned char* ws, float f, int odd) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   int local;
   const Mat& t = a->mat[find_mat(*a, GRAM, local)];
-  gram_tile<WT>(t, ws, local, f, odd, smem);
+  gram_tile<G>(t, ws, local, f, odd, smem);
 }
 
 // adds the partial tiles of A, a workgroup per 32 x 32 block, in the order of the splits
-template <int WT>
+template <typename G>
 __global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict__ a, unsigned char* ws, float f) {
-  using G = Tile<WT>;
   constexpr int B = G::T / 32;
   __shared__ float tile[32 * 34];
   int local, i, j;
@@ -645,11 +639,9 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict_
   triangle(tl, (t.m + G::T - 1) / G::T, i, j);
   const int p0 = i * G::T + (sub / B) * 32, q0 = j * G::T + (sub % B) * 32, mp = up32(t.m);
   if (p0 >= mp || q0 >= mp) return;
-  // 16 x 16 accumulator blocks (r, c) of the tile's waves that make up this block
+  // the four 16 x 16 blocks (r, c) of this one, a wave each
   const int r16 = (sub / B) * 2 + (threadIdx.x >> 7), c16 = (sub % B) * 2 + (threadIdx.x >> 6 & 1), lane = threadIdx.x & 63;
-  const int wave = (r16 / G::MR) * 2 + c16 / G::MR;
-  const f32x4* part = part_of(t, ws) + (int64_t)tl * t.ks * (G::T * G::T / 4) +
-                      ((wave * G::MR + r16 % G::MR) * G::MR + c16 % G::MR) * 64 + lane;
+  const f32x4* part = part_of(t, ws) + (int64_t)tl * t.ks * (G::T * G::T / 4) + (r16 * (G::T / 16) + c16) * 64 + lane;
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int k = 0; k < t.ks; ++k) s += part[(int64_t)k * (G::T * G::T / 4)];
@@ -674,23 +666,22 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict_
 // The m x m matrices of one group of steps live in slots of the workspace; all are polynomials in A, so they are symmetric
 // and commute, and one triangle of tiles is computed and stored on both sides.
 //   D = ca I + cb C + cc P Q of the stored (scaled) numbers; C is not read where ca and cb are 0.  D is none of the others.
-template <int WT, bool DEEP = false>
+template <typename G>
 __device__ __forceinline__ void square_tile(const Mat& t, unsigned char* ws, int local, const Op& op, unsigned char* smem) {
-  using G = Tile<WT>;
   int i, j;
   triangle(local, (t.m + G::T - 1) / G::T, i, j);
   const int mp = up32(t.m), KB = mp >> 5;
   const unsigned char* C = slot_of(t, ws, op.sc);
   unsigned char* D = slot_of(t, ws, op.sd);
-  f32x4 acc[G::MR][G::MR];
-  clear<WT>(acc);
-  product<WT, DEEP>(acc, slot_of(t, ws, op.sp), slot_of(t, ws, op.sq), i * G::T, j * G::T, t.m, t.m, KB, 0, KB, smem);
+  f32x4 acc[G::MR][G::NR];
+  clear(acc);
+  product<G>(acc, slot_of(t, ws, op.sp), slot_of(t, ws, op.sq), i * G::T, j * G::T, t.m, t.m, KB, 0, KB, smem);
   if (op.ca == 0.f && op.cb == 0.f) {
-    put_symmetric<WT>(acc, op.cc, t, D, i, j, smem);
+    put_symmetric<G>(acc, op.cc, t, D, i, j, smem);
     return;
   }
   float* tile = reinterpret_cast<float*>(smem);
-  to_lds<WT>(acc, op.cc, i * G::T, j * G::T, t.m, t.m, tile);
+  to_lds<G>(acc, op.cc, i * G::T, j * G::T, t.m, t.m, tile);
   auto put = [&](int r, int c, const float (&v)[8]) {        // eight numbers of row r from column c on
     if (r >= t.m || c >= mp) return;
     float w[8];
@@ -699,17 +690,17 @@ __device__ __forceinline__ void square_tile(const Mat& t, unsigned char* ws, int
     for (int e = 0; e < 8; ++e) w[e] = v[e] + op.cb * w[e] + (r == c + e ? op.ca : 0.f);
     store8(D + (int64_t)r * mp * 4, c, w);
   };
-  by_rows<WT>(tile, [&](int p, int q, const float (&v)[8]) { put(i * G::T + p, j * G::T + q, v); });
-  if (i != j) by_cols<WT>(tile, [&](int q, int p, const float (&v)[8]) { put(j * G::T + q, i * G::T + p, v); });
+  by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) { put(i * G::T + p, j * G::T + q, v); });
+  if (i != j) by_cols<G>(tile, [&](int q, int p, const float (&v)[8]) { put(j * G::T + q, i * G::T + p, v); });
 }
 
 // one or two operations that do not depend on each other: gridDim.y of them
-template <int WT, bool DEEP>
-__global__ __launch_bounds__(256, DEEP ? 1 : 2) void ortho_square_kernel(const Mats* __restrict__ a, unsigned char* ws, Op first, Op second) {
+template <typename G>
+__global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_square_kernel(const Mats* __restrict__ a, unsigned char* ws, Op first, Op second) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   int local;
   const Mat& t = a->mat[find_mat(*a, SQUARE, local)];
-  square_tile<WT, DEEP>(t, ws, local, blockIdx.y ? second : first, smem);
+  square_tile<G>(t, ws, local, blockIdx.y ? second : first, smem);
 }
 
 // eight consecutive results at (r, c) of the source's orientation, as many as lie within `cols`: 16-byte accesses of any
@@ -744,41 +735,40 @@ __device__ __forceinline__ void finish8(const Mat& t, int r, int c, int cols, co
 }
 
 // Q X with Q from slot sq: the next group's X, or the result.  Tiles of a column panel of X are neighbours.
-template <int WT, typename T, bool LAST, bool MUON>
+template <typename G, typename T, bool LAST, bool MUON>
 __device__ __forceinline__ void apply_tile(const Mat& t, unsigned char* ws, int local, const MuonArgs& u, int sq, float f, int odd,
                                            unsigned char* smem) {
-  using G = Tile<WT>;
   const int np = up32(t.n), KB = up32(t.m) >> 5;
   const int tp = (t.m + G::T - 1) / G::T, p0 = (local % tp) * G::T, q0 = (local / tp) * G::T;
-  f32x4 acc[G::MR][G::MR];
-  clear<WT>(acc);
-  product<WT, false, true>(acc, slot_of(t, ws, sq), x_of(t, ws, odd), p0, q0, t.m, t.n, KB, 0, KB, smem, t.m, np >> 5);
+  f32x4 acc[G::MR][G::NR];
+  clear(acc);
+  product<G, true>(acc, slot_of(t, ws, sq), x_of(t, ws, odd), p0, q0, t.m, t.n, KB, 0, KB, smem, t.m, np >> 5);
   float* tile = reinterpret_cast<float*>(smem);
-  to_lds<WT>(acc, f, p0, q0, t.m, t.n, tile);
+  to_lds<G>(acc, f, p0, q0, t.m, t.n, tile);
   if (LAST) {
     if (!t.flip)
-      by_rows<WT>(tile, [&](int p, int q, const float (&v)[8]) {
+      by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) {
         if (p0 + p < t.m && q0 + q < t.n) finish8<T, MUON>(t, p0 + p, q0 + q, t.n, v, u);
       });
     else
-      by_cols<WT>(tile, [&](int q, int p, const float (&v)[8]) {
+      by_cols<G>(tile, [&](int q, int p, const float (&v)[8]) {
         if (q0 + q < t.n && p0 + p < t.m) finish8<T, MUON>(t, q0 + q, p0 + p, t.m, v, u);
       });
     return;
   }
   unsigned char* X = x_of(t, ws, odd ^ 1);
-  by_rows<WT>(tile, [&](int p, int q, const float (&v)[8]) {
+  by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) {
     if (p0 + p < t.m && q0 + q < np) store8(X + (int64_t)(p0 + p) * np * 4, q0 + q, v);
   });
 }
 
-template <int WT, typename T, bool LAST, bool MUON>
-__global__ __launch_bounds__(256, 2) void ortho_apply_kernel(const Mats* __restrict__ a, unsigned char* ws, MuonArgs u, int sq, float f,
+template <typename G, typename T, bool LAST, bool MUON>
+__global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_apply_kernel(const Mats* __restrict__ a, unsigned char* ws, MuonArgs u, int sq, float f,
                                                              int odd) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   int local;
   const Mat& t = a->mat[find_mat(*a, APPLY, local)];
-  apply_tile<WT, T, LAST, MUON>(t, ws, local, u, sq, f, odd, smem);
+  apply_tile<G, T, LAST, MUON>(t, ws, local, u, sq, f, odd, smem);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -800,41 +790,40 @@ __device__ __forceinline__ V uniform(const V* p) {
 // kernel arguments into LDS, all at once
 template <typename V>
 __device__ __forceinline__ void keep(V* lds, const V& arg) {
-  for (int i = threadIdx.x; i < (int)(sizeof(V) / 4); i += 256) reinterpret_cast<int*>(lds)[i] = reinterpret_cast<const int*>(&arg)[i];
+  for (int i = threadIdx.x; i < (int)(sizeof(V) / 4); i += blockDim.x) reinterpret_cast<int*>(lds)[i] = reinterpret_cast<const int*>(&arg)[i];
 }
 
-// the sum of a matrix's partial tiles of A, in the order of the splits
-template <int WT>
-__device__ __forceinline__ void add_parts(f32x4 (&acc)[WT / 16][WT / 16], const Mat& t, unsigned char* ws) {
-  using G = Tile<WT>;
+// the sum of a matrix's partial tiles of A, in the order of the splits, in WM x WN waves' accumulators
+template <int T, int WN, int M, int N>
+__device__ __forceinline__ void add_parts(f32x4 (&acc)[M][N], const Mat& t, unsigned char* ws) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const f32x4* part = part_of(t, ws);
-  clear<WT>(acc);
+  const f32x4* part = part_of(t, ws) + lane;
+  clear(acc);
   for (int k = 0; k < t.ks; ++k)
 #pragma unroll
-    for (int r = 0; r < G::MR; ++r)
+    for (int r = 0; r < M; ++r)
 #pragma unroll
-      for (int c = 0; c < G::MR; ++c)
-        acc[r][c] += part[(int64_t)k * (G::T * G::T / 4) + ((wave * G::MR + r) * G::MR + c) * 64 + lane];
+      for (int c = 0; c < N; ++c)
+        acc[r][c] += part[(int64_t)k * (T * T / 4) + (((wave / WN) * M + r) * (T / 16) + (wave % WN) * N + c) * 64];
 }
 
 // The m x m operations of a group for matrices of 65 to 128 rows, a workgroup each, instead of a launch for every operation;
 // the partial tiles of A are added up on the way.
-__global__ __launch_bounds__(256) void ortho_chain128_kernel(const Mats* __restrict__ a, unsigned char* ws, float f, Program prog) {
-  using G = Tile<64>;
+__global__ __launch_bounds__(Alone::THREADS) void ortho_chain128_kernel(const Mats* __restrict__ a, unsigned char* ws, float f,
+                                                                        Program prog) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ Program kept;
   keep(&kept, prog);
   const Mat& t = a->mat[blockIdx.x];
   __syncthreads();
   if (t.ks > 1) {
-    f32x4 acc[G::MR][G::MR];
-    add_parts<64>(acc, t, ws);
-    put_symmetric<64>(acc, f, t, slot_of(t, ws, 0), 0, 0, smem);
+    f32x4 acc[Alone::MR][Alone::NR];
+    add_parts<128, Alone::WN>(acc, t, ws);
+    put_symmetric<Alone>(acc, f, t, slot_of(t, ws, 0), 0, 0, smem);
     phase_done();
   }
   for (int k = 0; k < prog.n; ++k) {
-    square_tile<64>(t, ws, 0, uniform(&kept.op[k]), smem);
+    square_tile<Alone>(t, ws, 0, uniform(&kept.op[k]), smem);
     phase_done();
   }
 }
@@ -916,7 +905,7 @@ __device__ __forceinline__ void product64(f32x4 (&acc)[2][2], const unsigned cha
 }
 __device__ __forceinline__ void square64(const Op& op, int m, unsigned char* slots, const Lane64& L) {
   f32x4 acc[2][2];
-  clear<32>(acc);
+  clear(acc);
   product64(acc, slots + op.sp * SLOT64, slots + op.sq * SLOT64, up32(m) >> 5, L);
   put64(acc, op.ca, op.cb, op.cc, m, slots + op.sd * SLOT64, slots + op.sc * SLOT64, L);
   lds_done();
@@ -933,7 +922,7 @@ __global__ __launch_bounds__(256) void ortho_chain64_kernel(const Mats* __restri
   unsigned char* A = slot_of(t, ws, 0);
   if (t.ks > 1) {
     f32x4 acc[2][2];
-    add_parts<32>(acc, t, ws);
+    add_parts<64, 2>(acc, t, ws);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -980,7 +969,7 @@ __device__ __forceinline__ void apply64(const Mat& t, unsigned char* X, const un
   const int tt = lane >> 2 & 3, cq = lane & 3, base = (cq >> 1) ^ (4 * (L.g & 1) + (tt >> 1));
   const unsigned char* row = X + (2 * c + L.wm < KB ? L.wm : 0) * 8192 + (8 * L.g + tt) * 128 + (cq & 1) * 8;
   f32x4 acc[2][2];
-  clear<32>(acc);
+  clear(acc);
   for (int b = 0; b < nb; ++b) {
     f16x8 x[2][2], q[2][2];
 #pragma unroll
@@ -1129,7 +1118,7 @@ __global__ __launch_bounds__(256) void ortho_small_kernel(Mats a, MuonArgs u, fl
     const Op op = uniform(&kept.op[k]);
     if (op.kind == K_GRAM) {
       f32x4 acc[2][2];
-      clear<32>(acc);
+      clear(acc);
       product64(acc, X, X, KB, L);
       put64(acc, 0.f, 0.f, op.cc, m, smem, smem, L);
       lds_done();
@@ -1200,7 +1189,7 @@ enum Mode { GENERAL, CHAIN, SMALL };
 
 struct Plan {
   Mode mode;
-  int wg, wp, wa;              // wave tiles of the three kinds of products: 64 or 32
+  int wg, wp, wa;              // tiles of the three kinds of products: 128 or 64
   int group;                   // steps taken together
   int64_t bytes, norms;        // of the workspace; where the partial sums of squares begin
 };
@@ -1237,10 +1226,10 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
     else if (mmax <= 128) p.mode = CHAIN;
   }
   // 128 x 128 tiles read each operand half as often as 64 x 64 ones, but need 256 of them to give every CU one
-  p.wg = mmax > 64 ? 64 : 32;
-  p.wp = p.mode == CHAIN ? p.wg : poly >= 256 ? 64 : 32;
-  p.wa = apply >= 256 ? 64 : 32;
-  const int T = 2 * p.wg;
+  p.wg = mmax > 64 ? 128 : 64;
+  p.wp = p.mode == CHAIN ? p.wg : poly >= 256 ? 128 : 64;
+  p.wa = apply >= 256 ? 128 : 64;
+  const int T = p.wg;
   int64_t work = 0;
   for (int i = 0; i < a.count; ++i) work += (int64_t)tri(a.mat[i].m, T) * (up32(a.mat[i].n) >> 5);
   // k-blocks per workgroup so that 512 of them, two per CU, share the whole contraction evenly; at least 8.  A chain adds
@@ -1265,8 +1254,8 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
     off = (off + 255) & ~(int64_t)255;
     const int B = T / 32;
     const int64_t n[PHASES] = {t.normc, (int64_t)cdiv(t.m, 64) * cdiv(t.n, 64), (int64_t)tri(t.m, T) * t.ks,
-                               t.ks > 1 ? (int64_t)tri(t.m, T) * B * B : 0, tri(t.m, 2 * p.wp),
-                               (int64_t)cdiv(t.m, 2 * p.wa) * cdiv(t.n, 2 * p.wa)};
+                               t.ks > 1 ? (int64_t)tri(t.m, T) * B * B : 0, tri(t.m, p.wp),
+                               (int64_t)cdiv(t.m, p.wa) * cdiv(t.n, p.wa)};
     for (int k2 = 0; k2 < PHASES; ++k2) a.end[k2][i] = (int)n[k2] + (i ? a.end[k2][i - 1] : 0);
   }
   p.norms = off;
@@ -1304,29 +1293,28 @@ struct Run {
   unsigned grid(Phase k) const { return (unsigned)a.end[k][a.count - 1]; }
   const Mats* table() const { return reinterpret_cast<const Mats*>(a.ws); }
 
-  template <int WT>
+  template <typename G>
   int gram(float f, int odd) const {
-    ORTHO_TRY((ready<&ortho_gram_kernel<WT>>(Tile<WT>::LDS, what)));
-    ortho_gram_kernel<WT><<<grid(GRAM), 256, Tile<WT>::LDS, st>>>(table(), a.ws, f, odd);
+    ORTHO_TRY((ready<&ortho_gram_kernel<G>>(G::LDS, what)));
+    ortho_gram_kernel<G><<<grid(GRAM), G::THREADS, G::LDS, st>>>(table(), a.ws, f, odd);
     SNWS_LAUNCH_CHECK(what);
     if (p.mode == GENERAL && grid(JOIN)) {
-      ortho_join_kernel<WT><<<grid(JOIN), 256, 0, st>>>(table(), a.ws, f);
+      ortho_join_kernel<G><<<grid(JOIN), 256, 0, st>>>(table(), a.ws, f);
       SNWS_LAUNCH_CHECK(what);
     }
     return SNWS_OK;
   }
-  template <int WT, bool DEEP>
+  template <typename G>
   int squares(const Op& first, const Op* second) const {
-    ORTHO_TRY((ready<&ortho_square_kernel<WT, DEEP>>(Tile<WT, DEEP>::LDS, what)));
-    ortho_square_kernel<WT, DEEP><<<dim3(grid(SQUARE), second ? 2 : 1), 256, Tile<WT, DEEP>::LDS, st>>>(table(), a.ws, first,
-                                                                                                     second ? *second : first);
+    ORTHO_TRY((ready<&ortho_square_kernel<G>>(G::LDS, what)));
+    ortho_square_kernel<G><<<dim3(grid(SQUARE), second ? 2 : 1), G::THREADS, G::LDS, st>>>(table(), a.ws, first, second ? *second : first);
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
   }
   int chain(float f, const Program& prog) const {
-    if (p.wg == 64) {
-      ORTHO_TRY((ready<&ortho_chain128_kernel>(Tile<64>::LDS, what)));
-      ortho_chain128_kernel<<<(unsigned)a.count, 256, Tile<64>::LDS, st>>>(table(), a.ws, f, prog);
+    if (p.wg == 128) {
+      ORTHO_TRY((ready<&ortho_chain128_kernel>(Alone::LDS, what)));
+      ortho_chain128_kernel<<<(unsigned)a.count, Alone::THREADS, Alone::LDS, st>>>(table(), a.ws, f, prog);
     } else {
       ORTHO_TRY((ready<&ortho_chain64_kernel>(SLOTS * SLOT64, what)));
       ortho_chain64_kernel<<<(unsigned)a.count, 256, SLOTS * SLOT64, st>>>(table(), a.ws, f, prog);
@@ -1334,10 +1322,10 @@ struct Run {
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
   }
-  template <int WT, typename T, bool LAST, bool MUON>
+  template <typename G, typename T, bool LAST, bool MUON>
   int apply(const Op& op, int odd) const {
-    ORTHO_TRY((ready<&ortho_apply_kernel<WT, T, LAST, MUON>>(Tile<WT>::LDS, what)));
-    ortho_apply_kernel<WT, T, LAST, MUON><<<grid(APPLY), 256, Tile<WT>::LDS, st>>>(table(), a.ws, u, op.sq, op.cc, odd);
+    ORTHO_TRY((ready<&ortho_apply_kernel<G, T, LAST, MUON>>(G::LDS, what)));
+    ortho_apply_kernel<G, T, LAST, MUON><<<grid(APPLY), G::THREADS, G::LDS, st>>>(table(), a.ws, u, op.sq, op.cc, odd);
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
   }
@@ -1410,7 +1398,7 @@ int run_all(const Mats& a, const Plan& p, const MuonArgs& u, const float* coeff,
     const int g = p.group < steps - k ? p.group : steps - k;
     Op op[MAX_OPS];
     const int n = group_ops(coeff, s, k, g, k + g == steps, op);
-    ORTHO_TRY(p.wg == 64 ? run.gram<64>(op[0].cc, odd) : run.gram<32>(op[0].cc, odd));
+    ORTHO_TRY(p.wg == 128 ? run.gram<Big>(op[0].cc, odd) : run.gram<Fine>(op[0].cc, odd));
     if (p.mode == CHAIN) {
       Program prog{};
       for (int i = 1; i + 1 < n; ++i) prog.op[prog.n++] = op[i];
@@ -1420,18 +1408,16 @@ int run_all(const Mats& a, const Plan& p, const MuonArgs& u, const float* coeff,
         // P A and P Q read the same matrices and write different ones: one launch for both
         const bool both = i + 2 < n && op[i].cb == 0.f && op[i + 1].cb == 0.f && op[i + 1].sp != op[i].sd && op[i + 1].sq != op[i].sd;
         const Op* second = both ? &op[i + 1] : nullptr;
-        const bool deep = run.grid(SQUARE) * (both ? 2 : 1) <= 256;
-        ORTHO_TRY(p.wp == 64 ? (run.squares<64, false>(op[i], second))
-                             : deep ? (run.squares<32, true>(op[i], second)) : (run.squares<32, false>(op[i], second)));
+        ORTHO_TRY(p.wp == 128 ? run.squares<Big>(op[i], second) : run.squares<Fine>(op[i], second));
         if (both) ++i;
       }
     }
     k += g;
     const Op& ap = op[n - 1];
     if (ap.last)
-      ORTHO_TRY((p.wa == 64 ? run.apply<64, T, true, MUON>(ap, odd) : run.apply<32, T, true, MUON>(ap, odd)));
+      ORTHO_TRY((p.wa == 128 ? run.apply<Big, T, true, MUON>(ap, odd) : run.apply<Fine, T, true, MUON>(ap, odd)));
     else
-      ORTHO_TRY((p.wa == 64 ? run.apply<64, float, false, false>(ap, odd) : run.apply<32, float, false, false>(ap, odd)));
+      ORTHO_TRY((p.wa == 128 ? run.apply<Big, float, false, false>(ap, odd) : run.apply<Fine, float, false, false>(ap, odd)));
     odd ^= 1;
   }
   return SNWS_OK;
