@@ -82,11 +82,12 @@ __device__ __forceinline__ f32x4* part_of(const Mat& t, unsigned char* ws) {
   return reinterpret_cast<f32x4*>(slot_of(t, ws, SLOTS));
 }
 
-// 16 bytes per lane from global memory into LDS, lane after lane from byte `lds` on (the same for the whole wave).  Written
+// 16 bytes per lane from global memory (base, the same for the whole wave, plus the lane's offset) into LDS, lane after
+// lane from byte `lds` on.  Written
 // out because the compiler would wait for every copy in flight before a transposing read; it has no result registers, and
 // the waits for it stand in product().  Nothing else here uses m0.
-__device__ __forceinline__ void glds16(const void* gsrc, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gsrc), "s"(lds));
+__device__ __forceinline__ void glds16(const unsigned char* base, unsigned offset, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds));
 }
 __device__ __forceinline__ unsigned lds_offset(const void* p) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
@@ -340,24 +341,30 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(const Mats* __restrict
 }
 
 // ------------------------------------------------------------------------------------------------ products
-// A workgroup of WM x WN waves on a T x T tile; k advances by 32 through a ring of S stages, of which S - 1 are on their
+// A workgroup of WM x WN waves on a TM x TN tile; k advances by 32 through a ring of S stages, of which S - 1 are on their
 // way while one is multiplied.
-template <int T_, int WM_, int WN_, int S_>
+template <int TM_, int TN_, int WM_, int WN_, int S_>
 struct Tile {
-  static constexpr int T = T_, WM = WM_, WN = WN_, S = S_, W = WM * WN, THREADS = 64 * W;
-  static constexpr int MR = T / WM / 16, NR = T / WN / 16, LP = T + 2;   // 16 x 16 products of a wave; LDS row of the epilogue
-  static constexpr int LOADS = 2 * T / 8 / W;                            // 1 KB LDS-DMA pieces of a stage, per wave
-  static constexpr int STAGE = 2 * T * 128;
-  static constexpr int LDS = S * STAGE > T * LP * 4 ? S * STAGE : T * LP * 4;
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, S = S_, W = WM * WN, THREADS = 64 * W;
+  static constexpr int MR = TM / WM / 16, NR = TN / WN / 16;              // 16 x 16 products of a wave
+  static constexpr int PL = TM / 8 / W, QL = TN / 8 / W;                  // 1 KB LDS-DMA pieces of P and Q, per wave and stage
+  static constexpr int LOADS = PL + QL, STAGE = (TM + TN) * 128;
+  static constexpr int LP = TN + 2, SLAB = TM * LP * 4 > 80 * 1024 ? 64 : TM;      // the epilogue's LDS tile: row, and rows at once
+  static constexpr int LDS = S * STAGE > SLAB * LP * 4 ? S * STAGE : SLAB * LP * 4;
   static constexpr int PER_CU = 2 * LDS <= 160 * 1024 && 2 * W <= 16 ? 2 : 1;
-  static_assert((S & (S - 1)) == 0 && LOADS % 2 == 0 && W % 4 == 0, "ring, halves and piece order");
+  static_assert(W % 4 == 0 && PL * W * 8 == TM && QL * W * 8 == TN && MR * WM * 16 == TM && NR * WN * 16 == TN && TN % 32 == 0, "whole pieces");
+  static_assert(LDS <= 160 * 1024, "LDS of a CU");
 };
-// 128 x 128, four waves of 64 x 64, two workgroups to a CU: one's products hide the other's waits
-typedef Tile<128, 2, 2, 2> Big;
-// 64 x 64, where there are few tiles and a CU holds one workgroup: eight waves, so that each SIMD has two to alternate
-typedef Tile<64, 2, 4, 4> Fine;
+// What bounds a step is the time a stage takes to arrive, 0.9 us from beyond the L2, so a CU needs enough of them in flight,
+// and large tiles that bring many products with each byte.
+// 128 x 128, four waves of 64 x 64, two workgroups to a CU
+typedef Tile<128, 128, 2, 2, 2> Big;
+// 128 x 160, four waves of 64 x 80, where that saves a round
+typedef Tile<128, 160, 2, 2, 2> Wide;
+// 64 x 64, where there are few tiles: eight waves, so that each SIMD has two to alternate
+typedef Tile<64, 64, 2, 4, 4> Fine;
 // 128 x 128 by one workgroup alone
-typedef Tile<128, 2, 4, 2> Alone;
+typedef Tile<128, 128, 2, 4, 2> Alone;
 
 typedef __attribute__((ext_vector_type(4))) short short4v;
 
@@ -367,93 +374,89 @@ typedef __attribute__((ext_vector_type(4))) short short4v;
 template <typename G, bool DOWN = false>
 __device__ __forceinline__ void product(f32x4 (&acc)[G::MR][G::NR], const unsigned char* P, const unsigned char* Q, int p0,
                                         int q0, int M, int N, int KB, int kb0, int kb1, unsigned char* smem, int K = 0, int QB = 0) {
-  constexpr int MR = G::MR, NR = G::NR, W = G::W, HALF = G::LOADS / 2;
+  constexpr int MR = G::MR, NR = G::NR, W = G::W, PL = G::PL;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / G::WN, wn = wave % G::WN;
   // LDS-DMA of rows: piece w + W j holds its rows 8 (w + W j) .. + 7; lane -> row lane >> 3, slot lane & 7, which receives the
   // 16-byte chunk slot ^ ((row >> 1) & 7), so that the 16 lanes of a fragment read hit distinct banks
   const int chunk = (lane & 7) ^ ((4 * (wave & 1) + (lane >> 4)) & 7);
-  const unsigned char* src[G::LOADS];
-#pragma unroll
-  for (int j = 0; j < (DOWN ? HALF : G::LOADS); ++j) {
-    const int r = 8 * (wave + W * j) + (lane >> 3);
-    const bool isq = j >= HALF;                            // the first half of the pieces is P, the second Q
-    int row = isq ? q0 + r - G::T : p0 + r;
-    const int last = (isq ? N : M) - 1;
-    if (row > last) row = last;
-    src[j] = (isq ? Q : P) + ((int64_t)row * KB + kb0) * 128 + chunk * 16;
-  }
+  // Offsets from the tile's first row: below 2^32, since a tile has at most 256 rows of at most 4 MB.  They are put together
+  // anew for every stage: an addition and a minimum each, where keeping them would cost registers the products need.
+  const unsigned line = KB * 128, first = (8 * wave + (lane >> 3)) * line, lastp = (unsigned)(M - 1 - p0) * line;
+  const int64_t pitch = (int64_t)QB * 128;
+  const unsigned lastq = DOWN ? (unsigned)(QB - 1) * 128 : (unsigned)(N - 1 - q0) * line;
   // DOWN: piece c of Q is column block c / 4, k-rows 8 (c % 4) .. + 7 of the stage.  A transposing read takes 32 bytes from
   // each of 16 rows 8 g + t (g, t < 4): pairs of chunks trade places by (t >> 1) + 2 (g & 1), so that they meet in twos.
-  const int krow = 8 * (wave & 3) + (lane >> 3);
-  const int64_t pitch = (int64_t)QB * 128;
-  int down[HALF];
+  const unsigned firstq = DOWN ? (unsigned)((q0 >> 5) + (wave >> 2)) * 128 : first;
+  unsigned krow = 0, kend = 0;       // offset of this lane's k-row and chunk in a stage; in the last one
   if (DOWN) {
-    const int dchunk = (lane & 7) ^ (((lane >> 4 & 1) + 2 * (wave & 1)) << 1);
-#pragma unroll
-    for (int j = 0; j < HALF; ++j) {
-      const int blk = (q0 >> 5) + (wave >> 2) + (W / 4) * j;
-      down[j] = (blk < QB ? blk : QB - 1) * 128 + dchunk * 16;
-    }
+    const int r = 8 * (wave & 3) + (lane >> 3), left = K - (KB - 1) * 32;
+    const unsigned dchunk = ((lane & 7) ^ (((lane >> 4 & 1) + 2 * (wave & 1)) << 1)) * 16;
+    krow = r * (unsigned)pitch + dchunk;
+    kend = (r < left ? r : left - 1) * (unsigned)pitch + dchunk;
   }
+  const unsigned char* Pt = P + (int64_t)p0 * line;
+  const unsigned char* Qt = DOWN ? Q : Q + (int64_t)q0 * line;
   const unsigned base = __builtin_amdgcn_readfirstlane(lds_offset(smem)) + wave * 1024;
-  auto stage = [&](int kb, int buf) {
-    const int64_t k128 = (int64_t)(kb - kb0) * 128;
-#pragma unroll
-    for (int j = 0; j < (DOWN ? HALF : G::LOADS); ++j) glds16(src[j] + k128, base + buf * G::STAGE + j * (W * 1024));
-    if (DOWN) {
-      const int k = kb * 32 + krow;
-      const unsigned char* row = Q + (int64_t)(k < K ? k : K - 1) * pitch;
-#pragma unroll
-      for (int j = 0; j < HALF; ++j) glds16(row + down[j], base + buf * G::STAGE + G::T * 128 + j * (W * 1024));
+  // copy c of this wave's PL + QL for stage kb
+  auto copy = [&](int c, int kb, int buf) {
+    const unsigned to = base + buf * G::STAGE;
+    if (c < PL) {
+      const unsigned at = first + c * (8 * W) * line;
+      glds16(Pt + (int64_t)kb * 128, (at < lastp ? at : lastp) + chunk * 16, to + c * (W * 1024));
+    } else {
+      const int j = c - PL;
+      const unsigned krows = kb + 1 < KB ? krow : kend;
+      const unsigned at = firstq + j * (DOWN ? (W / 4) * 128u : (8 * W) * line);
+      glds16(Qt + (DOWN ? kb * 32 * pitch : (int64_t)kb * 128), (at < lastq ? at : lastq) + (DOWN ? krows : chunk * 16),
+             to + G::TM * 128 + j * (W * 1024));
     }
   };
   int fro[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) fro[h] = (lane & 15) * 128 + (((h * 4 + (lane >> 4)) ^ ((lane >> 1) & 7)) * 16);
   // transposing reads: lane -> k-row 8 g + t of the eight 8 g .. (the upper four follow 512 bytes on), four columns 4 c ..
-  int tro[4];      // [half][16-column side of the block]
+  // [half][odd or even block r of the wave]; where a wave begins in the middle of a 32-column block, `mid`, the sides swap
+  // and an odd r belongs to the next block
+  int tro[4];
+  const int mid = (wn * NR) & 1;
   if (DOWN) {
     const int g = lane >> 4, t = lane >> 2 & 3, c = lane & 3, turn = (t >> 1) + 2 * (g & 1);
 #pragma unroll
-    for (int v = 0; v < 4; ++v) tro[v] = (8 * g + t) * 128 + ((v ^ turn) * 2 + (c >> 1)) * 16 + (c & 1) * 8;
+    for (int v = 0; v < 4; ++v)
+      tro[v] = ((wn * NR) >> 1) * 4096 + (8 * g + t) * 128 + ((v ^ mid ^ turn) * 2 + (c >> 1)) * 16 + (c & 1) * 8 + (v & mid) * 4096;
   }
   struct Frags { f16x8 ph[MR], pl[MR], qh[NR], ql[NR]; };
-  auto fetch = [&](Frags& f, int buf) {
+  // read x of the 2 MR + 2 NR fragments of a stage: high halves, low halves of Q, low halves of P, in the order of their use
+  auto fetch = [&](Frags& f, int buf, int x) {
     const unsigned char* pb = smem + buf * G::STAGE + wm * (MR * 2048);
-    const unsigned char* qb = smem + buf * G::STAGE + G::T * 128;
+    const unsigned char* qb = smem + buf * G::STAGE + G::TM * 128;
     auto q_of = [&](int r, int half) {
-      const int c16 = wn * NR + r;                           // 16 columns of the tile
-      if (!DOWN) return *reinterpret_cast<const f16x8*>(qb + c16 * 2048 + fro[half]);
+      if (!DOWN) return *reinterpret_cast<const f16x8*>(qb + (wn * NR + r) * 2048 + fro[half]);
       typedef __attribute__((ext_vector_type(8))) short short8v;
-      const int side = NR >= 2 ? r & 1 : wn & 1;             // (a wave with one block has the same side throughout)
-      const unsigned char* at = qb + (c16 >> 1) * 4096 + (NR >= 2 ? tro[half * 2 + side] : side ? tro[half * 2 + 1] : tro[half * 2]);
+      const unsigned char* at = qb + (r >> 1) * 4096 + tro[half * 2 + (r & 1)];
       const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)at);
       const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(at + 512));
       return __builtin_bit_cast(f16x8, short8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
     };
-#pragma unroll
-    for (int r = 0; r < MR; ++r) f.ph[r] = *reinterpret_cast<const f16x8*>(pb + r * 2048 + fro[0]);
-#pragma unroll
-    for (int r = 0; r < NR; ++r) f.qh[r] = q_of(r, 0);
-#pragma unroll
-    for (int r = 0; r < NR; ++r) f.ql[r] = q_of(r, 1);
-#pragma unroll
-    for (int r = 0; r < MR; ++r) f.pl[r] = *reinterpret_cast<const f16x8*>(pb + r * 2048 + fro[1]);
+    if (x < MR) f.ph[x] = *reinterpret_cast<const f16x8*>(pb + x * 2048 + fro[0]);
+    else if (x < MR + NR) f.qh[x - MR] = q_of(x - MR, 0);
+    else if (x < MR + 2 * NR) f.ql[x - MR - NR] = q_of(x - MR - NR, 1);
+    else f.pl[x - MR - 2 * NR] = *reinterpret_cast<const f16x8*>(pb + (x - MR - 2 * NR) * 2048 + fro[1]);
   };
-  auto multiply = [&](const Frags& f) {
-#pragma unroll
-    for (int w = 0; w < 3; ++w)
-#pragma unroll
-      for (int i = 0; i < MR; ++i)
-#pragma unroll
-        for (int j = 0; j < NR; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w == 2 ? f.pl[i] : f.ph[i], w == 1 ? f.ql[j] : f.qh[j], acc[i][j], 0, 0, 0);
+  // product x of the 3 MR NR of a stage
+  auto multiply = [&](const Frags& f, int x) {
+    const int w = x / (MR * NR), i = x / NR % MR, j = x % NR;
+    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w == 2 ? f.pl[i] : f.ph[i], w == 1 ? f.ql[j] : f.qh[j], acc[i][j], 0, 0, 0);
   };
   // The loop has no branches: the last stages are fetched again where there are no more, so that the number in flight,
   // and with it every wait, is a constant.
   const int nk = kb1 - kb0;
-  auto issue = [&](int k) { stage(kb0 + (k < nk ? k : nk - 1), k & (G::S - 1)); };
+  auto ring = [&](int k) { return (G::S & (G::S - 1)) == 0 ? k & (G::S - 1) : k % G::S; };
+  auto issue = [&](int k) {
+#pragma unroll
+    for (int c = 0; c < G::LOADS; ++c) copy(c, kb0 + (k < nk ? k : nk - 1), ring(k));
+  };
   // the oldest stage in flight has landed for every wave, and every wave holds its fragments of the one before
   auto landed = [&] {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((G::S - 2) * G::LOADS) : "memory");
@@ -464,23 +467,37 @@ __device__ __forceinline__ void product(f32x4 (&acc)[G::MR][G::NR], const unsign
 #pragma unroll
   for (int d = 0; d < G::S - 1; ++d) issue(d);
   landed();
-  fetch(f[0], 0);
+#pragma unroll
+  for (int x = 0; x < 2 * MR + 2 * NR; ++x) fetch(f[0], 0, x);
   issue(G::S - 1);
-  // while stage k is multiplied from registers, the fragments of k + 1 are read and stage k + S is on its way
+  // While stage k is multiplied from registers, the fragments of k + 1 are read and stage k + S is on its way.  A copy
+  // instruction occupies the CU's address unit for 16 cycles, as long as a product its matrix unit, and what waits for it
+  // holds up all that follows in its wave: so the copies are spread over the step, one to each part of it, with the reads
+  // (done before the last part, so that they have arrived at its end) and products.  All copies first: 0.9 us a step
+  // of 128 x 128 instead of 0.7.
   auto step = [&](int k, const Frags& now, Frags& next) {
     landed();
-    issue(k + G::S);
-    fetch(next, (k + 1) & (G::S - 1));
-    multiply(now);
-    // order: the copies, a first product (its operands are there: no wait), then reads and products in turn
-    constexpr int READS = 2 * MR + (DOWN ? 4 : 2) * NR, PRODUCTS = 3 * MR * NR, EACH = (PRODUCTS - 2) / READS > 0 ? (PRODUCTS - 2) / READS : 1;
-    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS > 12 ? 2 : 1, 0);
+    constexpr int PARTS = G::LOADS, PRODUCTS = 3 * MR * NR, READS = 2 * MR + 2 * NR, EARLY = PARTS > 2 ? PARTS - 1 : PARTS;
+    const int kc = kb0 + (k + G::S < nk ? k + G::S : nk - 1), to = ring(k + G::S), from = ring(k + 1);
 #pragma unroll
-    for (int q = 0; q < READS; ++q) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+    for (int c = 0; c < PARTS; ++c) {
+      constexpr int most = (PRODUCTS + PARTS - 1) / PARTS;
+      copy(c, kc, to);
+#pragma unroll
+      for (int x = c * READS / EARLY; x < (c + 1) * READS / EARLY && x < READS; ++x) fetch(next, from, x);
+#pragma unroll
+      for (int x = c * PRODUCTS / PARTS; x < (c + 1) * PRODUCTS / PARTS; ++x) multiply(now, x);
+#pragma unroll
+      for (int q = 0; q < most; ++q) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, DOWN ? 2 : 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto finish = [&](const Frags& now) {
+#pragma unroll
+    for (int x = 0; x < 3 * MR * NR; ++x) multiply(now, x);
   };
   int k = 0;
   for (; k + 2 < nk; k += 2) {
@@ -489,46 +506,50 @@ __device__ __forceinline__ void product(f32x4 (&acc)[G::MR][G::NR], const unsign
   }
   if (k + 1 < nk) {
     step(k, f[0], f[1]);
-    multiply(f[1]);
+    finish(f[1]);
   } else {
-    multiply(f[0]);
+    finish(f[0]);
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // the stages are free for other use
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// the accumulators, times f, as a T x LP float tile in LDS; zeros outside M x N
+// rows SLAB h .. of the tile: the accumulators, times f, as SLAB rows of LP floats in LDS; zeros outside M x N
 template <typename G>
-__device__ __forceinline__ void to_lds(const f32x4 (&acc)[G::MR][G::NR], float f, int p0, int q0, int M, int N, float* tile) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int pr = (wave / G::WN) * (16 * G::MR) + 4 * (lane >> 4), qc = (wave % G::WN) * (16 * G::NR) + (lane & 15);
-  if (p0 + G::T <= M && q0 + G::T <= N) {
+__device__ __forceinline__ void to_lds(const f32x4 (&acc)[G::MR][G::NR], float f, int h, int p0, int q0, int M, int N, float* tile) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int top = (wave / G::WN) * (16 * G::MR) - h * G::SLAB;
+  if (top >= 0 && top < G::SLAB) {
+    const int pr = top + 4 * (lane >> 4), qc = (wave % G::WN) * (16 * G::NR) + (lane & 15);
+    p0 += h * G::SLAB;
+    if (p0 + G::SLAB <= M && q0 + G::TN <= N) {
 #pragma unroll
-    for (int i = 0; i < G::MR; ++i)
+      for (int i = 0; i < G::MR; ++i)
 #pragma unroll
-      for (int j = 0; j < G::NR; ++j)
+        for (int j = 0; j < G::NR; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) tile[(pr + i * 16 + r) * G::LP + qc + j * 16] = acc[i][j][r] * f;
-  } else {
+          for (int r = 0; r < 4; ++r) tile[(pr + i * 16 + r) * G::LP + qc + j * 16] = acc[i][j][r] * f;
+    } else {
 #pragma unroll
-    for (int i = 0; i < G::MR; ++i)
+      for (int i = 0; i < G::MR; ++i)
 #pragma unroll
-      for (int j = 0; j < G::NR; ++j)
+        for (int j = 0; j < G::NR; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int p = pr + i * 16 + r, q = qc + j * 16;
-          tile[p * G::LP + q] = p0 + p < M && q0 + q < N ? acc[i][j][r] * f : 0.f;
-        }
+          for (int r = 0; r < 4; ++r) {
+            const int p = pr + i * 16 + r, q = qc + j * 16;
+            tile[p * G::LP + q] = p0 + p < M && q0 + q < N ? acc[i][j][r] * f : 0.f;
+          }
+    }
   }
   __syncthreads();
 }
-// f(p, q, v): eight columns q .. q + 7 of row p, for every row and octet of the tile
+// f(p, q, v): eight columns q .. q + 7 of row p, for every row and octet of a slab
 template <typename G, typename F>
 __device__ __forceinline__ void by_rows(const float* tile, F&& f) {
-  constexpr int C8 = G::T / 8;
+  constexpr int C8 = G::TN / 8;
 #pragma unroll 2
-  for (int id = threadIdx.x; id < G::T * C8; id += G::THREADS) {
+  for (int id = threadIdx.x; id < G::SLAB * C8; id += G::THREADS) {
     const int p = id / C8, q = (id % C8) * 8;
     float v[8];
 #pragma unroll
@@ -540,9 +561,9 @@ __device__ __forceinline__ void by_rows(const float* tile, F&& f) {
 // reads of a wave spread over all banks (8 LP = 16 mod 32) and the stores of four lanes share a line.
 template <typename G, typename F>
 __device__ __forceinline__ void by_cols(const float* tile, F&& f) {
-  constexpr int B = G::T / 32;
+  constexpr int B = G::SLAB / 32;
 #pragma unroll 2
-  for (int id = threadIdx.x; id < G::T * G::T / 8; id += G::THREADS) {
+  for (int id = threadIdx.x; id < G::SLAB * G::TN / 8; id += G::THREADS) {
     const int g = id >> 6, p = ((g % B) * 4 + (id & 3)) * 8, q = (g / B) * 16 + (id >> 2 & 15);
     float v[8];
 #pragma unroll
@@ -578,46 +599,55 @@ __device__ __forceinline__ void triangle(int t, int nt, int& i, int& j) {
   }
 }
 
-// a tile, times f, into the symmetric matrix D: rows i .. and, off the diagonal, their mirror image
 template <typename G>
-__device__ __forceinline__ void put_symmetric(const f32x4 (&acc)[G::MR][G::NR], float f, const Mat& t, unsigned char* D, int i,
-                                              int j, unsigned char* smem) {
+__device__ __forceinline__ void place(int t, int m, int& p0, int& q0) {
+  static_assert(G::TM == G::TN && G::TM == G::SLAB, "symmetric matrices: square tiles of one slab");
+  int i, j;
+  triangle(t, (m + G::TM - 1) / G::TM, i, j);
+  p0 = i * G::TM;
+  q0 = j * G::TN;
+}
+
+// a tile, times f, into the symmetric matrix D, and its mirror image
+template <typename G>
+__device__ __forceinline__ void put_symmetric(const f32x4 (&acc)[G::MR][G::NR], float f, const Mat& t, unsigned char* D, int p0, int q0,
+                                              unsigned char* smem) {
   float* tile = reinterpret_cast<float*>(smem);
   const int mp = up32(t.m);
-  to_lds<G>(acc, f, i * G::T, j * G::T, t.m, t.m, tile);
+  to_lds<G>(acc, f, 0, p0, q0, t.m, t.m, tile);
   by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) {
-    if (i * G::T + p < t.m && j * G::T + q < mp) store8(D + (int64_t)(i * G::T + p) * mp * 4, j * G::T + q, v);
+    if (p0 + p < t.m && q0 + q < mp) store8(D + (int64_t)(p0 + p) * mp * 4, q0 + q, v);
   });
-  if (i != j)
+  if (p0 != q0)
     by_cols<G>(tile, [&](int q, int p, const float (&v)[8]) {
-      if (j * G::T + q < t.m && i * G::T + p < mp) store8(D + (int64_t)(j * G::T + q) * mp * 4, i * G::T + p, v);
+      if (q0 + q < t.m && p0 + p < mp) store8(D + (int64_t)(q0 + q) * mp * 4, p0 + p, v);
     });
 }
 
 // A = X X^T in slot 0, one triangle of tiles, stored on both sides of the diagonal.  The contraction over n is split where
-// the tiles alone would not fill the chip: partial tiles go to the workspace as they lie in the accumulators.
+// the tiles alone would not fill the chip: partial tiles go to the workspace, 16 x 16 blocks as they lie in the accumulators.
 template <typename G>
 __device__ __forceinline__ void gram_tile(const Mat& t, unsigned char* ws, int local, float f, int odd, unsigned char* smem) {
-  const int nt = (t.m + G::T - 1) / G::T, tiles = nt * (nt + 1) / 2;
+  const int nt = (t.m + G::TM - 1) / G::TM, tiles = nt * (nt + 1) / 2;
   const int split = local / tiles, tl = local % tiles;      // tiles of one split are neighbours: they share its columns of X
-  int i, j;
-  triangle(tl, nt, i, j);
+  int p0, q0;
+  place<G>(tl, t.m, p0, q0);
   const int KB = up32(t.n) >> 5, kb0 = split * t.kc, kb1 = kb0 + t.kc < KB ? kb0 + t.kc : KB;
   const unsigned char* X = x_of(t, ws, odd);
   f32x4 acc[G::MR][G::NR];
   clear(acc);
-  product<G>(acc, X, X, i * G::T, j * G::T, t.m, t.m, KB, kb0, kb1, smem);
+  product<G>(acc, X, X, p0, q0, t.m, t.m, KB, kb0, kb1, smem);
   if (t.ks > 1) {
-    f32x4* part = part_of(t, ws) + (int64_t)(tl * t.ks + split) * (G::T * G::T / 4);
+    f32x4* part = part_of(t, ws) + (int64_t)(tl * t.ks + split) * (G::TM * G::TN / 4);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int r = 0; r < G::MR; ++r)
 #pragma unroll
-      for (int c = 0; c < G::NR; ++c)      // by 16 x 16 blocks of the tile, row by row
-        part[(((wave / G::WN) * G::MR + r) * (G::T / 16) + (wave % G::WN) * G::NR + c) * 64 + lane] = acc[r][c];
+      for (int c = 0; c < G::NR; ++c)
+        part[(((wave / G::WN) * G::MR + r) * (G::TN / 16) + (wave % G::WN) * G::NR + c) * 64 + lane] = acc[r][c];
     return;
   }
-  put_symmetric<G>(acc, f, t, slot_of(t, ws, 0), i, j, smem);
+  put_symmetric<G>(acc, f, t, slot_of(t, ws, 0), p0, q0, smem);
 }
 
 template <typename G>
@@ -631,20 +661,23 @@ __global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_gram_k
 // adds the partial tiles of A, a workgroup per 32 x 32 block, in the order of the splits
 template <typename G>
 __global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict__ a, unsigned char* ws, float f) {
-  constexpr int B = G::T / 32;
+  constexpr int B = G::TN / 32, BB = (G::TM / 32) * B;
   __shared__ float tile[32 * 34];
-  int local, i, j;
+  int local, p0, q0;
   const Mat& t = a->mat[find_mat(*a, JOIN, local)];
-  const int tl = local / (B * B), sub = local % (B * B);
-  triangle(tl, (t.m + G::T - 1) / G::T, i, j);
-  const int p0 = i * G::T + (sub / B) * 32, q0 = j * G::T + (sub % B) * 32, mp = up32(t.m);
+  const int tl = local / BB, sub = local % BB;
+  place<G>(tl, t.m, p0, q0);
+  const bool diagonal = p0 == q0;
+  p0 += (sub / B) * 32;
+  q0 += (sub % B) * 32;
+  const int mp = up32(t.m);
   if (p0 >= mp || q0 >= mp) return;
   // the four 16 x 16 blocks (r, c) of this one, a wave each
   const int r16 = (sub / B) * 2 + (threadIdx.x >> 7), c16 = (sub % B) * 2 + (threadIdx.x >> 6 & 1), lane = threadIdx.x & 63;
-  const f32x4* part = part_of(t, ws) + (int64_t)tl * t.ks * (G::T * G::T / 4) + (r16 * (G::T / 16) + c16) * 64 + lane;
+  const f32x4* part = part_of(t, ws) + (int64_t)tl * t.ks * (G::TM * G::TN / 4) + (r16 * (G::TN / 16) + c16) * 64 + lane;
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int k = 0; k < t.ks; ++k) s += part[(int64_t)k * (G::T * G::T / 4)];
+  for (int k = 0; k < t.ks; ++k) s += part[(int64_t)k * (G::TM * G::TN / 4)];
   const int pr = (r16 & 1) * 16 + 4 * (lane >> 4), qc = (c16 & 1) * 16 + (lane & 15);
 #pragma unroll
   for (int e = 0; e < 4; ++e) tile[(pr + e) * 34 + qc] = p0 + pr + e < t.m && q0 + qc < t.m ? s[e] * f : 0.f;
@@ -656,7 +689,7 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict_
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = tile[r * 34 + c + e];
     if (p0 + r < t.m) store8(A + (int64_t)(p0 + r) * mp * 4, q0 + c, v);
-  } else if (i != j) {
+  } else if (!diagonal) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = tile[(c + e) * 34 + r];
     if (q0 + r < t.m) store8(A + (int64_t)(q0 + r) * mp * 4, p0 + c, v);
@@ -668,20 +701,20 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict_
 //   D = ca I + cb C + cc P Q of the stored (scaled) numbers; C is not read where ca and cb are 0.  D is none of the others.
 template <typename G>
 __device__ __forceinline__ void square_tile(const Mat& t, unsigned char* ws, int local, const Op& op, unsigned char* smem) {
-  int i, j;
-  triangle(local, (t.m + G::T - 1) / G::T, i, j);
+  int p0, q0;
+  place<G>(local, t.m, p0, q0);
   const int mp = up32(t.m), KB = mp >> 5;
   const unsigned char* C = slot_of(t, ws, op.sc);
   unsigned char* D = slot_of(t, ws, op.sd);
   f32x4 acc[G::MR][G::NR];
   clear(acc);
-  product<G>(acc, slot_of(t, ws, op.sp), slot_of(t, ws, op.sq), i * G::T, j * G::T, t.m, t.m, KB, 0, KB, smem);
+  product<G>(acc, slot_of(t, ws, op.sp), slot_of(t, ws, op.sq), p0, q0, t.m, t.m, KB, 0, KB, smem);
   if (op.ca == 0.f && op.cb == 0.f) {
-    put_symmetric<G>(acc, op.cc, t, D, i, j, smem);
+    put_symmetric<G>(acc, op.cc, t, D, p0, q0, smem);
     return;
   }
   float* tile = reinterpret_cast<float*>(smem);
-  to_lds<G>(acc, op.cc, i * G::T, j * G::T, t.m, t.m, tile);
+  to_lds<G>(acc, op.cc, 0, p0, q0, t.m, t.m, tile);
   auto put = [&](int r, int c, const float (&v)[8]) {        // eight numbers of row r from column c on
     if (r >= t.m || c >= mp) return;
     float w[8];
@@ -690,8 +723,8 @@ __device__ __forceinline__ void square_tile(const Mat& t, unsigned char* ws, int
     for (int e = 0; e < 8; ++e) w[e] = v[e] + op.cb * w[e] + (r == c + e ? op.ca : 0.f);
     store8(D + (int64_t)r * mp * 4, c, w);
   };
-  by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) { put(i * G::T + p, j * G::T + q, v); });
-  if (i != j) by_cols<G>(tile, [&](int q, int p, const float (&v)[8]) { put(j * G::T + q, i * G::T + p, v); });
+  by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) { put(p0 + p, q0 + q, v); });
+  if (p0 != q0) by_cols<G>(tile, [&](int q, int p, const float (&v)[8]) { put(q0 + q, p0 + p, v); });
 }
 
 // one or two operations that do not depend on each other: gridDim.y of them
@@ -739,27 +772,31 @@ template <typename G, typename T, bool LAST, bool MUON>
 __device__ __forceinline__ void apply_tile(const Mat& t, unsigned char* ws, int local, const MuonArgs& u, int sq, float f, int odd,
                                            unsigned char* smem) {
   const int np = up32(t.n), KB = up32(t.m) >> 5;
-  const int tp = (t.m + G::T - 1) / G::T, p0 = (local % tp) * G::T, q0 = (local / tp) * G::T;
+  const int tp = (t.m + G::TM - 1) / G::TM, p0 = (local % tp) * G::TM, q0 = (local / tp) * G::TN;
   f32x4 acc[G::MR][G::NR];
   clear(acc);
   product<G, true>(acc, slot_of(t, ws, sq), x_of(t, ws, odd), p0, q0, t.m, t.n, KB, 0, KB, smem, t.m, np >> 5);
   float* tile = reinterpret_cast<float*>(smem);
-  to_lds<G>(acc, f, p0, q0, t.m, t.n, tile);
-  if (LAST) {
-    if (!t.flip)
+  unsigned char* X = x_of(t, ws, odd ^ 1);
+#pragma unroll
+  for (int h = 0; h < G::TM / G::SLAB; ++h) {
+    const int ph = p0 + h * G::SLAB;
+    if (ph >= t.m) break;
+    if (h) __syncthreads();
+    to_lds<G>(acc, f, h, p0, q0, t.m, t.n, tile);
+    if (!LAST)
       by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) {
-        if (p0 + p < t.m && q0 + q < t.n) finish8<T, MUON>(t, p0 + p, q0 + q, t.n, v, u);
+        if (ph + p < t.m && q0 + q < np) store8(X + (int64_t)(ph + p) * np * 4, q0 + q, v);
+      });
+    else if (!t.flip)
+      by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) {
+        if (ph + p < t.m && q0 + q < t.n) finish8<T, MUON>(t, ph + p, q0 + q, t.n, v, u);
       });
     else
       by_cols<G>(tile, [&](int q, int p, const float (&v)[8]) {
-        if (q0 + q < t.n && p0 + p < t.m) finish8<T, MUON>(t, q0 + q, p0 + p, t.m, v, u);
+        if (q0 + q < t.n && ph + p < t.m) finish8<T, MUON>(t, q0 + q, ph + p, t.m, v, u);
       });
-    return;
   }
-  unsigned char* X = x_of(t, ws, odd ^ 1);
-  by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) {
-    if (p0 + p < t.m && q0 + q < np) store8(X + (int64_t)(p0 + p) * np * 4, q0 + q, v);
-  });
 }
 
 template <typename G, typename T, bool LAST, bool MUON>
@@ -1189,7 +1226,7 @@ enum Mode { GENERAL, CHAIN, SMALL };
 
 struct Plan {
   Mode mode;
-  int wg, wp, wa;              // tiles of the three kinds of products: 128 or 64
+  int wg, wp, wa;              // columns of the tiles of the three kinds of products: 64, 128, or 160
   int group;                   // steps taken together
   int64_t bytes, norms;        // of the workspace; where the partial sums of squares begin
 };
@@ -1225,17 +1262,30 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
     if (mmax <= 64 && nmax <= SMALL_N) p.mode = SMALL;
     else if (mmax <= 128) p.mode = CHAIN;
   }
-  // 128 x 128 tiles read each operand half as often as 64 x 64 ones, but need 256 of them to give every CU one
+  // Few tiles: 64 x 64, to occupy CUs.  Else 128 rows, and for the products with X the width whose rounds of 512 workgroups
+  // make the least work: 9216 columns by 1024 rows are 576 tiles of 128 columns, two rounds, but 464 of 160, one.  A
+  // product with X^T splits its contraction to any number of workgroups.
   p.wg = mmax > 64 ? 128 : 64;
   p.wp = p.mode == CHAIN ? p.wg : poly >= 256 ? 128 : 64;
   p.wa = apply >= 256 ? 128 : 64;
-  const int T = p.wg;
+  if (apply >= 256) {
+    int64_t wide = 0;
+    for (int i = 0; i < a.count; ++i) wide += (int64_t)cdiv(a.mat[i].m, 128) * cdiv(a.mat[i].n, 160);
+    if (cdiv64(wide, 512) * 160 < cdiv64(apply, 512) * 128) p.wa = 160;
+  }
+  const int T = p.wg, AM = p.wa == 64 ? 64 : 128, AN = p.wa;
   int64_t work = 0;
   for (int i = 0; i < a.count; ++i) work += (int64_t)tri(a.mat[i].m, T) * (up32(a.mat[i].n) >> 5);
-  // k-blocks per workgroup so that 512 of them, two per CU, share the whole contraction evenly; at least 8.  A chain adds
-  // the partial tiles by itself: at most eight of them.
-  int64_t kc = cdiv64(work, 512);
+  // k-blocks per workgroup so that as many as the chip holds at once share the whole contraction evenly; at least 8.  A
+  // chain adds the partial tiles by itself: at most eight of them.
+  const int64_t round = 512;
+  int64_t kc = cdiv64(work, round);
   if (kc < 8) kc = 8;
+  for (;; ++kc) {        // each matrix rounds up: not more than one round in all
+    int64_t n = 0;
+    for (int i = 0; i < a.count; ++i) n += tri(a.mat[i].m, T) * cdiv64(up32(a.mat[i].n) >> 5, kc);
+    if (n <= round || kc >= 4 * cdiv64(work, round)) break;
+  }
   int64_t off = (sizeof(Mats) + 255) & ~(int64_t)255;
   int norms = 0;
   for (int i = 0; i < a.count; ++i) {
@@ -1252,10 +1302,10 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
     off += 2 * size_x(t) + SLOTS * size_slot(t);
     if (t.ks > 1) off += (int64_t)tri(t.m, T) * t.ks * T * T * 4;
     off = (off + 255) & ~(int64_t)255;
-    const int B = T / 32;
+    const int B = (T / 32) * (T / 32);
     const int64_t n[PHASES] = {t.normc, (int64_t)cdiv(t.m, 64) * cdiv(t.n, 64), (int64_t)tri(t.m, T) * t.ks,
-                               t.ks > 1 ? (int64_t)tri(t.m, T) * B * B : 0, tri(t.m, p.wp),
-                               (int64_t)cdiv(t.m, p.wa) * cdiv(t.n, p.wa)};
+                               t.ks > 1 ? (int64_t)tri(t.m, T) * B : 0, tri(t.m, p.wp),
+                               (int64_t)cdiv(t.m, AM) * cdiv(t.n, AN)};
     for (int k2 = 0; k2 < PHASES; ++k2) a.end[k2][i] = (int)n[k2] + (i ? a.end[k2][i - 1] : 0);
   }
   p.norms = off;
@@ -1323,11 +1373,19 @@ struct Run {
     return SNWS_OK;
   }
   template <typename G, typename T, bool LAST, bool MUON>
-  int apply(const Op& op, int odd) const {
+  int apply_by(const Op& op, int odd) const {
     ORTHO_TRY((ready<&ortho_apply_kernel<G, T, LAST, MUON>>(G::LDS, what)));
     ortho_apply_kernel<G, T, LAST, MUON><<<grid(APPLY), G::THREADS, G::LDS, st>>>(table(), a.ws, u, op.sq, op.cc, odd);
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
+  }
+  template <typename T, bool LAST, bool MUON>
+  int apply(const Op& op, int odd) const {
+    switch (p.wa) {
+      case 160: return apply_by<Wide, T, LAST, MUON>(op, odd);
+      case 128: return apply_by<Big, T, LAST, MUON>(op, odd);
+      default: return apply_by<Fine, T, LAST, MUON>(op, odd);
+    }
   }
   template <typename T, bool MUON>
   int small(const Program& prog, float eps, float scale) const {
@@ -1414,10 +1472,7 @@ int run_all(const Mats& a, const Plan& p, const MuonArgs& u, const float* coeff,
     }
     k += g;
     const Op& ap = op[n - 1];
-    if (ap.last)
-      ORTHO_TRY((p.wa == 128 ? run.apply<Big, T, true, MUON>(ap, odd) : run.apply<Fine, T, true, MUON>(ap, odd)));
-    else
-      ORTHO_TRY((p.wa == 128 ? run.apply<Big, float, false, false>(ap, odd) : run.apply<Fine, float, false, false>(ap, odd)));
+    ORTHO_TRY((ap.last ? run.apply<T, true, MUON>(ap, odd) : run.apply<float, false, false>(ap, odd)));
     odd ^= 1;
   }
   return SNWS_OK;
