@@ -185,7 +185,9 @@ class Trainer:
 
     def __init__(self, model, lr=0.002, weight_decay=5e-4, total_iters=1000, ignore_index=255, group=None,
                  bucket_mb=25.0, fused_loss=None, optimizer="flat", class_weight=None):
-        """class_weight: None or a float tensor of per-class loss weights (train.py:55-67, --use-balanced-weights)."""
+        """class_weight: None or a float tensor of per-class loss weights (train.py:55-67, --use-balanced-weights).
+        optimizer: "flat" (AdamW in one launch), "muon" (orthogonalised momentum for the filters, AdamW for the vectors and
+        the classification conv, both at lr) or "torch" (torch.optim.AdamW)."""
         self.model = model
         self.class_weight = class_weight
         self.val_loss = None
@@ -197,12 +199,16 @@ class Trainer:
         if optimizer == "flat":      # one fused launch over flat parameter / gradient buffers (snws.optim)
             from .optim import FlatAdamW
             self.opt = FlatAdamW(model.parameters(), lr=lr, weight_decay=weight_decay)
+        elif optimizer == "muon":    # updates of the size of AdamW's, so the reference's learning rate serves both parts
+            from .optim import FlatMuon
+            self.opt = FlatMuon(model.parameters(), lr=lr, weight_decay=weight_decay, adjust_lr_fn="match_rms_adamw",
+                                adamw_params=head.parameters())
         else:                        # torch's multi-tensor AdamW
             try:
                 self.opt = torch.optim.AdamW(model.parameters(), lr=lr, weight_decay=weight_decay, fused=True)
             except (RuntimeError, TypeError):
                 self.opt = torch.optim.AdamW(model.parameters(), lr=lr, weight_decay=weight_decay)
-        if optimizer == "flat":
+        if optimizer in ("flat", "muon"):
             self.buckets = GradBuckets(self.opt.params, bucket_mb, group, self.opt.flat_g, self.opt.offsets)
         else:
             self.buckets = GradBuckets(list(model.parameters()), bucket_mb, group)
