@@ -23,11 +23,14 @@ struct BwdArgs {
   int C;
 };
 
-constexpr int64_t MAX_BLOCKS = 512;   // two resident workgroups per CU
+// Workgroups that stay, and so partial rows: one per CU, four waves, has enough loads in flight where a lane holds three
+// chunks or more of each operand, two where it holds fewer (1048576 rows of 64 bfloat16: 80 us instead of 130; 1048576
+// rows of 320, five chunks: 387 us and 5 us for the partial rows, instead of 390 and 9).
+constexpr int64_t most_blocks(int nv) { return nv <= 2 ? 512 : 256; }
 
 template <typename T, int G, int NV, bool TAIL>
 __global__ __launch_bounds__(G <= 256 ? 256 : G) void ln_bwd_kernel(BwdArgs a) {
-  constexpr int VEC = Geo<T>::VEC, BT = G <= 256 ? 256 : G, GB = BT / G, R = Rows<NV>::R;
+  constexpr int VEC = Geo<T>::VEC, BT = G <= 256 ? 256 : G, GB = BT / G;
   constexpr int NW = BT / 64, WC = (G < 64 ? G : 64) * NV * VEC;       // waves; columns that one wave holds
   __shared__ float red[2 * NW];
   __shared__ float fold[G < 256 ? 2 * WC : 1];
@@ -47,63 +50,51 @@ __global__ __launch_bounds__(G <= 256 ? 256 : G) void ln_bwd_kernel(BwdArgs a) {
     for (int e = 0; e < VEC; ++e) dw[k][e] = db[k][e] = 0.f;
   }
   const float inv = 1.f / (float)a.C;
-  const int64_t step = (int64_t)gridDim.x * GB * R;
-  for (int64_t r0 = ((int64_t)blockIdx.x * GB + grp) * R; r0 < a.rows; r0 += step) {
-    uint4 vx[R][NV], vg[R][NV];
-    float mean[R], rstd[R];
+  for (int64_t row = (int64_t)blockIdx.x * GB + grp; row < a.rows; row += (int64_t)gridDim.x * GB) {
+    uint4 vx[NV], vg[NV];
+    const float mean = a.mean[row], rstd = a.rstd[row];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t row = r0 + r < a.rows ? r0 + r : a.rows - 1;
-      mean[r] = a.mean[row];
-      rstd[r] = a.rstd[row];
+    for (int k = 0; k < NV; ++k) {
+      vx[k] = load_raw(x + row * a.ldx + col[k]);
+      vg[k] = load_raw(dy + row * a.lddy + col[k]);
+    }
+    float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        vx[r][k] = load_raw(x + row * a.ldx + col[k]);
-        vg[r][k] = load_raw(dy + row * a.lddy + col[k]);
+    for (int k = 0; k < NV; ++k) {
+      float f[VEC], g[VEC];
+      unpack(vx[k], f);
+      unpack(vg[k], g);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float z = (f[e] - mean) * rstd;
+        const bool on = !TAIL || e >= dup[k];
+        const float d = on ? g[e] : 0.f, dz = on ? g[e] * z : 0.f;
+        db[k][e] += d;
+        dw[k][e] += dz;
+        s1 += d * w[k][e];
+        s2 += dz * w[k][e];
       }
     }
+    if (!dx) continue;
+    group_sum2<G>(s1, s2, red);
+    const float m1 = s1 * inv, m2 = s2 * inv;
+    T* o = dx + row * a.lddx;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const bool live = R == 1 || r0 + r < a.rows;
-      float s1 = 0.f, s2 = 0.f;
+    for (int k = 0; k < NV; ++k) {
+      float f[VEC], g[VEC];
+      unpack(vx[k], f);
+      unpack(vg[k], g);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        float f[VEC], g[VEC];
-        unpack(vx[r][k], f);
-        unpack(vg[r][k], g);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float z = (f[e] - mean[r]) * rstd[r];
-          const bool on = (!TAIL || e >= dup[k]) && live;
-          const float d = on ? g[e] : 0.f, dz = on ? g[e] * z : 0.f;
-          db[k][e] += d;
-          dw[k][e] += dz;
-          s1 += d * w[k][e];
-          s2 += dz * w[k][e];
-        }
+      for (int e = 0; e < VEC; ++e) {
+        const float z = (f[e] - mean) * rstd;
+        f[e] = rstd * (g[e] * w[k][e] - m1 - z * m2);
       }
-      if (!dx) continue;
-      group_sum2<G>(s1, s2, red);
-      if (!live) continue;
-      const float m1 = s1 * inv, m2 = s2 * inv;
-      T* o = dx + (r0 + r) * a.lddx;
+      if (!TAIL || dup[k] == 0) {
+        store_raw(o + col[k], pack(f));
+      } else {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        float f[VEC], g[VEC];
-        unpack(vx[r][k], f);
-        unpack(vg[r][k], g);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float z = (f[e] - mean[r]) * rstd[r];
-          f[e] = rstd[r] * (g[e] * w[k][e] - m1 - z * m2);
-        }
-        if (!TAIL || dup[k] == 0) {
-          store_raw(o + col[k], pack(f));
-        } else {
-#pragma unroll
-          for (int e = 1; e < VEC; ++e)
-            if (e >= dup[k]) o[col[k] + e] = (T)f[e];
-        }
+        for (int e = 1; e < VEC; ++e)
+          if (e >= dup[k]) o[col[k] + e] = (T)f[e];
       }
     }
   }
@@ -233,12 +224,19 @@ __global__ __launch_bounds__(256) void ln_bwd_wide_param_kernel(BwdArgs a) {
 // dweight[c] / dbias[c] = sum over the partial rows, in float64 and a fixed order: 32 columns x 32 row lanes
 __global__ __launch_bounds__(1024) void ln_param_sum_kernel(const float* __restrict__ part, int blocks, int C,
                                                             float* __restrict__ dw, float* __restrict__ db) {
+  constexpr int LOADS = 8;
   __shared__ double red[32][33];
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
   const int i = blockIdx.x * 32 + cl;
   double s = 0.0;
   if (i < 2 * C)
-    for (int r = rl; r < blocks; r += 32) s += (double)part[(int64_t)r * 2 * C + i];
+    for (int r = rl; r < blocks; r += 32 * LOADS) {
+      float f[LOADS];        // in flight together
+#pragma unroll
+      for (int k = 0; k < LOADS; ++k) f[k] = r + 32 * k < blocks ? part[(int64_t)(r + 32 * k) * 2 * C + i] : 0.f;
+#pragma unroll
+      for (int k = 0; k < LOADS; ++k) s += (double)f[k];
+    }
   red[rl][cl] = s;
   __syncthreads();
   if (rl == 0 && i < 2 * C) {
@@ -254,7 +252,7 @@ __global__ __launch_bounds__(1024) void ln_param_sum_kernel(const float* __restr
 template <typename T>
 int64_t bwd_blocks(int64_t rows, int C) {
   constexpr int VEC = Geo<T>::VEC;
-  int64_t need;
+  int64_t need, most = most_blocks(1);
   if (C < VEC) {
     need = cdiv64(rows, 256);
   } else {
@@ -263,13 +261,13 @@ int64_t bwd_blocks(int64_t rows, int C) {
     if (!G) {
       need = cdiv64(rows, 16);                       // slices of the column sums
       const int64_t cb = cdiv64(C, 256);
-      const int64_t most = cdiv64(1024, cb);
+      most = cdiv64(1024, cb);
       return need < most ? need : most;
     }
-    const int nv = (int)cdiv64(chunks, G), R = nv == 1 ? 4 : nv == 2 ? 2 : 1;
-    need = cdiv64(rows, (int64_t)(G <= 256 ? 256 / G : 1) * R);
+    need = cdiv64(rows, G <= 256 ? 256 / G : 1);
+    most = most_blocks((int)cdiv64(chunks, G));
   }
-  return need < MAX_BLOCKS ? need : MAX_BLOCKS;
+  return need < most ? need : most;
 }
 
 template <typename T>

@@ -160,7 +160,4 @@ int dispatch(int64_t chunks, F&& f) {
 }
 #undef LN_CASE
 
-// rows in flight per group: enough 16-byte loads per lane to cover the memory's latency where a row needs only one or two
-template <int NV> struct Rows { static constexpr int R = NV == 1 ? 4 : NV == 2 ? 2 : 1; };
-
 }  // namespace ln

@@ -1243,12 +1243,13 @@ int tri(int m, int T) { const int n = cdiv(m, T); return n * (n + 1) / 2; }
 // 1.0 from m = 512 on, where long float32 sums dominate; groups of five lose up to 100 times.  So: three from m = 512
 // on and for results that carry less (bfloat16; an update added to a parameter), else two.
 void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
-  int64_t apply = 0, poly = 0;
+  int64_t apply = 0, poly = 0, grams = 0;
   double long_ops = 0.0, square_ops = 0.0;
   int mmax = 0, mmin = 1 << 30, nmax = 0;
   for (int i = 0; i < a.count; ++i) {
     const Mat& t = a.mat[i];
     poly += tri(t.m, 128);
+    grams += tri(t.m, 128) * cdiv64(up32(t.n) >> 5, 8);
     apply += (int64_t)cdiv(t.m, 128) * cdiv(t.n, 128);
     mmax = t.m > mmax ? t.m : mmax;
     mmin = t.m < mmin ? t.m : mmin;
@@ -1265,7 +1266,7 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
   // Few tiles: 64 x 64, to occupy CUs.  Else 128 rows, and for the products with X the width whose rounds of 512 workgroups
   // make the least work: 9216 columns by 1024 rows are 576 tiles of 128 columns, two rounds, but 464 of 160, one.  A
   // product with X^T splits its contraction to any number of workgroups.
-  p.wg = mmax > 64 ? 128 : 64;
+  p.wg = mmax > 64 && (p.mode == CHAIN || grams >= 256) ? 128 : 64;
   p.wp = p.mode == CHAIN ? p.wg : poly >= 256 ? 128 : 64;
   p.wa = apply >= 256 ? 128 : 64;
   if (apply >= 256) {
