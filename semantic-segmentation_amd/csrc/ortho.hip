@@ -16,6 +16,10 @@
 // X down its columns, through the transposing LDS read, so X is kept in one orientation only.
 //
 // All matrices of a list share each launch: a workgroup finds its matrix and tile from its index.
+//
+// Measured, float32, five steps: 64 x 126 28 us (one launch), 1024 x 9216 365 us (norm 8, start 17, X X^T 32 and its join
+// 8.5 twice, 13 launches of m x m products at 11.3, Q X 55 and 61), the 21 million numbers of 18 filters with their Muon
+// update 715 us (46, 51, 61 and 10 twice, 13 x 20, 106 and 126).
 #include "common.h"
 #include <math.h>
 
@@ -83,9 +87,8 @@ __device__ __forceinline__ f32x4* part_of(const Mat& t, unsigned char* ws) {
 }
 
 // 16 bytes per lane from global memory (base, the same for the whole wave, plus the lane's offset) into LDS, lane after
-// lane from byte `lds` on.  Written
-// out because the compiler would wait for every copy in flight before a transposing read; it has no result registers, and
-// the waits for it stand in product().  Nothing else here uses m0.
+// lane from byte `lds` on.  Written out because the compiler would wait for every copy in flight before a transposing read;
+// it has no result registers, and the waits for it stand in product().  Nothing else here uses m0.
 __device__ __forceinline__ void glds16(const unsigned char* base, unsigned offset, unsigned lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds));
 }
@@ -158,7 +161,8 @@ __device__ __forceinline__ float direction(float g, float m, const MuonArgs& u) 
 }
 
 // Partial sums of squares in float64 (no overflow or underflow over float32's range, a fixed order); a Muon item's
-// momentum is advanced on the way: m <- momentum m + (1 - momentum) grad_scale g.
+// momentum is advanced on the way: m <- momentum m + (1 - momentum) grad_scale g.  Bound by memory: 4.6 TB/s for a
+// 1024 x 9216 matrix, 5.5 TB/s for the gradients and momenta of 21 million parameters.
 template <typename T, bool MUON>
 __device__ __forceinline__ double norm_chunk(const Mat& t, int chunk, const MuonArgs& u) {
   constexpr int VEC = MUON ? 4 : 16 / (int)sizeof(T);
@@ -263,9 +267,9 @@ __device__ __forceinline__ void read8(const bf16_t* p, float (&v)[8]) {
 }
 
 // A 64 x 64 tile of the source, times f, into X: 16-byte reads to 16-byte stores, row by row, or - where X is the
-// transpose - through LDS.
+// transpose - through LDS.  Bound by memory: 4.5 TB/s read and written for 1024 x 9216, 5 TB/s for a model's filters.
 template <typename T, bool MUON>
-__device__ __forceinline__ void start_tile(const Mat& t, unsigned char* ws, int local, float f, const MuonArgs& u, float* tile) {
+__device__ __forceinline__ void start_tile(const Mat& t, unsigned char* ws, int local, double f, const MuonArgs& u, float* tile) {
   constexpr int LP = 66;
   const int rows = t.flip ? t.n : t.m, cols = t.flip ? t.m : t.n;
   const int tc = (cols + 63) >> 6, r0 = (local / tc) * 64, c0 = (local % tc) * 64;
@@ -294,7 +298,7 @@ __device__ __forceinline__ void start_tile(const Mat& t, unsigned char* ws, int 
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[k][e] = f * (MUON ? direction(v[k][e] * u.grad_scale, m[e], u) : v[k][e]);
+    for (int e = 0; e < 8; ++e) v[k][e] = (float)(f * (double)(MUON ? direction(v[k][e] * u.grad_scale, m[e], u) : v[k][e]));
   }
   if (!t.flip) {
 #pragma unroll
@@ -321,10 +325,10 @@ __device__ __forceinline__ void start_tile(const Mat& t, unsigned char* ws, int 
   }
 }
 
-// scale / max(norm, eps): a NaN stays one
-__device__ __forceinline__ float start_factor(double sum, float eps, float scale) {
+// scale / max(norm, eps): a NaN stays one.  In float64, and multiplied as such: the inverse of a small norm leaves float32.
+__device__ __forceinline__ double start_factor(double sum, float eps, float scale) {
   const double norm = sqrt(sum);
-  return (float)((double)scale / (norm < (double)eps ? (double)eps : norm));
+  return (double)scale / (norm < (double)eps ? (double)eps : norm);
 }
 
 // X_0: the matrices, normalised
@@ -355,13 +359,16 @@ struct Tile {
   static_assert(W % 4 == 0 && PL * W * 8 == TM && QL * W * 8 == TN && MR * WM * 16 == TM && NR * WN * 16 == TN && TN % 32 == 0, "whole pieces");
   static_assert(LDS <= 160 * 1024, "LDS of a CU");
 };
-// What bounds a step is the time a stage takes to arrive, 0.9 us from beyond the L2, so a CU needs enough of them in flight,
-// and large tiles that bring many products with each byte.
-// 128 x 128, four waves of 64 x 64, two workgroups to a CU
+// Large tiles bring more products with each byte copied, small ones occupy more CUs.  Two workgroups on a CU take turns: one
+// multiplies while the other waits.
+// 128 x 128, four waves of 64 x 64, two workgroups to a CU: X X^T of 1024 x 9216 in 32 us, 0.9 PFLOP/s (64 x 64: 41 us)
 typedef Tile<128, 128, 2, 2, 2> Big;
-// 128 x 160, four waves of 64 x 80, where that saves a round
+// 128 x 160, four waves of 64 x 80, where that saves a round: Q X there in 55 us, 1.05 PFLOP/s (128 x 128: 67, 64 x 64: 74)
 typedef Tile<128, 160, 2, 2, 2> Wide;
-// 64 x 64, where there are few tiles: eight waves, so that each SIMD has two to alternate
+// 64 x 64, where there are few tiles; eight waves, so that each SIMD has two to alternate: a product of 1024 x 1024 in
+// 11.3 us (128 x 128: 28 us).  Of those about 4 are the launch, the first copies and the epilogue; in the rest the matrix
+// units are busy for 2.6: the operands come from beyond the L2s, of which each needs half the matrix, 26 MB in all.  A
+// deeper ring or a barrier for every second stage only change nothing.
 typedef Tile<64, 64, 2, 4, 4> Fine;
 // 128 x 128 by one workgroup alone
 typedef Tile<128, 128, 2, 4, 2> Alone;
@@ -658,7 +665,8 @@ __global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_gram_k
   gram_tile<G>(t, ws, local, f, odd, smem);
 }
 
-// adds the partial tiles of A, a workgroup per 32 x 32 block, in the order of the splits
+// Adds the partial tiles of A, a workgroup per 32 x 32 block, in the order of the splits.  Bound by memory: 8.5 us for the
+// 33 MB of 1024 x 9216, 3.9 TB/s.
 template <typename G>
 __global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict__ a, unsigned char* ws, float f) {
   constexpr int B = G::TN / 32, BB = (G::TM / 32) * B;
@@ -1120,7 +1128,7 @@ __global__ __launch_bounds__(256) void ortho_small_kernel(Mats a, MuonArgs u, fl
   for (int k = 0; k < MOST; ++k)
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += (double)v[k][e] * (double)v[k][e];
-  const float f = start_factor(block_sum(s, red), eps, scale);
+  const double f = start_factor(block_sum(s, red), eps, scale);
   for (int i = threadIdx.x; i < KB * 512; i += 256) reinterpret_cast<uint4*>(X)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
 #pragma unroll
@@ -1129,7 +1137,7 @@ __global__ __launch_bounds__(256) void ortho_small_kernel(Mats a, MuonArgs u, fl
     if (id >= chunks) continue;
     float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = v[k][e] * f;
+    for (int e = 0; e < 8; ++e) w[e] = (float)(f * (double)v[k][e]);
     uint4 hi, lo;
     split8(w, hi, lo);
     if (!t.flip) {      // row r, columns c ..: two chunks of 16 bytes (zeros past the end)
@@ -1215,7 +1223,7 @@ bool ortho_scales(const float* coeff, int steps, Scales* s) {
     s->a[k] = pow2_for(r * r);
     s->pa[k] = pow2_for(am * 1.01);
     s->p[k] = pow2_for(s->pmax[k]);
-    r = xm * 1.01;
+    r = xm * 1.001;       // (rounding; more would grow through steps such as s^5, which stay within 1)
   }
   return true;
 }
@@ -1237,11 +1245,12 @@ int tri(int m, int T) { const int n = cdiv(m, T); return n * (n + 1) / 2; }
 //
 // Steps in groups: with A = X X^T a step multiplies X by P = a I + b A + c A^2, and the next A is P A P.  Two steps then cost
 // one product each way with X and five with m x m matrices instead of two each way and two; three steps 1 + 1 and nine.
-// That pays where n >= 2 m.  Its price is rounding: A is not taken anew from X, so directions far below the largest lose
-// digits.  Measured against float64 on 12 kinds of spectra, 64 x 126 to 1024 x 9216, the error of groups of two stays within
-// 0.6 to 1.9 of what float32 products of single steps have (median 1.0), of groups of three within 0.6 to 3.9, but within
-// 1.0 from m = 512 on, where long float32 sums dominate; groups of five lose up to 100 times.  So: three from m = 512
-// on and for results that carry less (bfloat16; an update added to a parameter), else two.
+// That pays where n >= 2 m: 1024 x 9216 takes 708 us in single steps, 557 in twos, 481 in threes (with the tiles of that
+// time).  Its price is rounding: A is not taken anew from X, so directions far below the largest lose digits.  The error
+// against float64, over that of single steps with float32 products (six kinds of spectra, 64 x 126 to 1024 x 9216): single
+// 0.4 to 1.6; groups of two 0.4 to 2.1; of three 1.0 to 3.9 below m = 512, 0.6 to 1.2 from there on, where the long float32
+// sums dominate; of five up to 600.  So: three from m = 512 on and for results that carry less (bfloat16; an update added
+// to a parameter), else two.
 void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
   int64_t apply = 0, poly = 0, grams = 0;
   double long_ops = 0.0, square_ops = 0.0;
@@ -1263,9 +1272,11 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
     if (mmax <= 64 && nmax <= SMALL_N) p.mode = SMALL;
     else if (mmax <= 128) p.mode = CHAIN;
   }
-  // Few tiles: 64 x 64, to occupy CUs.  Else 128 rows, and for the products with X the width whose rounds of 512 workgroups
-  // make the least work: 9216 columns by 1024 rows are 576 tiles of 128 columns, two rounds, but 464 of 160, one.  A
-  // product with X^T splits its contraction to any number of workgroups.
+  // Few tiles: 64 x 64, to occupy CUs; fewer than 256 of 128 x 128 are few (Q X of 333 x 1000, 24: 13.5 us against 6.6; m x m
+  // products of 1024, 36: 28 against 11.3, of the filters of a whole model, 114: 31.6 against 20.2).  X X^T splits its
+  // contraction, at least eight blocks to a workgroup: 512 x 4608, 180 workgroups of 128 x 128, 12.1 us against 9.8, but
+  // 1024 x 9216, 512 of them, 32 against 41.  From 256 on 128 rows, and for Q X the width whose rounds of 512 workgroups make
+  // the least work: 9216 columns by 1024 rows are 576 tiles of 128 columns, two rounds, but 464 of 160, one.
   p.wg = mmax > 64 && (p.mode == CHAIN || grams >= 256) ? 128 : 64;
   p.wp = p.mode == CHAIN ? p.wg : poly >= 256 ? 128 : 64;
   p.wa = apply >= 256 ? 128 : 64;

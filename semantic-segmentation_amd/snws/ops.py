@@ -1251,7 +1251,7 @@ _HERE = contextlib.nullcontext()
 
 def on_device(t):
     """Context in which t's device is the current one, so that launches, streams and workspaces belong to it."""
-    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def stream_of(t):
@@ -1302,7 +1302,7 @@ def _ln_forward(x, w32, b32, eps, keep):
             if rows:
                 mp = stats.data_ptr()
                 rp = mp + 4 * rows
-        _launch("ln_fwd", 2.0 * x.element_size() * rows * C, "snws_ln_fwd", xs.data_ptr(), ldx,
+        _launch("ln_fwd", 0.0 if PROFILE is None else 2.0 * x.element_size() * rows * C, "snws_ln_fwd", xs.data_ptr(), ldx,
                 None if w32 is None else w32.data_ptr(), None if b32 is None else b32.data_ptr(), y.data_ptr(), C, _DT[x.dtype],
                 rows, C, eps, mp, rp, stream_of(x))
     return y, xs, ldx, stats
@@ -1315,8 +1315,9 @@ class LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, w32, b32, eps):
         y, xs, ctx.ldx, stats = _ln_forward(x, w32, b32, eps, True)
         ctx.save_for_backward(xs, w32, stats)
-        ctx.weight = None if weight is None else (grad_key(weight), weight.shape, weight.dtype)
-        ctx.bias = None if bias is None else (grad_key(bias), bias.shape, bias.dtype)
+        ctx.keys = grad_key(weight), grad_key(bias)
+        # parameters of another shape or type than the kernel's float32 (C,)
+        ctx.odd = [None if p is None or (p is q and p.dim() == 1) else (p.shape, p.dtype) for p, q in ((weight, w32), (bias, b32))]
         return y
 
     @staticmethod
@@ -1324,32 +1325,38 @@ class LayerNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         xs, w32, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        C, dev, dt = xs.shape[-1], xs.device, _DT[xs.dtype]
+        shape, dtype, dev = xs.shape, xs.dtype, xs.device
+        C, dt = shape[-1], _DT[dtype]
         with on_device(xs):
-            dys, lddy, rows = _as_rows(dy if dy.dtype is xs.dtype else dy.to(xs.dtype))
-            dx = torch.empty(xs.shape, dtype=xs.dtype, device=dev) if need_x else None
-            dw = grad_out(ctx.weight[0], (C,), dev) if need_w else None
-            db = grad_out(ctx.bias[0], (C,), dev) if need_b else None
-            part, n = None, 0
+            dys, lddy, rows = _as_rows(dy if dy.dtype is dtype else dy.to(dtype))
+            dx = dw = db = None
+            dxp = dwp = dbp = part = mp = rp = None
+            n = 0
+            if need_x:
+                dx = torch.empty(shape, dtype=dtype, device=dev)
+                dxp = dx.data_ptr()
+            if need_w:
+                dw = grad_out(ctx.keys[0], (C,), dev)
+                dwp = dw.data_ptr()
+            if need_b:
+                db = grad_out(ctx.keys[1], (C,), dev)
+                dbp = db.data_ptr()
             if need_w or need_b:
                 n = L.lib().snws_ln_bwd_workspace_floats(dt, rows, C)
-                part = torch.empty(n, dtype=torch.float32, device=dev)
-            mp = stats.data_ptr() if rows else None
-            _launch("ln_bwd", 3.0 * xs.element_size() * rows * C, "snws_ln_bwd", dys.data_ptr(), lddy, xs.data_ptr(), ctx.ldx,
-                    mp, mp + 4 * rows if rows else None, None if w32 is None else w32.data_ptr(), dt, rows, C,
-                    None if dx is None else dx.data_ptr(), C, None if dw is None else dw.data_ptr(),
-                    None if db is None else db.data_ptr(), None if part is None else part.data_ptr(), n, stream_of(xs))
-            return dx, _param_grad(dw, ctx.weight), _param_grad(db, ctx.bias), None, None, None
+                ws = torch.empty(n, dtype=torch.float32, device=dev)
+                part = ws.data_ptr()
+            if rows:
+                mp = stats.data_ptr()
+                rp = mp + 4 * rows
+            _launch("ln_bwd", 0.0 if PROFILE is None else 3.0 * xs.element_size() * rows * C, "snws_ln_bwd", dys.data_ptr(), lddy,
+                    xs.data_ptr(), ctx.ldx, mp, rp, None if w32 is None else w32.data_ptr(), dt, rows, C, dxp, C, dwp, dbp, part, n,
+                    stream_of(xs))
+            return dx, _param_grad(dw, ctx.odd[0]), _param_grad(db, ctx.odd[1]), None, None, None
 
 
-def _param_grad(g, param):
+def _param_grad(g, odd):
     g = grad_fold(g)
-    if g is None:
-        return None
-    _, shape, dtype = param
-    if g.shape != shape:
-        g = g.view(shape)
-    return g if g.dtype is dtype else g.to(dtype)
+    return g if g is None or odd is None else g.view(odd[0]).to(odd[1])
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -2349,13 +2356,13 @@ def _ortho_coefficients(coefficients, steps):
     return known
 
 
-def _ortho_workspace(rows, cols, steps, device):
+def _ortho_bytes(rows, cols, steps):
     n = len(rows)
     ints = ctypes.c_int * n
     nbytes = L.lib().snws_ortho_workspace_bytes(ints(*rows), ints(*cols), n, steps)
     if nbytes < 0:
         raise ValueError(L.lib().snws_last_error().decode("utf-8", "replace"))
-    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+    return nbytes
 
 
 def _ortho_flops(rows, cols, steps):
@@ -2424,7 +2431,8 @@ def _orthogonalize(mats, steps, coefficients, eps, out=None):
                 it.x, it.out, it.ldx, it.ldo, it.rows, it.cols = t.data_ptr(), out[live[k]].data_ptr(), ld if r > 1 else c, c, r, c
                 rows.append(r)
                 cols.append(c)
-            ws, nbytes = _ortho_workspace(rows, cols, steps, device)
+            nbytes = _ortho_bytes(rows, cols, steps)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
             _launch("orthogonalize", 0.0 if PROFILE is None else _ortho_flops(rows, cols, steps), "snws_orthogonalize", items, n,
                     dt, coeff, steps, float(eps), ws.data_ptr(), nbytes, stream_of(first))
     return out
@@ -2446,7 +2454,8 @@ def muon_update(params, grads, momentum_buffers, lr, weight_decay=0.1, momentum=
     taken together, so a filter (O, I, kh, kw) is an O x (I kh kw) matrix):
         m <- momentum m + (1 - momentum) g;  u = (1 - momentum) g + momentum m  (nesterov)  or  m;
         p <- (1 - lr weight_decay) p - lr factor orthogonalize(u),  factor: see muon_lr_factor.
-    g is grad_scale times the gradient.  Parameters and momentum buffers must be contiguous, and none may overlap another."""
+    g is grad_scale times the gradient.  Parameters and momentum buffers must be contiguous, and none may overlap another
+    tensor of the call."""
     params, grads, bufs = list(params), list(grads), list(momentum_buffers)
     if not (len(params) == len(grads) == len(bufs)):
         raise ValueError("muon_update: %d parameters, %d gradients, %d momentum buffers" % (len(params), len(grads), len(bufs)))
@@ -2456,7 +2465,7 @@ def muon_update(params, grads, momentum_buffers, lr, weight_decay=0.1, momentum=
     if not params:
         return
     device, f32 = params[0].device, torch.float32
-    live, spans, keep = [], [], []
+    live, spans = [], []
     for p, g, m in zip(params, grads, bufs):
         require_gpu(p, "muon_update")
         shape = p.shape
@@ -2470,21 +2479,29 @@ def muon_update(params, grads, momentum_buffers, lr, weight_decay=0.1, momentum=
             raise ValueError("muon_update: contiguous parameters and momentum buffers expected")
         n = p.numel()
         if n:
-            if not g.is_contiguous():
-                g = g.contiguous()
-                keep.append(g)
-            pp, mp = p.data_ptr(), m.data_ptr()
-            live.append((n, shape[0], n // shape[0], pp, g.data_ptr(), mp))
-            spans += ((pp, pp + 4 * n), (mp, mp + 4 * n))
+            g = g.contiguous()
+            pp, gp, mp = p.data_ptr(), g.data_ptr(), m.data_ptr()
+            live.append((n, shape[0], n // shape[0], pp, gp, mp, g))
+            spans += ((pp, pp + 4 * n, True), (mp, mp + 4 * n, True), (gp, gp + 4 * n, False))
     spans.sort()
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-        raise ValueError("muon_update: a parameter or momentum buffer is given twice, or overlaps another")
+    read = written = 0          # how far the gradients so far reach, and the tensors that are written
+    for lo, hi, out in spans:
+        if lo < written or (out and lo < read):
+            raise ValueError("muon_update: a parameter or momentum buffer is given twice, or overlaps another tensor")
+        if out:
+            written = hi
+        else:
+            read = max(read, hi)
     with on_device(params[0]):
+        calls = []
         for part in _by_size([t[0] for t in live]):
             part = [live[i] for i in part]
-            items = (L.MuonItem * len(part))(*[(pp, gp, mp, r, c, lr * muon_lr_factor(adjust_lr, r, c)) for _, r, c, pp, gp, mp in part])
             rows, cols = [t[1] for t in part], [t[2] for t in part]
-            ws, nbytes = _ortho_workspace(rows, cols, steps, device)
+            calls.append((part, rows, cols, _ortho_bytes(rows, cols, steps)))      # every size is checked before any update
+        for part, rows, cols, nbytes in calls:
+            items = (L.MuonItem * len(part))(*[(pp, gp, mp, r, c, lr * muon_lr_factor(adjust_lr, r, c))
+                                               for _, r, c, pp, gp, mp, _ in part])
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
             _launch("muon_update", 0.0 if PROFILE is None else _ortho_flops(rows, cols, steps), "snws_muon_update", items,
                     len(part), float(momentum), int(bool(nesterov)), float(grad_scale), lr * weight_decay, coeff, steps,
                     float(eps), ws.data_ptr(), nbytes, stream_of(params[0]))

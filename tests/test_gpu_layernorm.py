@@ -47,6 +47,15 @@ def test_entry_points_refuse_bad_arguments():
     assert L.lib().snws_ln_bwd_workspace_floats(L.SNWS_F32, 0, 8) == 0
 
 
+def test_entry_points_refuse_rows_beyond_their_counters():
+    P, C = 4096, (1 << 28) + 1
+    with pytest.raises(ValueError, match="sizes"):
+        L.call("snws_ln_fwd", P, C, None, None, P, C, L.SNWS_F32, 4, C, 1e-5, None, None, None)
+    with pytest.raises(ValueError, match="sizes"):
+        L.call("snws_ln_bwd", P, C, P, C, P, P, None, L.SNWS_F32, 4, C, P, C, P, P, P, 1 << 40, None)
+    assert L.lib().snws_ln_bwd_workspace_floats(L.SNWS_F32, 4, C) == 0
+
+
 def test_rows_of_strided_views():
     x = torch.zeros(3, 4, 10)
     assert ops._as_rows(x)[1:] == (10, 12)

@@ -305,3 +305,61 @@ def test_ortho_on_other_streams_and_in_graphs():
         torch.cuda.synchronize()
         for o, w in zip(outs, want):
             assert all(torch.equal(p, q) for p, q in zip(o, w)), it
+
+
+@gpu
+@pytest.mark.parametrize("coeff", [(1.5, 0.0, -0.5), (1.5, -0.5, 0.0), (0.0, 0.0, 1.0), (0.0, 1.0, 0.0), (-1.2, 0.4, 0.0)])
+@pytest.mark.parametrize("rows,cols", [(40, 90), (60, 500), (100, 300), (150, 700), (150, 160)])
+def test_coefficients_that_vanish(rows, cols, coeff):
+    """Zero coefficients in each way a call is run: one launch, chains of 64 and 128 rows, a launch for every product.
+    The bound: a step's three products in a row (A, A^2, B X) have an error of (8 + sqrt(n)) 2^-23 each, relative to
+    |a| + |b| r^2 + |c| r^4 times |X|, r the largest singular value; an error that is there grows by at most the largest
+    slope |a + 3 b s^2 + 5 c s^4| over [0, r] (an odd function of the singular values); stored numbers: see definition()."""
+    g = matrix(rows, cols)
+    a, b, c = coeff
+    x = g.double().cpu()
+    x = x / x.norm()
+    bound = 0.0
+    for _ in range(5):
+        r = float(torch.linalg.matrix_norm(x, 2))
+        s = torch.linspace(0.0, r * 1.01, 1001, dtype=torch.float64)
+        slope = float((a + 3 * b * s ** 2 + 5 * c * s ** 4).abs().max())
+        size = abs(a) + abs(b) * r ** 2 + abs(c) * r ** 4
+        bound = bound * slope + 3 * (8 + math.sqrt(cols)) * 2.0 ** -23 * size * float(x.norm())
+        bound += 2.0 ** -39 * math.sqrt(x.numel()) * max(size, 1.0)
+        gram = x @ x.t()
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    got = ops.orthogonalize(g, coefficients=coeff).double().cpu()
+    assert float((got - x).norm()) <= bound + 2.0 ** -24 * 1.01 * float(x.norm()), (float((got - x).norm()), bound)
+
+
+@gpu
+def test_orthogonalize_tiny_matrices_without_eps():
+    """Norms whose inverse leaves float32, in both ways a matrix is read."""
+    for rows, cols in ((30, 64), (64, 30), (70, 200), (200, 70)):
+        for scale in (1e-36, 2e-39):
+            g = matrix(rows, cols, scale=1.0) * scale
+            check(ops.orthogonalize(g, eps=0.0), g, eps=0.0)
+
+
+@gpu
+def test_muon_update_refuses_before_it_writes():
+    p, m = torch.ones(4, 9, device=DEV), torch.zeros(4, 9, device=DEV)
+    both = torch.zeros(2, 4, 9, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.muon_update([p], [both[0]], [both[0]], lr=0.1)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.muon_update([both[0]], [both.view(-1)[18:54].view(4, 9)], [m], lr=0.1)
+    assert not bool(both.any())
+    # 33 matrices are two calls, the larger ones first; the last one is too long: nothing may have happened by then
+    shapes = [(3, 1 << 20)] * 32 + [(2, (1 << 20) + 1)]
+    grads = [torch.ones(shapes[0], device=DEV)] * 32 + [torch.ones(shapes[-1], device=DEV)]
+    many, bufs = ([torch.zeros(t, device=DEV) for t in shapes] for _ in range(2))
+    with pytest.raises(ValueError, match="larger"):
+        ops.muon_update(many, grads, bufs, lr=0.1)
+    assert not any(bool(t.any()) for t in many + bufs)
+    del many, bufs, grads
+    # one gradient for two parameters is fine
+    q, mq = p.clone(), m.clone()
+    ops.muon_update([p, q], [both[1] + 1] * 2, [m, mq], lr=0.1)
+    assert torch.equal(p, q) and not bool((p == 1).any())
