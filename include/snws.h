@@ -457,7 +457,7 @@ int snws_ln_fwd(const void* x, int64_t ldx, const float* weight, const float* bi
                 int64_t rows, int C, float eps, float* mean, float* rstd, void* stream);
 /* With z = (x - mean) rstd and g = dy weight: dx = rstd (g - sum(g)/C - z sum(g z)/C) in dtype (NULL: not wanted);
  * dweight = sum over rows of dy z, dbias = sum of dy, f32 (C), overwritten (NULL: not wanted; zeros for rows == 0).
- * workspace: snws_ln_bwd_workspace_floats(...) floats when dweight or dbias is wanted; contents irrelevant.  The sums are
+ * workspace: snws_ln_bwd_workspace_floats(...) floats (0 for few rows) when dweight or dbias is wanted; contents irrelevant.  The sums are
  * taken in a fixed order. */
 int64_t snws_ln_bwd_workspace_floats(int dtype, int64_t rows, int C);
 int snws_ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* mean, const float* rstd,

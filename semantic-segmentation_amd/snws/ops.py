@@ -6,6 +6,7 @@ the kernels read.  Everything here requires a GPU tensor: there is no CPU path.
 """
 import contextlib
 import ctypes
+import functools
 import os
 
 import torch
@@ -1285,78 +1286,93 @@ def _param32(p, C, what, x):
         return None
     if p.numel() != C:
         raise ValueError("layer_norm: %s has %d elements for rows of %d" % (what, p.numel(), C))
-    if p.device != x.device:
+    if p.get_device() != x.get_device():
         raise RuntimeError("layer_norm: %s is on %s, the input on %s" % (what, p.device, x.device))
     return p if p.dtype is torch.float32 and p.is_contiguous() else _f32c(p)
 
 
 def _ln_forward(x, w32, b32, eps, keep):
-    """(y, x as read, its row stride, [mean | rstd] or None without `keep`)."""
-    with on_device(x):
-        xs, ldx, rows = _as_rows(x)
-        C = xs.shape[-1]
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = mp = rp = None
-        if keep:
-            stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device)
-            if rows:
-                mp = stats.data_ptr()
-                rp = mp + 4 * rows
-        _launch("ln_fwd", 0.0 if PROFILE is None else 2.0 * x.element_size() * rows * C, "snws_ln_fwd", xs.data_ptr(), ldx,
-                None if w32 is None else w32.data_ptr(), None if b32 is None else b32.data_ptr(), y.data_ptr(), C, _DT[x.dtype],
-                rows, C, eps, mp, rp, stream_of(x))
-    return y, xs, ldx, stats
+    """(y, x as read, its row stride, rows, [mean | rstd] or None without `keep`)."""
+    xs, ldx, rows = _as_rows(x)
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    C = shape[-1]
+    y = torch.empty(shape, dtype=dtype, device=dev)
+    stats = mp = rp = None
+    if keep:
+        stats = torch.empty(2 * rows, dtype=torch.float32, device=dev)
+        if rows:
+            mp = stats.data_ptr()
+            rp = mp + 4 * rows
+    _launch("ln_fwd", 0.0 if PROFILE is None else 2.0 * x.element_size() * rows * C, "snws_ln_fwd", xs.data_ptr(), ldx,
+            None if w32 is None else w32.data_ptr(), None if b32 is None else b32.data_ptr(), y.data_ptr(), C, _DT[dtype],
+            rows, C, eps, mp, rp, stream_of(x))
+    return y, xs, ldx, rows, stats
+
+
+@functools.lru_cache(maxsize=256)
+def _ln_workspace_floats(dt, rows, C):
+    return L.lib().snws_ln_bwd_workspace_floats(dt, rows, C)
+
+
+def _ln_backward(ctx, dy):
+    xs, w32 = ctx.saved_tensors
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    ldx, rows, stats, wkey, bkey, odd = ctx.kept
+    shape, dtype, dev = xs.shape, xs.dtype, xs.device
+    C, dt = shape[-1], _DT[dtype]
+    dys, lddy, _ = _as_rows(dy if dy.dtype is dtype else dy.to(dtype))
+    dx = dw = db = dxp = dwp = dbp = part = mp = rp = None
+    n = 0
+    if need_x:
+        dx = torch.empty(shape, dtype=dtype, device=dev)
+        dxp = dx.data_ptr()
+    if need_w or need_b:
+        if need_w:
+            dw = grad_out(wkey, (C,), dev)
+            dwp = dw.data_ptr()
+        if need_b:
+            db = grad_out(bkey, (C,), dev)
+            dbp = db.data_ptr()
+        n = _ln_workspace_floats(dt, rows, C)
+        if n:
+            ws = torch.empty(n, dtype=torch.float32, device=dev)
+            part = ws.data_ptr()
+    if rows:
+        mp = stats.data_ptr()
+        rp = mp + 4 * rows
+    _launch("ln_bwd", 0.0 if PROFILE is None else 3.0 * xs.element_size() * rows * C, "snws_ln_bwd", dys.data_ptr(), lddy,
+            xs.data_ptr(), ldx, mp, rp, None if w32 is None else w32.data_ptr(), dt, rows, C, dxp, C, dwp, dbp, part, n,
+            stream_of(xs))
+    dw, db = grad_fold(dw), grad_fold(db)
+    if odd is not None:         # parameters of another shape or type than the kernel's float32 (C,)
+        dw, db = (g if g is None or o is None else g.view(o[0]).to(o[1]) for g, o in zip((dw, db), odd))
+    return dx, dw, db, None, None, None
 
 
 class LayerNormFn(torch.autograd.Function):
-    """layer_norm with its gradients: one sweep over x and dy gives dx and the parameter gradients' partial sums."""
+    """layer_norm with its gradients: one sweep over x and dy gives dx and the parameter gradients' partial sums.  Small calls
+    are bound by the host, which crosses into the autograd engine's thread and back: what runs there is kept short."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, w32, b32, eps):
-        y, xs, ctx.ldx, stats = _ln_forward(x, w32, b32, eps, True)
-        ctx.save_for_backward(xs, w32, stats)
-        ctx.keys = grad_key(weight), grad_key(bias)
-        # parameters of another shape or type than the kernel's float32 (C,)
-        ctx.odd = [None if p is None or (p is q and p.dim() == 1) else (p.shape, p.dtype) for p, q in ((weight, w32), (bias, b32))]
+        y, xs, ldx, rows, stats = _ln_forward(x, w32, b32, eps, True)
+        ctx.save_for_backward(xs, w32)
+        odd = None
+        if (weight is not None and (weight is not w32 or weight.dim() != 1)) or \
+                (bias is not None and (bias is not b32 or bias.dim() != 1)):
+            odd = [None if p is None else (p.shape, p.dtype) for p in (weight, bias)]
+        ctx.kept = ldx, rows, stats, grad_key(weight), grad_key(bias), odd
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        xs, w32, stats = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        shape, dtype, dev = xs.shape, xs.dtype, xs.device
-        C, dt = shape[-1], _DT[dtype]
-        with on_device(xs):
-            dys, lddy, rows = _as_rows(dy if dy.dtype is dtype else dy.to(dtype))
-            dx = dw = db = None
-            dxp = dwp = dbp = part = mp = rp = None
-            n = 0
-            if need_x:
-                dx = torch.empty(shape, dtype=dtype, device=dev)
-                dxp = dx.data_ptr()
-            if need_w:
-                dw = grad_out(ctx.keys[0], (C,), dev)
-                dwp = dw.data_ptr()
-            if need_b:
-                db = grad_out(ctx.keys[1], (C,), dev)
-                dbp = db.data_ptr()
-            if need_w or need_b:
-                n = L.lib().snws_ln_bwd_workspace_floats(dt, rows, C)
-                ws = torch.empty(n, dtype=torch.float32, device=dev)
-                part = ws.data_ptr()
-            if rows:
-                mp = stats.data_ptr()
-                rp = mp + 4 * rows
-            _launch("ln_bwd", 0.0 if PROFILE is None else 3.0 * xs.element_size() * rows * C, "snws_ln_bwd", dys.data_ptr(), lddy,
-                    xs.data_ptr(), ctx.ldx, mp, rp, None if w32 is None else w32.data_ptr(), dt, rows, C, dxp, C, dwp, dbp, part, n,
-                    stream_of(xs))
-            return dx, _param_grad(dw, ctx.odd[0]), _param_grad(db, ctx.odd[1]), None, None, None
+        if torch.is_grad_enabled() or dy.get_device() != torch._C._cuda_getDevice():
+            with on_device(dy):
+                return _ln_backward_once(ctx, dy)
+        return _ln_backward(ctx, dy)
 
 
-def _param_grad(g, odd):
-    g = grad_fold(g)
-    return g if g is None or odd is None else g.view(odd[0]).to(odd[1])
+_ln_backward_once = torch.autograd.function.once_differentiable(_ln_backward)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -1370,10 +1386,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     dtype_code(x)
     eps = float(eps)
     w32, b32 = _param32(weight, x.shape[-1], "weight", x), _param32(bias, x.shape[-1], "bias", x)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
-        return LayerNormFn.apply(x, weight, bias, w32, b32, eps)
-    return _ln_forward(x, w32, b32, eps, False)[0]
+    with on_device(x):
+        if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                        (bias is not None and bias.requires_grad)):
+            return LayerNormFn.apply(x, weight, bias, w32, b32, eps)
+        return _ln_forward(x, w32, b32, eps, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------ autograd

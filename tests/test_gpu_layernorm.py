@@ -40,11 +40,14 @@ def test_entry_points_refuse_bad_arguments():
                             (11, 7, "sizes"), (0, None, "NULL"), (2, None, "NULL"), (4, None, "NULL"), (5, None, "NULL"),
                             (14, None, "workspace"), (15, 1, "workspace")):
         args = list(good)
+        args[8] = 4000 if text == "workspace" else args[8]        # (few rows need none)
         args[at] = value
         with pytest.raises(ValueError, match=text):
             L.call("snws_ln_bwd", *args)
     assert L.call("snws_ln_fwd", None, 8, None, None, None, 8, L.SNWS_F32, 0, 8, 1e-5, None, None, None) == 0
     assert L.lib().snws_ln_bwd_workspace_floats(L.SNWS_F32, 0, 8) == 0
+    assert L.lib().snws_ln_bwd_workspace_floats(L.SNWS_F32, 256, 8) == 0
+    assert L.lib().snws_ln_bwd_workspace_floats(L.SNWS_F32, 257, 8) > 0 and L.lib().snws_ln_bwd_workspace_floats(L.SNWS_BF16, 4, 3) > 0
 
 
 def test_entry_points_refuse_rows_beyond_their_counters():
@@ -313,3 +316,16 @@ def test_layer_norm_on_other_streams_and_in_a_graph():
         junk = torch.randn(1 << 20, device=DEV).sum()          # the program's own work between the replays
         torch.cuda.synchronize()
         assert math.isfinite(float(junk))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,C", [(1, 33), (2, 9216), (255, 8), (256, 100), (257, 100), (256, 31), (300, 1040), (30, 2048)])
+def test_layer_norm_every_choice_of_gradients(rows, C, dtype):
+    """Each of the seven sets of wanted gradients, on both sides of the row count up to which one launch does it all."""
+    x, w, b, dy = make(rows, C, dtype, pad=3)
+    for want in range(1, 8):
+        leaves = [t.detach().clone().requires_grad_(bool(want >> i & 1)) for i, t in enumerate((x, w, b))]
+        y = ops.layer_norm(*leaves)
+        grads = iter(torch.autograd.grad(y, [t for t in leaves if t.requires_grad], dy))
+        check(x, w, b, dy, 1e-5, y.detach(), *[next(grads) if t.requires_grad else None for t in leaves])
