@@ -17,9 +17,9 @@
 //
 // All matrices of a list share each launch: a workgroup finds its matrix and tile from its index.
 //
-// Measured, float32, five steps: 64 x 126 28 us (one launch), 1024 x 9216 365 us (norm 8, start 17, X X^T 32 and its join
-// 8.5 twice, 13 launches of m x m products at 11.3, Q X 55 and 61), the 21 million numbers of 18 filters with their Muon
-// update 715 us (46, 51, 61 and 10 twice, 13 x 20, 106 and 126).
+// Measured, float32, five steps: 64 x 126 28 us (one launch), 1024 x 9216 355 us (norm 8, start 16, X X^T 31.5 and its join
+// 8 twice, 13 launches of m x m products at 10.8, Q X 53 and 59), the 21 million numbers of 18 filters with their Muon
+// update 705 us (45, 52, 60 and 9.5 twice, 13 x 20, 105 and 125).
 #include "common.h"
 #include <math.h>
 
@@ -53,6 +53,14 @@ struct Mats {
   int end[PHASES][MAXM];      // first workgroup index behind each matrix, by the kind of launch
   int count;
   unsigned char* ws;
+};
+
+// What the other kernels get: the list's copy in the workspace, and the matrix itself where there is only one: no trip to
+// memory before the first copy, 0.4 us of each of the twenty launches.
+struct Work {
+  unsigned char* ws;
+  int count;
+  Mat only;
 };
 
 // D = ca I + cb C + cc P Q on the slots of every matrix (see square_tile), or a product with X
@@ -102,15 +110,35 @@ __device__ __forceinline__ unsigned xcd_order(unsigned bid, unsigned nblk) {
   return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
 }
 
-// Matrix of this workgroup and its index there.  Workgroups of one XCD (every eighth) get neighbouring indices within each
-// matrix: they share operands in its L2, and every XCD gets its share of every matrix.
-__device__ __forceinline__ int find_mat(const Mats& a, int phase, int& local) {
-  const int lane = threadIdx.x & 63, id = blockIdx.x;
-  const bool past = lane < a.count && id >= a.end[phase][lane];
-  const int i = __builtin_amdgcn_readfirstlane(__popcll(__ballot(past)));
-  const int from = i ? a.end[phase][i - 1] : 0;
-  local = xcd_order(id - from, a.end[phase][i] - from);
-  return i;
+// Matrix of this workgroup of a list, and its index there.  Workgroups of one XCD (every eighth) get neighbouring indices
+// within each matrix: they share operands in its L2, and every XCD gets its share of every matrix.  Every lane reads a matrix
+// of its own together with its end, so that the choice costs one trip to memory instead of two.
+__device__ __forceinline__ Mat pick_mat(const Mats& a, int count, int phase, int& local) {
+  constexpr int V = sizeof(Mat) / 16;
+  static_assert(sizeof(Mat) % 16 == 0, "whole vectors");
+  const int lane = threadIdx.x & 63, mine = lane < count ? lane : 0, id = blockIdx.x;
+  uint4 v[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = reinterpret_cast<const uint4*>(&a.mat[mine])[k];
+  const int end = a.end[phase][mine];
+  const int i = __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < count && id >= end)));
+  const int from = i ? __builtin_amdgcn_readlane(end, i - 1) : 0;
+  local = xcd_order(id - from, __builtin_amdgcn_readlane(end, i) - from);
+  union { Mat m; int w[4 * V]; } t;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    t.w[4 * k] = __builtin_amdgcn_readlane((int)v[k].x, i);
+    t.w[4 * k + 1] = __builtin_amdgcn_readlane((int)v[k].y, i);
+    t.w[4 * k + 2] = __builtin_amdgcn_readlane((int)v[k].z, i);
+    t.w[4 * k + 3] = __builtin_amdgcn_readlane((int)v[k].w, i);
+  }
+  return t.m;
+}
+// A matrix alone comes with the kernel's arguments.
+__device__ __forceinline__ Mat find_mat(const Work& a, int phase, int& local) {
+  if (a.count > 1) return pick_mat(*reinterpret_cast<const Mats*>(a.ws), a.count, phase, local);
+  local = xcd_order(blockIdx.x, gridDim.x);
+  return a.only;
 }
 
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
@@ -235,11 +263,13 @@ __device__ __forceinline__ double norm_chunk(const Mat& t, int chunk, const Muon
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ortho_norm_kernel(Mats a, MuonArgs u, double* __restrict__ partial) {
   __shared__ double red[16];
-  if (blockIdx.x == 0)
+  if (blockIdx.x == 0 && a.count > 1)
     for (int i = threadIdx.x; i < (int)(sizeof(Mats) / 4); i += 256)
       reinterpret_cast<int*>(a.ws)[i] = reinterpret_cast<const int*>(&a)[i];
   int chunk;
-  const Mat& t = a.mat[find_mat(a, NORM, chunk)];
+  Mat t = a.mat[0];
+  if (a.count > 1) t = pick_mat(a, a.count, NORM, chunk);
+  else chunk = blockIdx.x;
   const double s = block_sum(norm_chunk<T, MUON>(t, chunk, u), red);
   if (threadIdx.x == 0) partial[t.norm0 + chunk] = s;
 }
@@ -333,15 +363,15 @@ __device__ __forceinline__ double start_factor(double sum, float eps, float scal
 
 // X_0: the matrices, normalised
 template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void ortho_start_kernel(const Mats* __restrict__ a, unsigned char* ws, MuonArgs u,
+__global__ __launch_bounds__(256) void ortho_start_kernel(Work a, MuonArgs u,
                                                           const double* __restrict__ partial, float eps, float scale) {
   __shared__ float tile[64 * 66];
   __shared__ double red[16];
   int local;
-  const Mat& t = a->mat[find_mat(*a, START, local)];
+  const Mat t = find_mat(a, START, local);
   double s = 0.0;
   for (int i = threadIdx.x; i < t.normc; i += 256) s += partial[t.norm0 + i];
-  start_tile<T, MUON>(t, ws, local, start_factor(block_sum(s, red), eps, scale), u, tile);
+  start_tile<T, MUON>(t, a.ws, local, start_factor(block_sum(s, red), eps, scale), u, tile);
 }
 
 // ------------------------------------------------------------------------------------------------ products
@@ -361,12 +391,12 @@ struct Tile {
 };
 // Large tiles bring more products with each byte copied, small ones occupy more CUs.  Two workgroups on a CU take turns: one
 // multiplies while the other waits.
-// 128 x 128, four waves of 64 x 64, two workgroups to a CU: X X^T of 1024 x 9216 in 32 us, 0.9 PFLOP/s (64 x 64: 41 us)
+// 128 x 128, four waves of 64 x 64, two workgroups to a CU: X X^T of 1024 x 9216 in 31.5 us, 0.92 PFLOP/s (64 x 64: 41 us)
 typedef Tile<128, 128, 2, 2, 2> Big;
-// 128 x 160, four waves of 64 x 80, where that saves a round: Q X there in 55 us, 1.05 PFLOP/s (128 x 128: 67, 64 x 64: 74)
+// 128 x 160, four waves of 64 x 80, where that saves a round: Q X there in 53 us, 1.09 PFLOP/s (128 x 128: 67, 64 x 64: 74)
 typedef Tile<128, 160, 2, 2, 2> Wide;
 // 64 x 64, where there are few tiles; eight waves, so that each SIMD has two to alternate: a product of 1024 x 1024 in
-// 11.3 us (128 x 128: 28 us).  Of those about 4 are the launch, the first copies and the epilogue; in the rest the matrix
+// 10.8 us (128 x 128: 28 us).  Of those about 4 are the launch, the first copies and the epilogue; in the rest the matrix
 // units are busy for 2.6: the operands come from beyond the L2s, of which each needs half the matrix: 26 MB, 5 us.  A
 // deeper ring or a barrier for every second stage only change nothing.
 typedef Tile<64, 64, 2, 4, 4> Fine;
@@ -665,21 +695,21 @@ __device__ __forceinline__ void gram_tile(const Mat& t, unsigned char* ws, int l
 }
 
 template <typename G>
-__global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_gram_kernel(const Mats* __restrict__ a, unsigned char* ws, float f, int odd) {
+__global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_gram_kernel(Work a, float f, int odd) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   int local;
-  const Mat& t = a->mat[find_mat(*a, GRAM, local)];
-  gram_tile<G>(t, ws, local, f, odd, smem);
+  const Mat t = find_mat(a, GRAM, local);
+  gram_tile<G>(t, a.ws, local, f, odd, smem);
 }
 
-// Adds the partial tiles of A, a workgroup per 32 x 32 block, in the order of the splits.  Bound by memory: 8.5 us for the
-// 33 MB of 1024 x 9216, 3.9 TB/s.
+// Adds the partial tiles of A, a workgroup per 32 x 32 block, in the order of the splits.  Bound by memory: 8 us for the
+// 33 MB of 1024 x 9216, 4.1 TB/s.
 template <typename G>
-__global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict__ a, unsigned char* ws, float f) {
+__global__ __launch_bounds__(256) void ortho_join_kernel(Work a, float f) {
   constexpr int B = G::TN / 32, BB = (G::TM / 32) * B;
   __shared__ float tile[32 * 34];
   int local, p0, q0;
-  const Mat& t = a->mat[find_mat(*a, JOIN, local)];
+  const Mat t = find_mat(a, JOIN, local);
   const int tl = local / BB, sub = local % BB;
   place<G>(tl, t.m, p0, q0);
   const bool diagonal = p0 == q0;
@@ -689,7 +719,7 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict_
   if (p0 >= mp || q0 >= mp) return;
   // the four 16 x 16 blocks (r, c) of this one, a wave each
   const int r16 = (sub / B) * 2 + (threadIdx.x >> 7), c16 = (sub % B) * 2 + (threadIdx.x >> 6 & 1), lane = threadIdx.x & 63;
-  const f32x4* part = part_of(t, ws) + (int64_t)tl * t.ks * (G::TM * G::TN / 4) + (r16 * (G::TN / 16) + c16) * 64 + lane;
+  const f32x4* part = part_of(t, a.ws) + (int64_t)tl * t.ks * (G::TM * G::TN / 4) + (r16 * (G::TN / 16) + c16) * 64 + lane;
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int k = 0; k < t.ks; ++k) s += part[(int64_t)k * (G::TM * G::TN / 4)];
@@ -697,7 +727,7 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(const Mats* __restrict_
 #pragma unroll
   for (int e = 0; e < 4; ++e) tile[(pr + e) * 34 + qc] = p0 + pr + e < t.m && q0 + qc < t.m ? s[e] * f : 0.f;
   __syncthreads();
-  unsigned char* A = slot_of(t, ws, 0);
+  unsigned char* A = slot_of(t, a.ws, 0);
   const int id = threadIdx.x & 127, r = id >> 2, c = (id & 3) * 8;
   float v[8];
   if (threadIdx.x < 128) {
@@ -744,11 +774,11 @@ __device__ __forceinline__ void square_tile(const Mat& t, unsigned char* ws, int
 
 // one or two operations that do not depend on each other: gridDim.y of them
 template <typename G>
-__global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_square_kernel(const Mats* __restrict__ a, unsigned char* ws, Op first, Op second) {
+__global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_square_kernel(Work a, Op first, Op second) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   int local;
-  const Mat& t = a->mat[find_mat(*a, SQUARE, local)];
-  square_tile<G>(t, ws, local, blockIdx.y ? second : first, smem);
+  const Mat t = find_mat(a, SQUARE, local);
+  square_tile<G>(t, a.ws, local, blockIdx.y ? second : first, smem);
 }
 
 // eight consecutive results at (r, c) of the source's orientation, as many as lie within `cols`: 16-byte accesses of any
@@ -815,12 +845,12 @@ __device__ __forceinline__ void apply_tile(const Mat& t, unsigned char* ws, int 
 }
 
 template <typename G, typename T, bool LAST, bool MUON>
-__global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_apply_kernel(const Mats* __restrict__ a, unsigned char* ws, MuonArgs u, int sq, float f,
+__global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_apply_kernel(Work a, MuonArgs u, int sq, float f,
                                                              int odd) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   int local;
-  const Mat& t = a->mat[find_mat(*a, APPLY, local)];
-  apply_tile<G, T, LAST, MUON>(t, ws, local, u, sq, f, odd, smem);
+  const Mat t = find_mat(a, APPLY, local);
+  apply_tile<G, T, LAST, MUON>(t, a.ws, local, u, sq, f, odd, smem);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -830,7 +860,7 @@ __device__ __forceinline__ void phase_done() {
   __syncthreads();
 }
 
-// a value that lies in LDS, the same for all lanes, in scalar registers
+// a value in memory, the same for all lanes, in scalar registers
 template <typename V>
 __device__ __forceinline__ V uniform(const V* p) {
   static_assert(sizeof(V) % 4 == 0, "whole words");
@@ -861,21 +891,21 @@ __device__ __forceinline__ void add_parts(f32x4 (&acc)[M][N], const Mat& t, unsi
 
 // The m x m operations of a group for matrices of 65 to 128 rows, a workgroup each, instead of a launch for every operation;
 // the partial tiles of A are added up on the way.
-__global__ __launch_bounds__(Alone::THREADS) void ortho_chain128_kernel(const Mats* __restrict__ a, unsigned char* ws, float f,
+__global__ __launch_bounds__(Alone::THREADS) void ortho_chain128_kernel(Work a, float f,
                                                                         Program prog) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ Program kept;
   keep(&kept, prog);
-  const Mat& t = a->mat[blockIdx.x];
+  const Mat t = a.count > 1 ? uniform(&reinterpret_cast<const Mats*>(a.ws)->mat[blockIdx.x]) : a.only;
   __syncthreads();
   if (t.ks > 1) {
     f32x4 acc[Alone::MR][Alone::NR];
-    add_parts<128, Alone::WN>(acc, t, ws);
-    put_symmetric<Alone>(acc, f, t, slot_of(t, ws, 0), 0, 0, smem);
+    add_parts<128, Alone::WN>(acc, t, a.ws);
+    put_symmetric<Alone>(acc, f, t, slot_of(t, a.ws, 0), 0, 0, smem);
     phase_done();
   }
   for (int k = 0; k < prog.n; ++k) {
-    square_tile<Alone>(t, ws, 0, uniform(&kept.op[k]), smem);
+    square_tile<Alone>(t, a.ws, 0, uniform(&kept.op[k]), smem);
     phase_done();
   }
 }
@@ -964,17 +994,17 @@ __device__ __forceinline__ void square64(const Op& op, int m, unsigned char* slo
 }
 
 // The m x m operations of a group for matrices of up to 64 rows; the last slot written is Q, which goes to global memory.
-__global__ __launch_bounds__(256) void ortho_chain64_kernel(const Mats* __restrict__ a, unsigned char* ws, float f, Program prog) {
+__global__ __launch_bounds__(256) void ortho_chain64_kernel(Work a, float f, Program prog) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ Program kept;
   keep(&kept, prog);
-  const Mat& t = a->mat[blockIdx.x];
+  const Mat t = a.count > 1 ? uniform(&reinterpret_cast<const Mats*>(a.ws)->mat[blockIdx.x]) : a.only;
   const Lane64 L;
   const int m = t.m, nb = up32(m) >> 5;
-  unsigned char* A = slot_of(t, ws, 0);
+  unsigned char* A = slot_of(t, a.ws, 0);
   if (t.ks > 1) {
     f32x4 acc[2][2];
-    add_parts<64, 2>(acc, t, ws);
+    add_parts<64, 2>(acc, t, a.ws);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -997,7 +1027,7 @@ __global__ __launch_bounds__(256) void ortho_chain64_kernel(const Mats* __restri
     square64(op, m, smem, L);
     last = op.sd;
   }
-  unsigned char* Q = slot_of(t, ws, last);
+  unsigned char* Q = slot_of(t, a.ws, last);
   for (int id = threadIdx.x; id < m * nb * 8; id += 256) {
     const int r = id / (nb * 8), b = (id >> 3) % nb, c = id & 7;
     *reinterpret_cast<uint4*>(Q + ((int64_t)r * nb + b) * 128 + c * 16) =
@@ -1280,7 +1310,7 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
     else if (mmax <= 128) p.mode = CHAIN;
   }
   // Few tiles: 64 x 64, to occupy CUs; fewer than 256 of 128 x 128 are few (Q X of 333 x 1000, 24: 13.5 us against 6.6; m x m
-  // products of 1024, 36: 28 against 11.3, of the filters of a whole model, 114: 31.6 against 20.2).  X X^T splits its
+  // products of 1024, 36: 28 against 11, of the filters of a whole model, 114: 31.6 against 20.2).  X X^T splits its
   // contraction, at least eight blocks to a workgroup: 512 x 4608, 180 workgroups of 128 x 128, 12.1 us against 9.8, but
   // 1024 x 9216, 512 of them, 32 against 41.  From 256 on 128 rows, and for Q X the width whose rounds of 512 workgroups make
   // the least work: 9216 columns by 1024 rows are 576 tiles of 128 columns, two rounds, but 464 of 160, one.
@@ -1360,15 +1390,15 @@ struct Run {
   const char* what;
   hipStream_t st;
   unsigned grid(Phase k) const { return (unsigned)a.end[k][a.count - 1]; }
-  const Mats* table() const { return reinterpret_cast<const Mats*>(a.ws); }
+  Work work() const { return Work{a.ws, a.count, a.mat[0]}; }
 
   template <typename G>
   int gram(float f, int odd) const {
     ORTHO_TRY((ready<&ortho_gram_kernel<G>>(G::LDS, what)));
-    ortho_gram_kernel<G><<<grid(GRAM), G::THREADS, G::LDS, st>>>(table(), a.ws, f, odd);
+    ortho_gram_kernel<G><<<grid(GRAM), G::THREADS, G::LDS, st>>>(work(), f, odd);
     SNWS_LAUNCH_CHECK(what);
     if (p.mode == GENERAL && grid(JOIN)) {
-      ortho_join_kernel<G><<<grid(JOIN), 256, 0, st>>>(table(), a.ws, f);
+      ortho_join_kernel<G><<<grid(JOIN), 256, 0, st>>>(work(), f);
       SNWS_LAUNCH_CHECK(what);
     }
     return SNWS_OK;
@@ -1376,17 +1406,17 @@ struct Run {
   template <typename G>
   int squares(const Op& first, const Op* second) const {
     ORTHO_TRY((ready<&ortho_square_kernel<G>>(G::LDS, what)));
-    ortho_square_kernel<G><<<dim3(grid(SQUARE), second ? 2 : 1), G::THREADS, G::LDS, st>>>(table(), a.ws, first, second ? *second : first);
+    ortho_square_kernel<G><<<dim3(grid(SQUARE), second ? 2 : 1), G::THREADS, G::LDS, st>>>(work(), first, second ? *second : first);
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
   }
   int chain(float f, const Program& prog) const {
     if (p.wg == 128) {
       ORTHO_TRY((ready<&ortho_chain128_kernel>(Alone::LDS, what)));
-      ortho_chain128_kernel<<<(unsigned)a.count, Alone::THREADS, Alone::LDS, st>>>(table(), a.ws, f, prog);
+      ortho_chain128_kernel<<<(unsigned)a.count, Alone::THREADS, Alone::LDS, st>>>(work(), f, prog);
     } else {
       ORTHO_TRY((ready<&ortho_chain64_kernel>(SLOTS * SLOT64, what)));
-      ortho_chain64_kernel<<<(unsigned)a.count, 256, SLOTS * SLOT64, st>>>(table(), a.ws, f, prog);
+      ortho_chain64_kernel<<<(unsigned)a.count, 256, SLOTS * SLOT64, st>>>(work(), f, prog);
     }
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
@@ -1394,7 +1424,7 @@ struct Run {
   template <typename G, typename T, bool LAST, bool MUON>
   int apply_by(const Op& op, int odd) const {
     ORTHO_TRY((ready<&ortho_apply_kernel<G, T, LAST, MUON>>(G::LDS, what)));
-    ortho_apply_kernel<G, T, LAST, MUON><<<grid(APPLY), G::THREADS, G::LDS, st>>>(table(), a.ws, u, op.sq, op.cc, odd);
+    ortho_apply_kernel<G, T, LAST, MUON><<<grid(APPLY), G::THREADS, G::LDS, st>>>(work(), u, op.sq, op.cc, odd);
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
   }
@@ -1468,7 +1498,7 @@ int run_all(const Mats& a, const Plan& p, const MuonArgs& u, const float* coeff,
   double* partial = reinterpret_cast<double*>(a.ws + p.norms);
   ortho_norm_kernel<T, MUON><<<run.grid(NORM), 256, 0, st>>>(a, u, partial);
   SNWS_LAUNCH_CHECK(what);
-  ortho_start_kernel<T, MUON><<<run.grid(START), 256, 0, st>>>(run.table(), a.ws, u, partial, eps, (float)s.x[0]);
+  ortho_start_kernel<T, MUON><<<run.grid(START), 256, 0, st>>>(run.work(), u, partial, eps, (float)s.x[0]);
   SNWS_LAUNCH_CHECK(what);
   int odd = 0;
   for (int k = 0; k < steps;) {
