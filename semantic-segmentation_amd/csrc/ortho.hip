@@ -19,7 +19,7 @@
 //
 // Measured, float32, five steps: 64 x 126 28 us (one launch), 1024 x 9216 355 us (norm 8, start 16, X X^T 31.5 and its join
 // 8 twice, 13 launches of m x m products at 10.8, Q X 53 and 59), the 21 million numbers of 18 filters with their Muon
-// update 705 us (45, 52, 60 and 9.5 twice, 13 x 20, 105 and 125).
+// update 700 us (45, 52, 60 and 9.5 twice, 13 x 18.5, 105 and 125).
 #include "common.h"
 #include <math.h>
 
@@ -400,6 +400,8 @@ typedef Tile<128, 160, 2, 2, 2> Wide;
 // units are busy for 2.6: the operands come from beyond the L2s, of which each needs half the matrix: 26 MB, 5 us.  A
 // deeper ring or a barrier for every second stage only change nothing.
 typedef Tile<64, 64, 2, 4, 4> Fine;
+// 96 x 64, four waves of 48 x 32, for m x m products where that makes fewer rounds
+typedef Tile<96, 64, 2, 2, 4> Tall;
 // 128 x 128 by one workgroup alone
 typedef Tile<128, 128, 2, 4, 2> Alone;
 
@@ -643,14 +645,33 @@ __device__ __forceinline__ void triangle(int t, int nt, int& i, int& j) {
   }
 }
 
+// Tiles half as high again as wide: strip i needs columns up to its own end, 3 (i + 1) / 2 tiles; two strips together, column
+// by column.
+__device__ __forceinline__ void tall_triangle(int t, int rows, int cols, int& i, int& j) {
+  int I = (int)((sqrtf(1.f + 3.f * (float)t) - 1.f) * 0.33333333f);      // 3 I^2 + 2 I tiles lie before strip 2 I
+  while (3 * (I + 1) * (I + 1) + 2 * (I + 1) <= t) ++I;
+  while (3 * I * I + 2 * I > t) --I;
+  const int rem = t - 3 * I * I - 2 * I, first = 3 * I + 2 < cols ? 3 * I + 2 : cols;
+  const bool alone = 2 * I + 1 >= rows, both = !alone && rem < 2 * first;
+  i = alone ? 2 * I : both ? 2 * I + (rem & 1) : 2 * I + 1;
+  j = alone ? rem : both ? rem >> 1 : rem - first;
+}
+
 template <typename G>
 __device__ __forceinline__ void place(int t, int m, int& p0, int& q0) {
-  static_assert(G::TM == G::TN && G::TM == G::SLAB, "symmetric matrices: square tiles of one slab");
+  static_assert((G::TM == G::TN || 2 * G::TM == 3 * G::TN) && G::TM == G::SLAB, "symmetric matrices: tiles of one slab");
   int i, j;
-  triangle(t, (m + G::TM - 1) / G::TM, i, j);
+  if (G::TM == G::TN) triangle(t, (m + G::TM - 1) / G::TM, i, j);
+  else tall_triangle(t, (m + G::TM - 1) / G::TM, (m + G::TN - 1) / G::TN, i, j);
   p0 = i * G::TM;
   q0 = j * G::TN;
 }
+
+// Of a symmetric matrix a tile stores what lies left of its strip's end, and the mirror image of what lies left of its strip.
+template <typename G>
+__device__ __forceinline__ bool own(int p0, int col) { return G::TM == G::TN || col < p0 + G::TM; }
+template <typename G>
+__device__ __forceinline__ bool mirrored(int p0, int col) { return G::TM == G::TN || col < p0; }
 
 // a tile, times f, into the symmetric matrix D, and its mirror image
 template <typename G>
@@ -660,11 +681,11 @@ __device__ __forceinline__ void put_symmetric(const f32x4 (&acc)[G::MR][G::NR], 
   const int mp = up32(t.m);
   to_lds<G>(acc, f, 0, p0, q0, t.m, t.m, tile);
   by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) {
-    if (p0 + p < t.m && q0 + q < mp) store8(D + (int64_t)(p0 + p) * mp * 4, q0 + q, v);
+    if (p0 + p < t.m && q0 + q < mp && own<G>(p0, q0 + q)) store8(D + (int64_t)(p0 + p) * mp * 4, q0 + q, v);
   });
-  if (p0 != q0)
+  if (q0 < p0)
     by_cols<G>(tile, [&](int q, int p, const float (&v)[8]) {
-      if (q0 + q < t.m && p0 + p < mp) store8(D + (int64_t)(q0 + q) * mp * 4, p0 + p, v);
+      if (q0 + q < t.m && p0 + p < mp && mirrored<G>(p0, q0 + q)) store8(D + (int64_t)(q0 + q) * mp * 4, p0 + p, v);
     });
 }
 
@@ -768,8 +789,13 @@ __device__ __forceinline__ void square_tile(const Mat& t, unsigned char* ws, int
     for (int e = 0; e < 8; ++e) w[e] = v[e] + op.cb * w[e] + (r == c + e ? op.ca : 0.f);
     store8(D + (int64_t)r * mp * 4, c, w);
   };
-  by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) { put(p0 + p, q0 + q, v); });
-  if (p0 != q0) by_cols<G>(tile, [&](int q, int p, const float (&v)[8]) { put(q0 + q, p0 + p, v); });
+  by_rows<G>(tile, [&](int p, int q, const float (&v)[8]) {
+    if (own<G>(p0, q0 + q)) put(p0 + p, q0 + q, v);
+  });
+  if (q0 < p0)
+    by_cols<G>(tile, [&](int q, int p, const float (&v)[8]) {
+      if (mirrored<G>(p0, q0 + q)) put(q0 + q, p0 + p, v);
+    });
 }
 
 // one or two operations that do not depend on each other: gridDim.y of them
@@ -1271,12 +1297,22 @@ enum Mode { GENERAL, CHAIN, SMALL };
 
 struct Plan {
   Mode mode;
-  int wg, wp, wa;              // columns of the tiles of the three kinds of products: 64, 128, or 160
+  int wg, wp, wa;              // tiles of the three kinds of products: 64 and 128 square, 96 x 64, 128 x 160
   int group;                   // steps taken together
   int64_t bytes, norms;        // of the workspace; where the partial sums of squares begin
 };
 
 int tri(int m, int T) { const int n = cdiv(m, T); return n * (n + 1) / 2; }
+// tiles of an m x m product by the rows of a tile: 64 or 128 (square), or 96 (by 64)
+int square_tiles(int m, int T) {
+  if (T != 96) return tri(m, T);
+  int n = 0;
+  for (int i = 0; 96 * i < m; ++i) {
+    const int end = 96 * (i + 1) < m ? 96 * (i + 1) : m;
+    n += cdiv(end, 64);
+  }
+  return n;
+}
 
 // Places the workspace, chooses mode, tiles and splits, and counts workgroups.
 //
@@ -1289,12 +1325,11 @@ int tri(int m, int T) { const int n = cdiv(m, T); return n * (n + 1) / 2; }
 // sums dominate; of five up to 600.  So: three from m = 512 on and for results that carry less (bfloat16; an update added
 // to a parameter), else two.
 void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
-  int64_t apply = 0, poly = 0, grams = 0;
+  int64_t apply = 0, grams = 0;
   double long_ops = 0.0, square_ops = 0.0;
   int mmax = 0, mmin = 1 << 30, nmax = 0;
   for (int i = 0; i < a.count; ++i) {
     const Mat& t = a.mat[i];
-    poly += tri(t.m, 128);
     grams += tri(t.m, 128) * cdiv64(up32(t.n) >> 5, 8);
     apply += (int64_t)cdiv(t.m, 128) * cdiv(t.n, 128);
     mmax = t.m > mmax ? t.m : mmax;
@@ -1309,13 +1344,28 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
     if (mmax <= 64 && nmax <= SMALL_N) p.mode = SMALL;
     else if (mmax <= 128) p.mode = CHAIN;
   }
-  // Few tiles: 64 x 64, to occupy CUs; fewer than 256 of 128 x 128 are few (Q X of 333 x 1000, 24: 13.5 us against 6.6; m x m
-  // products of 1024, 36: 28 against 11, of the filters of a whole model, 114: 31.6 against 20.2).  X X^T splits its
-  // contraction, at least eight blocks to a workgroup: 512 x 4608, 180 workgroups of 128 x 128, 12.1 us against 9.8, but
-  // 1024 x 9216, 512 of them, 32 against 41.  From 256 on 128 rows, and for Q X the width whose rounds of 512 workgroups make
-  // the least work: 9216 columns by 1024 rows are 576 tiles of 128 columns, two rounds, but 464 of 160, one.
+  // Few tiles: 64 x 64, to occupy CUs; fewer than 256 of 128 x 128 are few (Q X of 333 x 1000, 24: 13.5 us against 6.6).
+  // X X^T splits its contraction, at least eight blocks to a workgroup: 512 x 4608, 180 workgroups of 128 x 128, 12.1 us
+  // against 9.8, but 1024 x 9216, 512 of them, 32 against 41.  From 256 on 128 rows, and for Q X the width whose rounds of 512
+  // workgroups make the least work: 9216 columns by 1024 rows are 576 tiles of 128 columns, two rounds, but 464 of 160, one.
   p.wg = mmax > 64 && (p.mode == CHAIN || grams >= 256) ? 128 : 64;
-  p.wp = p.mode == CHAIN ? p.wg : poly >= 256 ? 128 : 64;
+  p.wp = p.wg;
+  if (p.mode == GENERAL) {
+    // Products of m x m matrices take as long as the CU with the most tiles.  In units of a 64 x 64 tile, one of 96 x 64 takes
+    // 1.5, one of 128 x 128 3.7, and two of these, that share a CU, 5.9; a tile of a smaller matrix counts by its share of the
+    // longest contraction.  Whole calls of m x 2 m with 64, 96, 128 rows (us): m = 1100 283, 296, 508; 1409 475, 425, 665;
+    // 1800 654, 692, 867; 2200 1133, 1047, 1242; 2750 1859, 1922, 1747; 3700 4192, 4038, 3568; 4096 6168, 5649, 6020.
+    double n64 = 0.0, n96 = 0.0, n128 = 0.0;
+    for (int i = 0; i < a.count; ++i) {
+      const double share = (double)a.mat[i].m / mmax;
+      n64 += square_tiles(a.mat[i].m, 64) * share;
+      n96 += square_tiles(a.mat[i].m, 96) * share;
+      n128 += square_tiles(a.mat[i].m, 128) * share;
+    }
+    const double c64 = ceil(n64 / 256), c96 = 1.5 * ceil(n96 / 256), left = fmod(n128, 512.0);
+    const double c128 = 5.9 * floor(n128 / 512) + (left > 256.0 ? 5.9 : left > 0.0 ? 3.7 : 0.0);
+    p.wp = c128 <= c96 && c128 <= c64 ? 128 : c96 <= c64 ? 96 : 64;
+  }
   p.wa = apply >= 256 ? 128 : 64;
   if (apply >= 256) {
     int64_t wide = 0;
@@ -1353,7 +1403,7 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
     off = (off + 255) & ~(int64_t)255;
     const int B = (T / 32) * (T / 32);
     const int64_t n[PHASES] = {t.normc, (int64_t)cdiv(t.m, 64) * cdiv(t.n, 64), (int64_t)tri(t.m, T) * t.ks,
-                               t.ks > 1 ? (int64_t)tri(t.m, T) * B : 0, tri(t.m, p.wp),
+                               t.ks > 1 ? (int64_t)tri(t.m, T) * B : 0, square_tiles(t.m, p.wp),
                                (int64_t)cdiv(t.m, AM) * cdiv(t.n, AN)};
     for (int k2 = 0; k2 < PHASES; ++k2) a.end[k2][i] = (int)n[k2] + (i ? a.end[k2][i - 1] : 0);
   }
@@ -1515,7 +1565,8 @@ int run_all(const Mats& a, const Plan& p, const MuonArgs& u, const float* coeff,
         // P A and P Q read the same matrices and write different ones: one launch for both
         const bool both = i + 2 < n && op[i].cb == 0.f && op[i + 1].cb == 0.f && op[i + 1].sp != op[i].sd && op[i + 1].sq != op[i].sd;
         const Op* second = both ? &op[i + 1] : nullptr;
-        ORTHO_TRY(p.wp == 128 ? run.squares<Big>(op[i], second) : run.squares<Fine>(op[i], second));
+        ORTHO_TRY(p.wp == 128 ? run.squares<Big>(op[i], second) : p.wp == 96 ? run.squares<Tall>(op[i], second)
+                                                                             : run.squares<Fine>(op[i], second));
         if (both) ++i;
       }
     }

@@ -363,3 +363,13 @@ def test_muon_update_refuses_before_it_writes():
     q, mq = p.clone(), m.clone()
     ops.muon_update([p, q], [both[1] + 1] * 2, [m, mq], lr=0.1)
     assert torch.equal(p, q) and not bool((p == 1).any())
+
+
+@gpu
+@pytest.mark.parametrize("sizes", [[(1500, 1530)], [(1409, 3000)], [(2100, 1441)], [(2200, 2210)], [(2790, 2800)], [(1030, 2070), (1024, 1024), (1000, 2500), (70, 90)]])
+def test_orthogonalize_sizes_by_tile(sizes):
+    """Sizes whose m x m products take tiles of 96 x 64 and 128 x 128."""
+    mats = [matrix(r, c) for r, c in sizes]
+    for got, g in zip(ops.orthogonalize(mats), mats):
+        check(got, g)
+    assert all(torch.equal(p, q) for p, q in zip(ops.orthogonalize(mats), ops.orthogonalize(mats)))
