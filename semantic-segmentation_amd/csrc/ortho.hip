@@ -19,7 +19,7 @@
 //
 // Measured, float32, five steps: 64 x 126 28 us (one launch), 1024 x 9216 355 us (norm 8, start 16, X X^T 31.5 and its join
 // 8 twice, 13 launches of m x m products at 10.8, Q X 53 and 59), the 21 million numbers of 18 filters with their Muon
-// update 700 us (45, 52, 60 and 9.5 twice, 13 x 18.5, 105 and 125).
+// update 700 us (45, 52, 60 and 9.5 twice, 13 x 19, 105 and 125).
 #include "common.h"
 #include <math.h>
 
