@@ -18,7 +18,7 @@
 // All matrices of a list share each launch: a workgroup finds its matrix and tile from its index.
 //
 // Measured, float32, five steps: 64 x 126 28 us (one launch), 1024 x 9216 355 us (norm 8, start 16, X X^T 31.5 and its join
-// 8 twice, 13 launches of m x m products at 10.8, Q X 53 and 59), the 21 million numbers of 18 filters with their Muon
+// 8 twice, 13 launches of m x m products at 10.8, Q X 53 and 59), the 21 million numbers of 17 filters with their Muon
 // update 700 us (45, 52, 60 and 9.5 twice, 13 x 19, 105 and 125).
 #include "common.h"
 #include <math.h>
@@ -938,7 +938,7 @@ __global__ __launch_bounds__(Alone::THREADS) void ortho_chain128_kernel(Work a, 
 
 // Up to 64 rows the m x m matrices stay in LDS, 16 KB each: slot k, 32-column block b, row r, 16-byte chunks as in the
 // stages of product().  A workgroup computes the whole 64 x 64 product, and a lane's four rows of one column are, by
-// symmetry, four columns of one row: they go back without any transposition.  An operation takes 0.4 us this way,
+// symmetry, four columns of one row: they go back without any transposition.  An operation takes 1.3 us this way,
 // 2.7 us through global memory.
 constexpr int SLOT64 = 64 * 2 * 128;
 
