@@ -1379,7 +1379,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (..., C), float32 or bfloat16; mean and
     variance (biased) in float32 over each position's own C elements.  weight / bias: C values (kept in float32) or None.
     Leading axes may be strided like a channel slice of a wider buffer; the result is contiguous.  Differentiable once
-    in x, weight and bias."""
+    in x, weight and bias.  (Before a backward pass is captured into a graph, let go of earlier graphs of the same leaves.)"""
     require_gpu(x, "layer_norm")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("layer_norm: a last axis of at least one element expected, got shape %s" % (tuple(x.shape),))
@@ -2472,7 +2472,7 @@ def muon_update(params, grads, momentum_buffers, lr, weight_decay=0.1, momentum=
         m <- momentum m + (1 - momentum) g;  u = (1 - momentum) g + momentum m  (nesterov)  or  m;
         p <- (1 - lr weight_decay) p - lr factor orthogonalize(u),  factor: see muon_lr_factor.
     g is grad_scale times the gradient.  Parameters and momentum buffers must be contiguous, and none may overlap another
-    tensor of the call."""
+    tensor of the call.  A captured call keeps lr and the other numbers, and whoever replays it calls weights_changed()."""
     params, grads, bufs = list(params), list(grads), list(momentum_buffers)
     if not (len(params) == len(grads) == len(bufs)):
         raise ValueError("muon_update: %d parameters, %d gradients, %d momentum buffers" % (len(params), len(grads), len(bufs)))

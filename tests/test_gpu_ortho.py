@@ -373,3 +373,29 @@ def test_orthogonalize_sizes_by_tile(sizes):
     for got, g in zip(ops.orthogonalize(mats), mats):
         check(got, g)
     assert all(torch.equal(p, q) for p, q in zip(ops.orthogonalize(mats), ops.orthogonalize(mats)))
+
+
+@gpu
+def test_muon_update_in_a_graph():
+    """A captured update, replayed between eager ones of other parameters, follows the eager sequence bit for bit."""
+    shapes = [(64, 14, 3, 3), (10, 12), (200, 300), (33, 5)]
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    new = lambda s: [torch.randn(t, generator=gen, device=DEV) for t in s]  # noqa: E731
+    params, grads, bufs = new(shapes), new(shapes), [torch.zeros(s, device=DEV) for s in shapes]
+    eager = [[t.clone() for t in ts] for ts in (params, grads, bufs)]
+    other = [new(shapes[:2]), new(shapes[:2]), new(shapes[:2])]
+    ops.muon_update(*other, lr=0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ops.muon_update(params, grads, bufs, lr=0.05)
+    for it in range(4):
+        for g, e in zip(grads, eager[1]):
+            g.copy_(torch.randn(g.shape, generator=gen, device=DEV))
+            e.copy_(g)
+        graph.replay()
+        ops.muon_update(*other, lr=0.1)
+        ops.muon_update(*eager, lr=0.05)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(params + bufs, eager[0] + eager[2])), it
