@@ -901,6 +901,24 @@ __device__ __forceinline__ void keep(V* lds, const V& arg) {
   for (int i = threadIdx.x; i < (int)(sizeof(V) / 4); i += blockDim.x) reinterpret_cast<int*>(lds)[i] = reinterpret_cast<const int*>(&arg)[i];
 }
 
+// A program from the kernel's arguments, an operation to a lane: read once, and the next one is a few lane reads away.
+struct Ops {
+  int w[sizeof(Op) / 4];
+  __device__ __forceinline__ explicit Ops(const Program& p) {
+    const int lane = threadIdx.x & 63;
+    const int* from = reinterpret_cast<const int*>(&p.op[lane < MAX_OPS ? lane : 0]);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Op) / 4); ++i) w[i] = from[i];
+  }
+  __device__ __forceinline__ Op operator[](int k) const {
+    union { Op op; int v[sizeof(Op) / 4]; } u;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Op) / 4); ++i) u.v[i] = __builtin_amdgcn_readlane(w[i], k);
+    return u.op;
+  }
+};
+static_assert(MAX_OPS <= 64 && sizeof(Op) % 4 == 0, "an operation to a lane");
+
 // the sum of a matrix's partial tiles of A, in the order of the splits, in WM x WN waves' accumulators
 template <int T, int WN, int M, int N>
 __device__ __forceinline__ void add_parts(f32x4 (&acc)[M][N], const Mat& t, unsigned char* ws) {
@@ -920,10 +938,8 @@ __device__ __forceinline__ void add_parts(f32x4 (&acc)[M][N], const Mat& t, unsi
 __global__ __launch_bounds__(Alone::THREADS) void ortho_chain128_kernel(Work a, float f,
                                                                         Program prog) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  __shared__ Program kept;
-  keep(&kept, prog);
+  const Ops ops(prog);
   const Mat t = a.count > 1 ? uniform(&reinterpret_cast<const Mats*>(a.ws)->mat[blockIdx.x]) : a.only;
-  __syncthreads();
   if (t.ks > 1) {
     f32x4 acc[Alone::MR][Alone::NR];
     add_parts<128, Alone::WN>(acc, t, a.ws);
@@ -931,7 +947,7 @@ __global__ __launch_bounds__(Alone::THREADS) void ortho_chain128_kernel(Work a, 
     phase_done();
   }
   for (int k = 0; k < prog.n; ++k) {
-    square_tile<Alone>(t, a.ws, 0, uniform(&kept.op[k]), smem);
+    square_tile<Alone>(t, a.ws, 0, ops[k], smem);
     phase_done();
   }
 }
@@ -958,9 +974,21 @@ struct Lane64 {
   }
 };
 
+// a lane's four numbers of each accumulator in a matrix C
+struct Old64 { f16x4 hi[2][2], lo[2][2]; };
+__device__ __forceinline__ void load_old(Old64& c, const unsigned char* C, const Lane64& L) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      c.hi[i][j] = *reinterpret_cast<const f16x4*>(C + L.at[i][0] + j * 2048);
+      c.lo[i][j] = *reinterpret_cast<const f16x4*>(C + L.at[i][1] + j * 2048);
+    }
+}
+
 // D = ca I + cb C + cc acc into slot D.  What lies outside m x m is zero in C and in acc, and stays zero.
-__device__ __forceinline__ void put64(const f32x4 (&acc)[2][2], float ca, float cb, float cc, int m, unsigned char* D,
-                                      const unsigned char* C, const Lane64& L) {
+__device__ __forceinline__ void put64(const f32x4 (&acc)[2][2], float ca, float cb, float cc, int m, unsigned char* D, const Old64& C,
+                                      const Lane64& L) {
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -968,18 +996,16 @@ __device__ __forceinline__ void put64(const f32x4 (&acc)[2][2], float ca, float 
       float v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = cc * acc[i][j][e];
-      f16x4 hi, lo;
       if (cb != 0.f) {
-        hi = *reinterpret_cast<const f16x4*>(C + L.at[i][0] + j * 2048);
-        lo = *reinterpret_cast<const f16x4*>(C + L.at[i][1] + j * 2048);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = fmaf((float)lo[e], cb, fmaf((float)hi[e], cb, v[e]));
+        for (int e = 0; e < 4; ++e) v[e] = fmaf((float)C.lo[i][j][e], cb, fmaf((float)C.hi[i][j][e], cb, v[e]));
       }
       const int c = L.wm * 32 + i * 16 + 4 * L.g, r = L.wn * 32 + j * 16 + L.r;
       if (ca != 0.f && L.wm == L.wn && i == j) {         // a block on the diagonal
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += r == c + e && r < m ? ca : 0.f;
       }
+      f16x4 hi, lo;
       split4(v, hi, lo);
       *reinterpret_cast<f16x4*>(D + L.at[i][0] + j * 2048) = hi;
       *reinterpret_cast<f16x4*>(D + L.at[i][1] + j * 2048) = lo;
@@ -990,40 +1016,54 @@ __device__ __forceinline__ void lds_done() {
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
 }
-// acc += P Q^T over nb 32-column blocks of two matrices of 64 rows in LDS
+// acc += P Q^T over nb 32-column blocks of two matrices of 64 rows in LDS; a block is read while the one before is multiplied
+struct Block64 { f16x8 p[2][2], q[2][2]; };
 __device__ __forceinline__ void product64(f32x4 (&acc)[2][2], const unsigned char* P, const unsigned char* Q, int nb, const Lane64& L) {
   P += L.wm * 4096;
   Q += L.wn * 4096;
-  for (int b = 0; b < nb; ++b) {
-    f16x8 p[2][2], q[2][2];
+  auto load = [&](Block64& f, int b) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        p[h][i] = *reinterpret_cast<const f16x8*>(P + b * 8192 + i * 2048 + L.fro[h]);
-        q[h][i] = *reinterpret_cast<const f16x8*>(Q + b * 8192 + i * 2048 + L.fro[h]);
+        f.p[h][i] = *reinterpret_cast<const f16x8*>(P + b * 8192 + i * 2048 + L.fro[h]);
+        f.q[h][i] = *reinterpret_cast<const f16x8*>(Q + b * 8192 + i * 2048 + L.fro[h]);
       }
+  };
+  auto multiply = [&](const Block64& f) {
 #pragma unroll
     for (int w = 0; w < 3; ++w)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[w == 2][i], q[w == 1][j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < 2; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[w == 2][i], f.q[w == 1][j], acc[i][j], 0, 0, 0);
+  };
+  Block64 f, g;
+  load(f, 0);
+  int b = 0;
+  for (; b + 1 < nb; b += 2) {
+    load(g, b + 1);
+    multiply(f);
+    if (b + 2 < nb) load(f, b + 2);
+    multiply(g);
   }
+  if (b < nb) multiply(f);
 }
 __device__ __forceinline__ void square64(const Op& op, int m, unsigned char* slots, const Lane64& L) {
   f32x4 acc[2][2];
+  Old64 old{};
+  if (op.cb != 0.f) load_old(old, slots + op.sc * SLOT64, L);
   clear(acc);
   product64(acc, slots + op.sp * SLOT64, slots + op.sq * SLOT64, up32(m) >> 5, L);
-  put64(acc, op.ca, op.cb, op.cc, m, slots + op.sd * SLOT64, slots + op.sc * SLOT64, L);
+  put64(acc, op.ca, op.cb, op.cc, m, slots + op.sd * SLOT64, old, L);
   lds_done();
 }
 
 // The m x m operations of a group for matrices of up to 64 rows; the last slot written is Q, which goes to global memory.
 __global__ __launch_bounds__(256) void ortho_chain64_kernel(Work a, float f, Program prog) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  __shared__ Program kept;
-  keep(&kept, prog);
+  const Ops ops(prog);
   const Mat t = a.count > 1 ? uniform(&reinterpret_cast<const Mats*>(a.ws)->mat[blockIdx.x]) : a.only;
   const Lane64 L;
   const int m = t.m, nb = up32(m) >> 5;
@@ -1038,7 +1078,7 @@ __global__ __launch_bounds__(256) void ortho_chain64_kernel(Work a, float f, Pro
 #pragma unroll
         for (int e = 0; e < 4; ++e)      // rows past the last repeat it in the partial tiles
           if (L.wm * 32 + i * 16 + 4 * L.g + e >= m || L.wn * 32 + j * 16 + L.r >= m) acc[i][j][e] = 0.f;
-    put64(acc, 0.f, 0.f, f, m, smem, smem, L);
+    put64(acc, 0.f, 0.f, f, m, smem, Old64{}, L);
   } else {
     for (int id = threadIdx.x; id < 64 * nb * 8; id += 256) {
       const int r = id / (nb * 8), b = (id >> 3) % nb, c = id & 7;
@@ -1049,7 +1089,7 @@ __global__ __launch_bounds__(256) void ortho_chain64_kernel(Work a, float f, Pro
   __syncthreads();
   int last = 0;
   for (int k = 0; k < prog.n; ++k) {
-    const Op op = uniform(&kept.op[k]);
+    const Op op = ops[k];
     square64(op, m, smem, L);
     last = op.sd;
   }
@@ -1141,9 +1181,8 @@ template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ortho_small_kernel(Mats a, MuonArgs u, float eps, float scale, Program prog) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ double red[16];
-  __shared__ Program kept;
   __shared__ Mat mine;
-  keep(&kept, prog);
+  const Ops ops(prog);
   keep(&mine, a.mat[blockIdx.x]);
   __syncthreads();
   const Mat t = uniform(&mine);
@@ -1221,14 +1260,13 @@ __global__ __launch_bounds__(256) void ortho_small_kernel(Mats a, MuonArgs u, fl
     }
   }
   __syncthreads();
-  const int ops = uniform(&kept.n);
-  for (int k = 0; k < ops; ++k) {
-    const Op op = uniform(&kept.op[k]);
+  for (int k = 0; k < prog.n; ++k) {
+    const Op op = ops[k];
     if (op.kind == K_GRAM) {
       f32x4 acc[2][2];
       clear(acc);
       product64(acc, X, X, KB, L);
-      put64(acc, 0.f, 0.f, op.cc, m, smem, smem, L);
+      put64(acc, 0.f, 0.f, op.cc, m, smem, Old64{}, L);
       lds_done();
     } else if (op.kind == K_SQUARE) {
       square64(op, m, smem, L);
