@@ -17,7 +17,7 @@
 //
 // All matrices of a list share each launch: a workgroup finds its matrix and tile from its index.
 //
-// Measured, float32, five steps: 64 x 126 28 us (one launch), 1024 x 9216 355 us (norm 8, start 16, X X^T 31.5 and its join
+// Measured, float32, five steps: 64 x 126 21 us (one launch), 1024 x 9216 355 us (norm 8, start 16, X X^T 31.5 and its join
 // 8 twice, 13 launches of m x m products at 10.8, Q X 53 and 59), the 21 million numbers of 17 filters with their Muon
 // update 700 us (45, 52, 60 and 9.5 twice, 13 x 19, 105 and 125).
 #include "common.h"
@@ -954,114 +954,98 @@ __global__ __launch_bounds__(Alone::THREADS) void ortho_chain128_kernel(Work a, 
 
 // Up to 64 rows the m x m matrices stay in LDS, 16 KB each: slot k, 32-column block b, row r, 16-byte chunks as in the
 // stages of product().  A workgroup computes the whole 64 x 64 product, and a lane's four rows of one column are, by
-// symmetry, four columns of one row: they go back without any transposition.  An operation takes 1.3 us this way,
-// 2.7 us through global memory.
+// symmetry, four columns of one row: they go back without any transposition.  An operation takes 0.9 us this way (1.2 with
+// four waves), 2.7 us through global memory.
 constexpr int SLOT64 = 64 * 2 * 128;
 
+constexpr int THREADS64 = 1024;      // 16 waves, a 16 x 16 block each: what counts is how soon each is done
+
 struct Lane64 {
-  int wm, wn, r, g, fro[2];
-  int at[2][2];      // byte of this lane's four numbers of accumulator (i, j = 0), [i][half], within a slot; j adds 2048
+  int wm, wn, r, g, fro[2];      // the wave's block of columns and of rows
+  int at[2];                     // byte of this lane's four numbers, [half], within a slot
+  int col, row;                  // of the first of them
   __device__ __forceinline__ Lane64() {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), turn = (lane >> 1) & 7;
-    wm = wave >> 1; wn = wave & 1; r = lane & 15; g = lane >> 4;
+    wm = wave >> 2; wn = wave & 3; r = lane & 15; g = lane >> 4;
+    col = wm * 16 + 4 * g; row = wn * 16 + r;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       fro[h] = r * 128 + (((h * 4 + g) ^ turn) * 16);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        at[i][h] = wm * 8192 + wn * 4096 + r * 128 + (((i * 2 + (g >> 1)) + 4 * h) ^ turn) * 16 + (g & 1) * 8;
+      at[h] = (wm >> 1) * 8192 + wn * 2048 + r * 128 + ((((wm & 1) * 2 + (g >> 1)) + 4 * h) ^ turn) * 16 + (g & 1) * 8;
     }
   }
 };
 
-// a lane's four numbers of each accumulator in a matrix C
-struct Old64 { f16x4 hi[2][2], lo[2][2]; };
-__device__ __forceinline__ void load_old(Old64& c, const unsigned char* C, const Lane64& L) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      c.hi[i][j] = *reinterpret_cast<const f16x4*>(C + L.at[i][0] + j * 2048);
-      c.lo[i][j] = *reinterpret_cast<const f16x4*>(C + L.at[i][1] + j * 2048);
-    }
-}
+// a lane's four numbers in a matrix C
+struct Old64 { f16x4 hi, lo; };
 
 // D = ca I + cb C + cc acc into slot D.  What lies outside m x m is zero in C and in acc, and stays zero.
-__device__ __forceinline__ void put64(const f32x4 (&acc)[2][2], float ca, float cb, float cc, int m, unsigned char* D, const Old64& C,
+__device__ __forceinline__ void put64(const f32x4& acc, float ca, float cb, float cc, int m, unsigned char* D, const Old64& C,
                                       const Lane64& L) {
+  float v[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int e = 0; e < 4; ++e) v[e] = cc * acc[e];
+  if (cb != 0.f) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float v[4];
+    for (int e = 0; e < 4; ++e) v[e] = fmaf((float)C.lo[e], cb, fmaf((float)C.hi[e], cb, v[e]));
+  }
+  if (ca != 0.f && L.wm == L.wn) {         // a block on the diagonal
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = cc * acc[i][j][e];
-      if (cb != 0.f) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = fmaf((float)C.lo[i][j][e], cb, fmaf((float)C.hi[i][j][e], cb, v[e]));
-      }
-      const int c = L.wm * 32 + i * 16 + 4 * L.g, r = L.wn * 32 + j * 16 + L.r;
-      if (ca != 0.f && L.wm == L.wn && i == j) {         // a block on the diagonal
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += r == c + e && r < m ? ca : 0.f;
-      }
-      f16x4 hi, lo;
-      split4(v, hi, lo);
-      *reinterpret_cast<f16x4*>(D + L.at[i][0] + j * 2048) = hi;
-      *reinterpret_cast<f16x4*>(D + L.at[i][1] + j * 2048) = lo;
-    }
+    for (int e = 0; e < 4; ++e) v[e] += L.row == L.col + e && L.row < m ? ca : 0.f;
+  }
+  f16x4 hi, lo;
+  split4(v, hi, lo);
+  *reinterpret_cast<f16x4*>(D + L.at[0]) = hi;
+  *reinterpret_cast<f16x4*>(D + L.at[1]) = lo;
 }
 __device__ __forceinline__ void lds_done() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
 }
-// acc += P Q^T over nb 32-column blocks of two matrices of 64 rows in LDS; a block is read while the one before is multiplied
-struct Block64 { f16x8 p[2][2], q[2][2]; };
-__device__ __forceinline__ void product64(f32x4 (&acc)[2][2], const unsigned char* P, const unsigned char* Q, int nb, const Lane64& L) {
-  P += L.wm * 4096;
-  Q += L.wn * 4096;
+// 32 columns of both operands, [half]
+struct Block64 { f16x8 p[2], q[2]; };
+__device__ __forceinline__ void multiply64(f32x4& acc, const Block64& f) {
+#pragma unroll
+  for (int w = 0; w < 3; ++w) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[w == 2], f.q[w == 1], acc, 0, 0, 0);
+}
+// P Q^T over nb 32-column blocks of two matrices of 64 rows in LDS; a block is read while the one before is multiplied
+__device__ __forceinline__ f32x4 product64(const unsigned char* P, const unsigned char* Q, int nb, const Lane64& L) {
+  P += L.wm * 2048;
+  Q += L.wn * 2048;
   auto load = [&](Block64& f, int b) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        f.p[h][i] = *reinterpret_cast<const f16x8*>(P + b * 8192 + i * 2048 + L.fro[h]);
-        f.q[h][i] = *reinterpret_cast<const f16x8*>(Q + b * 8192 + i * 2048 + L.fro[h]);
-      }
+    for (int h = 0; h < 2; ++h) {
+      f.p[h] = *reinterpret_cast<const f16x8*>(P + b * 8192 + L.fro[h]);
+      f.q[h] = *reinterpret_cast<const f16x8*>(Q + b * 8192 + L.fro[h]);
+    }
   };
-  auto multiply = [&](const Block64& f) {
-#pragma unroll
-    for (int w = 0; w < 3; ++w)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[w == 2][i], f.q[w == 1][j], acc[i][j], 0, 0, 0);
-  };
-  Block64 f, g;
-  load(f, 0);
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  Block64 one, two;
+  load(one, 0);
   int b = 0;
   for (; b + 1 < nb; b += 2) {
-    load(g, b + 1);
-    multiply(f);
-    if (b + 2 < nb) load(f, b + 2);
-    multiply(g);
+    load(two, b + 1);
+    multiply64(acc, one);
+    if (b + 2 < nb) load(one, b + 2);
+    multiply64(acc, two);
   }
-  if (b < nb) multiply(f);
+  if (b < nb) multiply64(acc, one);
+  return acc;
 }
 __device__ __forceinline__ void square64(const Op& op, int m, unsigned char* slots, const Lane64& L) {
-  f32x4 acc[2][2];
   Old64 old{};
-  if (op.cb != 0.f) load_old(old, slots + op.sc * SLOT64, L);
-  clear(acc);
-  product64(acc, slots + op.sp * SLOT64, slots + op.sq * SLOT64, up32(m) >> 5, L);
+  if (op.cb != 0.f) {
+    old.hi = *reinterpret_cast<const f16x4*>(slots + op.sc * SLOT64 + L.at[0]);
+    old.lo = *reinterpret_cast<const f16x4*>(slots + op.sc * SLOT64 + L.at[1]);
+  }
+  const f32x4 acc = product64(slots + op.sp * SLOT64, slots + op.sq * SLOT64, up32(m) >> 5, L);
   put64(acc, op.ca, op.cb, op.cc, m, slots + op.sd * SLOT64, old, L);
   lds_done();
 }
 
 // The m x m operations of a group for matrices of up to 64 rows; the last slot written is Q, which goes to global memory.
-__global__ __launch_bounds__(256) void ortho_chain64_kernel(Work a, float f, Program prog) {
+__global__ __launch_bounds__(THREADS64) void ortho_chain64_kernel(Work a, float f, Program prog) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const Ops ops(prog);
   const Mat t = a.count > 1 ? uniform(&reinterpret_cast<const Mats*>(a.ws)->mat[blockIdx.x]) : a.only;
@@ -1069,18 +1053,13 @@ __global__ __launch_bounds__(256) void ortho_chain64_kernel(Work a, float f, Pro
   const int m = t.m, nb = up32(m) >> 5;
   unsigned char* A = slot_of(t, a.ws, 0);
   if (t.ks > 1) {
-    f32x4 acc[2][2];
-    add_parts<64, 2>(acc, t, a.ws);
+    f32x4 sum[1][1], acc;
+    add_parts<64, 4>(sum, t, a.ws);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)      // rows past the last repeat it in the partial tiles
-          if (L.wm * 32 + i * 16 + 4 * L.g + e >= m || L.wn * 32 + j * 16 + L.r >= m) acc[i][j][e] = 0.f;
+    for (int e = 0; e < 4; ++e) acc[e] = L.col + e < m && L.row < m ? sum[0][0][e] : 0.f;      // rows past the last repeat it
     put64(acc, 0.f, 0.f, f, m, smem, Old64{}, L);
   } else {
-    for (int id = threadIdx.x; id < 64 * nb * 8; id += 256) {
+    for (int id = threadIdx.x; id < 64 * nb * 8; id += THREADS64) {
       const int r = id / (nb * 8), b = (id >> 3) % nb, c = id & 7;
       const uint4 v = r < m ? *reinterpret_cast<const uint4*>(A + ((int64_t)r * nb + b) * 128 + c * 16) : make_uint4(0, 0, 0, 0);
       *reinterpret_cast<uint4*>(smem + b * 8192 + r * 128 + (c ^ ((r >> 1) & 7)) * 16) = v;
@@ -1094,7 +1073,7 @@ __global__ __launch_bounds__(256) void ortho_chain64_kernel(Work a, float f, Pro
     last = op.sd;
   }
   unsigned char* Q = slot_of(t, a.ws, last);
-  for (int id = threadIdx.x; id < m * nb * 8; id += 256) {
+  for (int id = threadIdx.x; id < m * nb * 8; id += THREADS64) {
     const int r = id / (nb * 8), b = (id >> 3) % nb, c = id & 7;
     *reinterpret_cast<uint4*>(Q + ((int64_t)r * nb + b) * 128 + c * 16) =
         *reinterpret_cast<const uint4*>(smem + last * SLOT64 + b * 8192 + r * 128 + (c ^ ((r >> 1) & 7)) * 16);
@@ -1115,70 +1094,54 @@ __device__ __forceinline__ void apply64(const Mat& t, unsigned char* X, const un
   X += c * SLOT64;
   // transposing reads: k-row 8 g + t (+ 4), columns 4 q ..; the chunk a row holds them in: base ^ 4 half ^ 2 (side ^ upper four)
   const int tt = lane >> 2 & 3, cq = lane & 3, base = (cq >> 1) ^ (4 * (L.g & 1) + (tt >> 1));
-  const unsigned char* row = X + (2 * c + L.wm < KB ? L.wm : 0) * 8192 + (8 * L.g + tt) * 128 + (cq & 1) * 8;
-  f32x4 acc[2][2];
-  clear(acc);
-  for (int b = 0; b < nb; ++b) {
-    f16x8 x[2][2], q[2][2];
+  const bool past = 2 * c + (L.wm >> 1) >= KB;
+  const unsigned char* row = X + (past ? 0 : L.wm >> 1) * 8192 + (8 * L.g + tt) * 128 + (cq & 1) * 8;
+  auto load = [&](Block64& in, int b) {
+    const unsigned char* at = row + b * 4096;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
+      typedef __attribute__((ext_vector_type(8))) short short8v;
+      const int side = 2 * (L.wm & 1);
+      const short4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) short4v*)(at + (base ^ (4 * h) ^ side) * 16));
+      const short4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) short4v*)(at + 512 + (base ^ (4 * h) ^ (side ^ 2)) * 16));
+      in.p[h] = __builtin_bit_cast(f16x8, short8v{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]});
+      in.q[h] = *reinterpret_cast<const f16x8*>(Q + b * 8192 + L.wn * 2048 + L.fro[h]);
+    }
+  };
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  Block64 one, two;
+  load(one, 0);
+  if (nb > 1) load(two, 1);
+  multiply64(acc, one);
+  if (nb > 1) multiply64(acc, two);
+  float v[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        typedef __attribute__((ext_vector_type(8))) short short8v;
-        const unsigned char* at = row + b * 4096;
-        const short4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) short4v*)(at + (base ^ (4 * h) ^ (2 * i)) * 16));
-        const short4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) short4v*)(at + 512 + (base ^ (4 * h) ^ (2 * (i ^ 1))) * 16));
-        x[h][i] = __builtin_bit_cast(f16x8, short8v{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]});
-        q[h][i] = *reinterpret_cast<const f16x8*>(Q + b * 8192 + L.wn * 4096 + i * 2048 + L.fro[h]);
-      }
-#pragma unroll
-    for (int w = 0; w < 3; ++w)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[w == 2][i], q[w == 1][j], acc[i][j], 0, 0, 0);
-  }
-  if (2 * c + L.wm >= KB) return lds_done();                  // this wave's block lies past the end
+  for (int e = 0; e < 4; ++e) v[e] = acc[e] * f;
+  lds_done();                                                 // every wave has read the old columns
+  if (past) return;
   if (!last) {
-    lds_done();                                               // every wave has read the old columns
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float v[4];
-        f16x4 hi, lo;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f;
-        split4(v, hi, lo);
-        *reinterpret_cast<f16x4*>(X + L.at[i][0] + j * 2048) = hi;
-        *reinterpret_cast<f16x4*>(X + L.at[i][1] + j * 2048) = lo;
-      }
+    f16x4 hi, lo;
+    split4(v, hi, lo);
+    *reinterpret_cast<f16x4*>(X + L.at[0]) = hi;
+    *reinterpret_cast<f16x4*>(X + L.at[1]) = lo;
     return;
   }
+  const int col = c * 64 + L.col;
+  if (L.row >= m) return;
+  T* o = static_cast<T*>(t.out) + (t.flip ? (int64_t)col * t.ldo + L.row : (int64_t)L.row * t.ldo + col);
+  const int64_t next = t.flip ? t.ldo : 1;
+  float old[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int e = 0; e < 4; ++e) old[e] = MUON && col + e < n ? (float)o[e * next] : 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int col = c * 64 + L.wm * 32 + i * 16 + 4 * L.g, r = L.wn * 32 + j * 16 + L.r;
-      if (r >= m) continue;
-      T* o = static_cast<T*>(t.out) + (t.flip ? (int64_t)col * t.ldo + r : (int64_t)r * t.ldo + col);
-      const int64_t next = t.flip ? t.ldo : 1;
-      float old[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) old[e] = MUON && col + e < n ? (float)o[e * next] : 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = acc[i][j][e] * f;
-        if (col + e < n) o[e * next] = MUON ? (T)(old[e] * u.decay - t.step * v) : (T)v;
-      }
-    }
-  lds_done();
+  for (int e = 0; e < 4; ++e)
+    if (col + e < n) o[e * next] = MUON ? (T)(old[e] * u.decay - t.step * v[e]) : (T)v[e];
 }
 
 template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void ortho_small_kernel(Mats a, MuonArgs u, float eps, float scale, Program prog) {
+__global__ __launch_bounds__(THREADS64) void ortho_small_kernel(Mats a, MuonArgs u, float eps, float scale, Program prog) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ double red[16];
   __shared__ Mat mine;
@@ -1190,13 +1153,13 @@ __global__ __launch_bounds__(256) void ortho_small_kernel(Mats a, MuonArgs u, fl
   const Lane64 L;
   const int m = t.m, n = t.n, KB = up32(n) >> 5;
   // the matrix, eight elements at a time, stays in registers until its norm is known
-  constexpr int MOST = 64 * SMALL_N / 8 / 256;
+  constexpr int MOST = (64 * SMALL_N / 8 + THREADS64 - 1) / THREADS64;
   const int rows = t.flip ? n : m, cols = t.flip ? m : n, c8 = (cols + 7) >> 3, chunks = rows * c8;
   const T* x = static_cast<const T*>(t.x);
   float v[MOST][8];
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
-    const int id = k * 256 + threadIdx.x, r = id / c8, c = (id - r * c8) * 8;
+    const int id = k * THREADS64 + threadIdx.x, r = id / c8, c = (id - r * c8) * 8;
     float mo[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[k][e] = mo[e] = 0.f;
@@ -1231,11 +1194,11 @@ __global__ __launch_bounds__(256) void ortho_small_kernel(Mats a, MuonArgs u, fl
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += (double)v[k][e] * (double)v[k][e];
   const double f = start_factor(block_sum(s, red), eps, scale);
-  for (int i = threadIdx.x; i < KB * 512; i += 256) reinterpret_cast<uint4*>(X)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < KB * 512; i += THREADS64) reinterpret_cast<uint4*>(X)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
-    const int id = k * 256 + threadIdx.x, r = id / c8, c = (id - r * c8) * 8;
+    const int id = k * THREADS64 + threadIdx.x, r = id / c8, c = (id - r * c8) * 8;
     if (id >= chunks) continue;
     float w[8];
 #pragma unroll
@@ -1263,10 +1226,7 @@ __global__ __launch_bounds__(256) void ortho_small_kernel(Mats a, MuonArgs u, fl
   for (int k = 0; k < prog.n; ++k) {
     const Op op = ops[k];
     if (op.kind == K_GRAM) {
-      f32x4 acc[2][2];
-      clear(acc);
-      product64(acc, X, X, KB, L);
-      put64(acc, 0.f, 0.f, op.cc, m, smem, Old64{}, L);
+      put64(product64(X, X, KB, L), 0.f, 0.f, op.cc, m, smem, Old64{}, L);
       lds_done();
     } else if (op.kind == K_SQUARE) {
       square64(op, m, smem, L);
@@ -1504,7 +1464,7 @@ struct Run {
       ortho_chain128_kernel<<<(unsigned)a.count, Alone::THREADS, Alone::LDS, st>>>(work(), f, prog);
     } else {
       ORTHO_TRY((ready<&ortho_chain64_kernel>(SLOTS * SLOT64, what)));
-      ortho_chain64_kernel<<<(unsigned)a.count, 256, SLOTS * SLOT64, st>>>(work(), f, prog);
+      ortho_chain64_kernel<<<(unsigned)a.count, THREADS64, SLOTS * SLOT64, st>>>(work(), f, prog);
     }
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
@@ -1527,7 +1487,7 @@ struct Run {
   template <typename T, bool MUON>
   int small(const Program& prog, float eps, float scale) const {
     ORTHO_TRY((ready<&ortho_small_kernel<T, MUON>>(SMALL_LDS, what)));
-    ortho_small_kernel<T, MUON><<<(unsigned)a.count, 256, SMALL_LDS, st>>>(a, u, eps, scale, prog);
+    ortho_small_kernel<T, MUON><<<(unsigned)a.count, THREADS64, SMALL_LDS, st>>>(a, u, eps, scale, prog);
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
   }
