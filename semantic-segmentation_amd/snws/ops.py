@@ -2406,7 +2406,7 @@ def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
         if g.dim() < 2:
             raise ValueError("orthogonalize: matrices expected, got shape %s" % (tuple(g.shape),))
         require_gpu(g, "orthogonalize")
-        flat = g.detach().reshape((-1,) + g.shape[-2:])
+        flat = g.detach().flatten(0, -3)
         out = torch.empty(flat.shape, dtype=g.dtype, device=g.device)
         _orthogonalize(list(flat.unbind(0)), steps, coefficients, eps, list(out.unbind(0)))
         return out.view(g.shape)

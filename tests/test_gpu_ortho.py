@@ -399,3 +399,13 @@ def test_muon_update_in_a_graph():
         ops.muon_update(*eager, lr=0.05)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(params + bufs, eager[0] + eager[2])), it
+
+
+@gpu
+def test_orthogonalize_empty_batches():
+    for shape in ((0, 4, 5), (3, 0, 5), (2, 3, 4, 0), (0, 2, 3, 4), (0, 7), (7, 0)):
+        out = ops.orthogonalize(torch.zeros(shape, device=DEV))
+        assert out.shape == shape and out.numel() == 0
+    a, b = ops.orthogonalize([torch.zeros(0, 3, device=DEV), matrix(5, 9)])
+    assert a.shape == (0, 3)
+    check(b, matrix(5, 9))
