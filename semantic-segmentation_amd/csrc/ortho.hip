@@ -402,8 +402,6 @@ typedef Tile<128, 160, 2, 2, 2> Wide;
 typedef Tile<64, 64, 2, 4, 4> Fine;
 // 96 x 64, four waves of 48 x 32, for m x m products where that makes fewer rounds
 typedef Tile<96, 64, 2, 2, 4> Tall;
-// 128 x 128 by one workgroup alone
-typedef Tile<128, 128, 2, 4, 2> Alone;
 
 typedef __attribute__((ext_vector_type(4))) short short4v;
 
@@ -880,12 +878,6 @@ __global__ __launch_bounds__(G::THREADS, G::PER_CU * G::W / 4) void ortho_apply_
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// What one workgroup wrote to the workspace is there for all its waves: its stores have left, and its CU has one L1.
-__device__ __forceinline__ void phase_done() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  __syncthreads();
-}
-
 // a value in memory, the same for all lanes, in scalar registers
 template <typename V>
 __device__ __forceinline__ V uniform(const V* p) {
@@ -918,39 +910,6 @@ struct Ops {
   }
 };
 static_assert(MAX_OPS <= 64 && sizeof(Op) % 4 == 0, "an operation to a lane");
-
-// the sum of a matrix's partial tiles of A, in the order of the splits, in WM x WN waves' accumulators
-template <int T, int WN, int M, int N>
-__device__ __forceinline__ void add_parts(f32x4 (&acc)[M][N], const Mat& t, unsigned char* ws) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const f32x4* part = part_of(t, ws) + lane;
-  clear(acc);
-  for (int k = 0; k < t.ks; ++k)
-#pragma unroll
-    for (int r = 0; r < M; ++r)
-#pragma unroll
-      for (int c = 0; c < N; ++c)
-        acc[r][c] += part[(int64_t)k * (T * T / 4) + (((wave / WN) * M + r) * (T / 16) + (wave % WN) * N + c) * 64];
-}
-
-// The m x m operations of a group for matrices of 65 to 128 rows, a workgroup each, instead of a launch for every operation;
-// the partial tiles of A are added up on the way.
-__global__ __launch_bounds__(Alone::THREADS) void ortho_chain128_kernel(Work a, float f,
-                                                                        Program prog) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const Ops ops(prog);
-  const Mat t = a.count > 1 ? uniform(&reinterpret_cast<const Mats*>(a.ws)->mat[blockIdx.x]) : a.only;
-  if (t.ks > 1) {
-    f32x4 acc[Alone::MR][Alone::NR];
-    add_parts<128, Alone::WN>(acc, t, a.ws);
-    put_symmetric<Alone>(acc, f, t, slot_of(t, a.ws, 0), 0, 0, smem);
-    phase_done();
-  }
-  for (int k = 0; k < prog.n; ++k) {
-    square_tile<Alone>(t, a.ws, 0, ops[k], smem);
-    phase_done();
-  }
-}
 
 // Up to 64 rows the m x m matrices stay in LDS, 16 KB each: slot k, 32-column block b, row r, 16-byte chunks as in the
 // stages of product().  A workgroup computes the whole 64 x 64 product, and a lane's four rows of one column are, by
@@ -1053,10 +1012,13 @@ __global__ __launch_bounds__(THREADS64) void ortho_chain64_kernel(Work a, float 
   const int m = t.m, nb = up32(m) >> 5;
   unsigned char* A = slot_of(t, a.ws, 0);
   if (t.ks > 1) {
-    f32x4 sum[1][1], acc;
-    add_parts<64, 4>(sum, t, a.ws);
+    // the partial tiles of A, in the order of the splits
+    const f32x4* part = part_of(t, a.ws) + threadIdx.x;
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int k = 0; k < t.ks; ++k) acc += part[k * (64 * 64 / 4)];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = L.col + e < m && L.row < m ? sum[0][0][e] : 0.f;      // rows past the last repeat it
+    for (int e = 0; e < 4; ++e) acc[e] = L.col + e < m && L.row < m ? acc[e] : 0.f;      // rows past the last repeat it
     put64(acc, 0.f, 0.f, f, m, smem, Old64{}, L);
   } else {
     for (int id = threadIdx.x; id < 64 * nb * 8; id += THREADS64) {
@@ -1289,8 +1251,8 @@ bool ortho_scales(const float* coeff, int steps, Scales* s) {
   return true;
 }
 
-// How a call is run.  GENERAL: every product a launch over all its tiles.  CHAIN (all m <= 128): one launch for the m x m
-// products of a group.  SMALL: one launch for everything.
+// How a call is run.  GENERAL: every product a launch over all its tiles.  CHAIN: one launch for the m x m products of a
+// group, where they fit LDS (m <= 64).  SMALL: one launch for everything.
 enum Mode { GENERAL, CHAIN, SMALL };
 
 struct Plan {
@@ -1340,14 +1302,14 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
   p.mode = GENERAL;
   if (steps <= 6) {
     if (mmax <= 64 && nmax <= SMALL_N) p.mode = SMALL;
-    else if (mmax <= 128) p.mode = CHAIN;
+    else if (mmax <= 64) p.mode = CHAIN;
   }
   // Few tiles: 64 x 64, to occupy CUs; fewer than 256 of 128 x 128 are few (Q X of 333 x 1000, 24: 13.5 us against 6.6).
   // X X^T splits its contraction, at least eight blocks to a workgroup: 512 x 4608, 180 workgroups of 128 x 128, 12.1 us
   // against 9.8, but 1024 x 9216, 512 of them, 32 against 41.  From 256 on 128 rows, and for Q X the width whose rounds of 512
   // workgroups make the least work: 9216 columns by 1024 rows are 576 tiles of 128 columns, two rounds, but 464 of 160, one.
-  p.wg = mmax > 64 && (p.mode == CHAIN || grams >= 256) ? 128 : 64;
-  p.wp = p.wg;
+  p.wg = mmax > 64 && grams >= 256 ? 128 : 64;
+  p.wp = 64;
   if (p.mode == GENERAL) {
     // Products of m x m matrices take as long as the CU with the most tiles.  In units of a 64 x 64 tile, one of 96 x 64 takes
     // 1.5, one of 128 x 128 3.7, and two of these, that share a CU, 5.9; a tile of a smaller matrix counts by its share of the
@@ -1373,8 +1335,7 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
   const int T = p.wg, AM = p.wa == 64 ? 64 : 128, AN = p.wa;
   int64_t work = 0;
   for (int i = 0; i < a.count; ++i) work += (int64_t)tri(a.mat[i].m, T) * (up32(a.mat[i].n) >> 5);
-  // k-blocks per workgroup so that as many as the chip holds at once share the whole contraction evenly; at least 8.  A
-  // chain adds the partial tiles by itself: at most eight of them.
+  // k-blocks per workgroup so that as many as the chip holds at once share the whole contraction evenly; at least 8.
   const int64_t round = 512;
   int64_t kc = cdiv64(work, round);
   if (kc < 8) kc = 8;
@@ -1392,7 +1353,11 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
     t.norm0 = norms;
     norms += t.normc;
     int64_t k = kc;
-    if (p.mode == CHAIN && k < cdiv64(KB, 8)) k = cdiv64(KB, 8);
+    // A block takes 0.2 us, and about as long a part to be added, where few workgroups do it: their sum is least with
+    // sqrt(KB) of each; tiles of 128 have more workgroups to add them, and longer blocks.  64 x 9216: 62 us with 16 parts, 71
+    // with 8, 66 with 24; 64 x 131072: 171 with 64, 287 with 512; 100 x 131072: 295 with 91, 375 with 512.
+    const int64_t least = (int64_t)ceil(sqrt((double)KB) * (T == 128 ? 0.5 : 1.0));
+    if (k < least) k = least;
     t.kc = (int)(p.mode == SMALL || k > KB ? KB : k);
     t.ks = (int)cdiv64(KB, t.kc);
     t.at = off;
@@ -1459,13 +1424,8 @@ struct Run {
     return SNWS_OK;
   }
   int chain(float f, const Program& prog) const {
-    if (p.wg == 128) {
-      ORTHO_TRY((ready<&ortho_chain128_kernel>(Alone::LDS, what)));
-      ortho_chain128_kernel<<<(unsigned)a.count, Alone::THREADS, Alone::LDS, st>>>(work(), f, prog);
-    } else {
-      ORTHO_TRY((ready<&ortho_chain64_kernel>(SLOTS * SLOT64, what)));
-      ortho_chain64_kernel<<<(unsigned)a.count, THREADS64, SLOTS * SLOT64, st>>>(work(), f, prog);
-    }
+    ORTHO_TRY((ready<&ortho_chain64_kernel>(SLOTS * SLOT64, what)));
+    ortho_chain64_kernel<<<(unsigned)a.count, THREADS64, SLOTS * SLOT64, st>>>(work(), f, prog);
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
   }

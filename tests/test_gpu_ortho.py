@@ -409,3 +409,10 @@ def test_orthogonalize_empty_batches():
     a, b = ops.orthogonalize([torch.zeros(0, 3, device=DEV), matrix(5, 9)])
     assert a.shape == (0, 3)
     check(b, matrix(5, 9))
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(64, 40000), (60000, 50), (3, 200000), (100, 30000), (33, 49153)])
+def test_orthogonalize_long(rows, cols):
+    g = matrix(rows, cols)
+    check(ops.orthogonalize(g), g)
