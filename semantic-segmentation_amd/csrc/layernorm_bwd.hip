@@ -32,6 +32,7 @@ struct BwdArgs {
 
 // One launch up to here: 160 rows of 512 float32 take 4.1 us instead of 5.4 + 2.7 us in two launches.
 constexpr int64_t FEW_ROWS = 256;
+constexpr int64_t SLICE_ROWS = 16;     // rows to a thread of the columns' sums, where rows are longer than registers hold
 
 // parameter gradients of 32 columns, by all threads of a workgroup: float32 over a thread's rows, float64 over the threads
 template <typename T, int BT>
@@ -224,26 +225,54 @@ __global__ __launch_bounds__(256) void ln_bwd_narrow_kernel(BwdArgs a) {
   }
 }
 
+// rows beyond what the kernel above holds: 4 chunks of x and dy of each of 1024 threads stay in registers
 template <typename T>
-__global__ __launch_bounds__(512) void ln_bwd_wide_kernel(BwdArgs a) {
-  __shared__ float red[16];
+__global__ __launch_bounds__(WIDE) void ln_bwd_wide_kernel(BwdArgs a) {
+  constexpr int VEC = Geo<T>::VEC, KEEP = 4;
+  __shared__ float red[2 * (WIDE / 64)];
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
   T* dx = static_cast<T*>(a.dx) + row * a.lddx;
   const float mean = a.mean[row], rstd = a.rstd[row];
+  uint4 vx[KEEP], vg[KEEP];
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) vx[i] = vg[i] = make_uint4(0, 0, 0, 0);
   float s1 = 0.f, s2 = 0.f;
-  for (int c = threadIdx.x; c < a.C; c += 512) {
-    const float g = (float)dy[c] * (a.w ? a.w[c] : 1.f);
-    s1 += g;
-    s2 += g * ((float)x[c] - mean) * rstd;
-  }
-  group_sum2<512>(s1, s2, red);
+  wide_row<VEC, KEEP>(a.C, [&](int kept, int c, int dup) {
+    const uint4 rx = load_raw(x + c), rg = load_raw(dy + c);
+    if (kept >= 0) {
+      vx[kept] = rx;
+      vg[kept] = rg;
+    }
+    float f[VEC], g[VEC], w[VEC];
+    unpack(rx, f);
+    unpack(rg, g);
+    load_param<VEC>(a.w, c, 1.f, w);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float d = e >= dup ? g[e] * w[e] : 0.f;
+      s1 += d;
+      s2 += e >= dup ? d * ((f[e] - mean) * rstd) : 0.f;
+    }
+  });
+  group_sum2<WIDE>(s1, s2, red);
   const float m1 = s1 / (float)a.C, m2 = s2 / (float)a.C;
-  for (int c = threadIdx.x; c < a.C; c += 512) {
-    const float z = ((float)x[c] - mean) * rstd;
-    dx[c] = (T)(rstd * ((float)dy[c] * (a.w ? a.w[c] : 1.f) - m1 - z * m2));
-  }
+  wide_row<VEC, KEEP>(a.C, [&](int kept, int c, int dup) {
+    float f[VEC], g[VEC], w[VEC];
+    unpack(kept >= 0 ? vx[kept] : load_raw(x + c), f);
+    unpack(kept >= 0 ? vg[kept] : load_raw(dy + c), g);
+    load_param<VEC>(a.w, c, 1.f, w);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = rstd * (g[e] * w[e] - m1 - (f[e] - mean) * rstd * m2);
+    if (dup == 0) {
+      store_raw(dx + c, pack(f));
+    } else {
+#pragma unroll
+      for (int e = 1; e < VEC; ++e)
+        if (e >= dup) dx[c + e] = (T)f[e];
+    }
+  });
 }
 
 // parameter gradients of such rows: a thread per column, rows dealt to gridDim.y slices
@@ -258,6 +287,11 @@ __global__ __launch_bounds__(256) void ln_bwd_wide_param_kernel(BwdArgs a) {
     const float g = (float)dy[row * a.lddy + c];
     db += g;
     dw += g * ((float)x[row * a.ldx + c] - a.mean[row]) * a.rstd[row];
+  }
+  if (!a.part) {               // one slice: no partial rows
+    if (a.dw) a.dw[c] = dw;
+    if (a.db) a.db[c] = db;
+    return;
   }
   float* part = a.part + (int64_t)blockIdx.y * 2 * a.C;
   part[c] = dw;
@@ -302,7 +336,7 @@ int64_t bwd_blocks(int64_t rows, int C) {
     const int64_t chunks = cdiv64(C, VEC);
     const int G = pick_group(chunks);
     if (!G) {
-      need = cdiv64(rows, 16);                       // slices of the column sums
+      need = cdiv64(rows, SLICE_ROWS);               // slices of the column sums
       const int64_t cb = cdiv64(C, 256);
       most = cdiv64(1024, cb);
       return need < most ? need : most;
@@ -313,14 +347,14 @@ int64_t bwd_blocks(int64_t rows, int C) {
   return need < most ? need : most;
 }
 
-// few rows, in registers: one launch
+// few rows: no partial rows
 template <typename T>
-bool one_launch(int64_t rows, int C) {
+bool few_rows(int64_t rows, int C) {
   constexpr int VEC = Geo<T>::VEC;
-  return rows <= FEW_ROWS && C >= VEC && pick_group(cdiv64(C, VEC));
+  return C >= VEC && rows <= (pick_group(cdiv64(C, VEC)) ? FEW_ROWS : SLICE_ROWS);
 }
-bool one_launch(int dtype, int64_t rows, int C) {
-  return dtype == SNWS_F32 ? one_launch<float>(rows, C) : one_launch<bf16_t>(rows, C);
+bool few_rows(int dtype, int64_t rows, int C) {
+  return dtype == SNWS_F32 ? few_rows<float>(rows, C) : few_rows<bf16_t>(rows, C);
 }
 
 template <typename T>
@@ -339,11 +373,11 @@ struct Bwd {
   int wide() {
     if (a.rows > 0x7fffffff) SNWS_UNSUPPORTED("snws_ln_bwd: too many rows of this length");
     if (a.dx) {
-      ln_bwd_wide_kernel<T><<<(unsigned)a.rows, 512, 0, st>>>(a);
+      ln_bwd_wide_kernel<T><<<(unsigned)a.rows, WIDE, 0, st>>>(a);
       SNWS_LAUNCH_CHECK("snws_ln_bwd");
     }
-    if (a.part) {
-      ln_bwd_wide_param_kernel<T><<<dim3((unsigned)cdiv64(a.C, 256), (unsigned)blocks), 256, 0, st>>>(a);
+    if (a.dw || a.db) {
+      ln_bwd_wide_param_kernel<T><<<dim3((unsigned)cdiv64(a.C, 256), a.part ? (unsigned)blocks : 1), 256, 0, st>>>(a);
       SNWS_LAUNCH_CHECK("snws_ln_bwd");
     }
     return SNWS_OK;
@@ -362,7 +396,7 @@ struct Bwd {
 }  // namespace
 
 extern "C" int64_t snws_ln_bwd_workspace_floats(int dtype, int64_t rows, int C) {
-  if (rows < 1 || C < 1 || C > LN_MAX_C || one_launch(dtype, rows, C)) return 0;
+  if (rows < 1 || C < 1 || C > LN_MAX_C || few_rows(dtype, rows, C)) return 0;
   return 2 * (int64_t)C * (dtype == SNWS_F32 ? bwd_blocks<float>(rows, C) : bwd_blocks<bf16_t>(rows, C));
 }
 
@@ -380,7 +414,7 @@ extern "C" int snws_ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t 
   int64_t blocks = 0;
   if (rows > 0 && (dx || params)) {
     blocks = dtype == SNWS_F32 ? bwd_blocks<float>(rows, C) : bwd_blocks<bf16_t>(rows, C);
-    const bool few = one_launch(dtype, rows, C);
+    const bool few = few_rows(dtype, rows, C);
     const BwdArgs a{dy, x, mean, rstd, weight, dx, params && !few ? workspace : nullptr, dweight, dbias, lddy, ldx, lddx, rows, C,
                     few && !dx ? 0 : (int)blocks};
     if (few) blocks = a.row_blocks + (params ? cdiv64(C, 32) : 0);

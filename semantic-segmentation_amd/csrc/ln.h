@@ -119,6 +119,23 @@ __device__ __forceinline__ float group_sum(float a, float* red) {
   return a;
 }
 
+// A row by a workgroup of 1024 threads, chunk after chunk: f(kept index or -1, chunk's first column, its dup).  The first KEEP
+// chunks of a thread have a constant index, so that what is kept of them stays in registers.
+constexpr int WIDE = 1024;
+template <int VEC, int KEEP, typename F>
+__device__ __forceinline__ void wide_row(int C, F&& f) {
+  const int chunks = (C + VEC - 1) / VEC;
+  auto one = [&](int kept, int k) {
+    const int c0 = k * VEC, c = c0 + VEC > C ? C - VEC : c0;
+    f(kept, c, c0 - c);
+  };
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i)
+    if ((int)threadIdx.x + i * WIDE < chunks) one(i, threadIdx.x + i * WIDE);
+#pragma unroll 4
+  for (int k = threadIdx.x + KEEP * WIDE; k < chunks; k += WIDE) one(-1, k);
+}
+
 // Lanes per row and chunks per lane for a row of `chunks` chunks.  The narrowest group that needs at most five chunks per
 // lane wastes the fewest lanes on a ragged end (320 bfloat16 channels: 40 chunks = 8 lanes x 5, none idle); from 160
 // chunks on a whole wave, then a workgroup of 4 or 8 waves takes a row, with up to eight.  0: longer than registers hold.

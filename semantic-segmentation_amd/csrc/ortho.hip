@@ -1355,7 +1355,7 @@ void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
     int64_t k = kc;
     // A block takes 0.2 us, and about as long a part to be added, where few workgroups do it: their sum is least with
     // sqrt(KB) of each; tiles of 128 have more workgroups to add them, and longer blocks.  64 x 9216: 62 us with 16 parts, 71
-    // with 8, 66 with 24; 64 x 131072: 171 with 64, 287 with 512; 100 x 131072: 295 with 91, 375 with 512.
+    // with 8, 66 with 24; 64 x 131072: 171 with 64, 287 with 512; 100 x 131072: 282 with 128, 375 with 512.
     const int64_t least = (int64_t)ceil(sqrt((double)KB) * (T == 128 ? 0.5 : 1.0));
     if (k < least) k = least;
     t.kc = (int)(p.mode == SMALL || k > KB ? KB : k);

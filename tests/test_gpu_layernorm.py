@@ -329,3 +329,19 @@ def test_layer_norm_every_choice_of_gradients(rows, C, dtype):
         y = ops.layer_norm(*leaves)
         grads = iter(torch.autograd.grad(y, [t for t in leaves if t.requires_grad], dy))
         check(x, w, b, dy, 1e-5, y.detach(), *[next(grads) if t.requires_grad else None for t in leaves])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,C", [(1, 60000), (16, 33001), (17, 33001), (2, 65539)])
+def test_layer_norm_rows_beyond_registers(rows, C, dtype):
+    """Rows partly read again, at most 64 elements to a thread and half; with and without partial sums of the parameters."""
+    x, w, b, dy = make(rows, C, dtype, pad=5)
+    for want in (7, 1, 2, 6):
+        leaves = [t.detach().clone().requires_grad_(bool(want >> i & 1)) for i, t in enumerate((x, w, b))]
+        leaves[0] = x.detach().requires_grad_(bool(want & 1))
+        y = ops.layer_norm(*leaves)
+        grads = iter(torch.autograd.grad(y, [t for t in leaves if t.requires_grad], dy))
+        check(x, w, b, dy, 1e-5, y.detach(), *[next(grads) if t.requires_grad else None for t in leaves])
+    with torch.no_grad():
+        assert torch.equal(ops.layer_norm(x, w, b), y.detach())
