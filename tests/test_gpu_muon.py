@@ -1,9 +1,13 @@
 """snws.optim.FlatMuon and Trainer(optimizer="muon"): every update against its definition in float64, the state's format,
 checkpoints, and a block of a standardized convolution and a layer normalisation trained with it."""
 import math
+import os
+import socket
 
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 import patterns
 from modeling.layernorm import LayerNorm2d
@@ -244,3 +248,47 @@ def test_block_trained_with_flat_muon():
         opt.step()
         check_matrix(block.conv.weight, opt._slots[0][2], want, 0.02, "match_rms_adamw")
     opt.release()
+
+
+def _rank(rank, port, q):
+    import faulthandler
+    faulthandler.dump_traceback_later(90, exit=True)
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE="2")
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    from modeling.UNet3p_SNws import UNet3p_SNws
+    img, lab = patterns.synth_batch(2, 14, 64, 101)
+    model = UNet3p_SNws(14, 4, 10, 1, 1)
+    patterns.det_init(model)
+    tr = harness.Trainer(model.to(DEV), optimizer="muon", total_iters=50, bucket_mb=0.05)
+    opt = tr.opt
+    for it in range(2):
+        before, moments = opt.flat_p.clone(), opt.exp_avg.clone()
+        tr.step(img[rank:rank + 1].to(DEV), lab[rank:rank + 1].to(DEV))
+        for i in (i for i, m in enumerate(opt.is_matrix) if m and opt._touched[i]):
+            p, part = opt.params[i], slice(opt.offsets[i], opt.offsets[i] + opt.params[i].numel())
+            g, m, b = (t[part].view(p.shape) for t in (opt.flat_g, moments, before))
+            check_matrix(p, opt._slots[i][2], muon_definition(b, g, m, harness.poly_lr(0.002, it, 50), 5e-4, 0.95, True,
+                                                              "match_rms_adamw"), 0.002, "match_rms_adamw")
+    q.put((rank, opt.flat_p.cpu().numpy(), opt.flat_g.cpu().numpy(), len(tr.buckets.buckets)))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+@gpu
+def test_two_ranks_train_with_muon():
+    """Two ranks, an image each, gradients summed in buckets of the flat buffer: every update follows from the summed
+    gradient, and the replicas stay the same bit for bit."""
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_rank, args=(r, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    res = sorted((q.get(timeout=100) for _ in procs), key=lambda t: t[0])
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    assert res[0][3] >= 2
+    assert (res[0][1] == res[1][1]).all() and (res[0][2] == res[1][2]).all()
