@@ -417,11 +417,14 @@ __device__ __forceinline__ void product(f32x4 (&acc)[G::MR][G::NR], const unsign
   // LDS-DMA of rows: piece w + W j holds its rows 8 (w + W j) .. + 7; lane -> row lane >> 3, slot lane & 7, which receives the
   // 16-byte chunk slot ^ ((row >> 1) & 7), so that the 16 lanes of a fragment read hit distinct banks
   const int chunk = (lane & 7) ^ ((4 * (wave & 1) + (lane >> 4)) & 7);
-  // Offsets from the tile's first row: below 2^32, since a tile has at most 256 rows of at most 4 MB.  They are put together
-  // anew for every stage: an addition and a minimum each, where keeping them would cost registers the products need.
-  const unsigned line = KB * 128, first = (8 * wave + (lane >> 3)) * line, lastp = (unsigned)(M - 1 - p0) * line;
+  // Offsets from the tile's first row: at most 127 rows (Q: TN - 1) of at most 4 MB, below 2^30.  They are put together anew for
+  // every stage: an addition and a minimum each, where keeping them would cost registers the products need.  The last row they
+  // may reach is the matrix's or the tile's, whichever comes first: the distance to the matrix's alone would leave 32 bits from
+  // 2^30 numbers on.
+  const unsigned line = KB * 128, first = (8 * wave + (lane >> 3)) * line;
+  const unsigned lastp = (unsigned)(M - 1 - p0 < G::TM - 1 ? M - 1 - p0 : G::TM - 1) * line;
   const int64_t pitch = (int64_t)QB * 128;
-  const unsigned lastq = DOWN ? (unsigned)(QB - 1) * 128 : (unsigned)(N - 1 - q0) * line;
+  const unsigned lastq = DOWN ? (unsigned)(QB - 1) * 128 : (unsigned)(N - 1 - q0 < G::TN - 1 ? N - 1 - q0 : G::TN - 1) * line;
   // DOWN: piece c of Q is column block c / 4, k-rows 8 (c % 4) .. + 7 of the stage.  A transposing read takes 32 bytes from
   // each of 16 rows 8 g + t (g, t < 4): pairs of chunks trade places by (t >> 1) + 2 (g & 1), so that they meet in twos.
   const unsigned firstq = DOWN ? (unsigned)((q0 >> 5) + (wave >> 2)) * 128 : first;
