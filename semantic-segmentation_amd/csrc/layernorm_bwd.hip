@@ -298,30 +298,33 @@ __global__ __launch_bounds__(256) void ln_bwd_wide_param_kernel(BwdArgs a) {
   part[a.C + c] = db;
 }
 
-// dweight[c] / dbias[c] = sum over the partial rows, in float64 and a fixed order: 32 columns x 32 row lanes
+// dweight[c] / dbias[c] = sum over the partial rows, in float64 and a fixed order: 32 columns x 32 row lanes at a time
 __global__ __launch_bounds__(1024) void ln_param_sum_kernel(const float* __restrict__ part, int blocks, int C,
                                                             float* __restrict__ dw, float* __restrict__ db) {
   constexpr int LOADS = 8;
   __shared__ double red[32][33];
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  const int i = blockIdx.x * 32 + cl;
-  double s = 0.0;
-  if (i < 2 * C)
-    for (int r = rl; r < blocks; r += 32 * LOADS) {
-      float f[LOADS];        // in flight together
+  for (int i0 = blockIdx.x * 32; i0 < 2 * C; i0 += gridDim.x * 32) {
+    const int i = i0 + cl;
+    double s = 0.0;
+    if (i < 2 * C)
+      for (int r = rl; r < blocks; r += 32 * LOADS) {
+        float f[LOADS];        // in flight together
 #pragma unroll
-      for (int k = 0; k < LOADS; ++k) f[k] = r + 32 * k < blocks ? part[(int64_t)(r + 32 * k) * 2 * C + i] : 0.f;
+        for (int k = 0; k < LOADS; ++k) f[k] = r + 32 * k < blocks ? part[(int64_t)(r + 32 * k) * 2 * C + i] : 0.f;
 #pragma unroll
-      for (int k = 0; k < LOADS; ++k) s += (double)f[k];
+        for (int k = 0; k < LOADS; ++k) s += (double)f[k];
+      }
+    __syncthreads();           // the previous columns have been read
+    red[rl][cl] = s;
+    __syncthreads();
+    if (rl == 0 && i < 2 * C) {
+      s = 0.0;
+#pragma unroll
+      for (int r = 0; r < 32; ++r) s += red[r][cl];
+      float* o = i < C ? dw : db;
+      if (o) o[i < C ? i : i - C] = (float)s;
     }
-  red[rl][cl] = s;
-  __syncthreads();
-  if (rl == 0 && i < 2 * C) {
-    s = 0.0;
-#pragma unroll
-    for (int r = 0; r < 32; ++r) s += red[r][cl];
-    float* o = i < C ? dw : db;
-    if (o) o[i < C ? i : i - C] = (float)s;
   }
 }
 
@@ -371,7 +374,7 @@ struct Bwd {
     return SNWS_OK;
   }
   int wide() {
-    if (a.rows > 0x7fffffff) SNWS_UNSUPPORTED("snws_ln_bwd: too many rows of this length");
+    if (a.rows >= MAX_WIDE_ROWS) SNWS_UNSUPPORTED("snws_ln_bwd: too many rows of this length");
     if (a.dx) {
       ln_bwd_wide_kernel<T><<<(unsigned)a.rows, WIDE, 0, st>>>(a);
       SNWS_LAUNCH_CHECK("snws_ln_bwd");
@@ -422,7 +425,9 @@ extern "C" int snws_ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t 
     if (rc != SNWS_OK || few) return rc;
   }
   if (params) {
-    ln_param_sum_kernel<<<(unsigned)cdiv64(2 * (int64_t)C, 32), 1024, 0, st>>>(workspace, (int)blocks, C, dweight, dbias);
+    // (a launch holds less than 2^32 threads: the longest rows have more columns)
+    const int64_t most = 1 << 16, need = cdiv64(2 * (int64_t)C, 32);
+    ln_param_sum_kernel<<<(unsigned)(need < most ? need : most), 1024, 0, st>>>(workspace, (int)blocks, C, dweight, dbias);
     SNWS_LAUNCH_CHECK("snws_ln_bwd");
   }
   return SNWS_OK;

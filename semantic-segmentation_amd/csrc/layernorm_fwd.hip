@@ -194,7 +194,7 @@ struct Fwd {
     return SNWS_OK;
   }
   int wide() {
-    if (a.rows > 0x7fffffff) SNWS_UNSUPPORTED("snws_ln_fwd: too many rows of this length");
+    if (a.rows >= MAX_WIDE_ROWS) SNWS_UNSUPPORTED("snws_ln_fwd: too many rows of this length");
     ln_fwd_wide_kernel<T><<<(unsigned)a.rows, WIDE, 0, st>>>(a);
     SNWS_LAUNCH_CHECK("snws_ln_fwd");
     return SNWS_OK;

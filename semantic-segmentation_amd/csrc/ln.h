@@ -122,6 +122,7 @@ __device__ __forceinline__ float group_sum(float a, float* red) {
 // A row by a workgroup of 1024 threads, chunk after chunk: f(kept index or -1, chunk's first column, its dup).  The first KEEP
 // chunks of a thread have a constant index, so that what is kept of them stays in registers.
 constexpr int WIDE = 1024;
+constexpr int64_t MAX_WIDE_ROWS = (1ll << 32) / WIDE;      // a launch holds less than 2^32 threads: 4 million rows of 64 KB or more
 template <int VEC, int KEEP, typename F>
 __device__ __forceinline__ void wide_row(int C, F&& f) {
   const int chunks = (C + VEC - 1) / VEC;
