@@ -2,9 +2,13 @@
 // row's own C elements (the channels of one pixel in NHWC), rstd = 1 / sqrt(var + eps).
 //
 // Bound by memory: x is read once and y written once.  A row stays in registers between the two (ln.h), so the variance is
-// taken around the mean in a second sweep over registers - no cancellation however large the mean - in float32.
-// Measured: 262144 x 64 bfloat16 11.6 us (5.8 TB/s), 1048576 x 320 bfloat16 222 us (6.0 TB/s), 997 x 9216 float32 16.7 us
-// (4.4 TB/s), 10 x 512 float32 2.2 us (a launch).
+// taken around the mean in a second sweep over registers, in float32.  A float32 sum of C elements is off by some roundings of
+// the mean, which for a row far from zero is no small part of its spread: a constant row of 1000.1 came out as up to 0.4
+// instead of 0 (512 to 16384 elements).  So the second sweep also adds up the distances to that mean - exact numbers, where the row is far from zero -
+// and their mean corrects it.  The bfloat16 elements of such a row are multiples of one unit, at most 2^9 of it each: up to 2^15
+// of them add exactly in float32, and there is nothing to correct.
+// Measured: 262144 x 64 bfloat16 11.6 us (5.8 TB/s), 1048576 x 320 bfloat16 222 us (6.0 TB/s), 997 x 9216 float32 17.1 us
+// (4.3 TB/s), 10 x 512 float32 2.2 us (a launch).
 #include "ln.h"
 #include <math.h>
 
@@ -28,6 +32,13 @@ __device__ __forceinline__ float over(float s, float C, float inv) {
   const float m = s * inv;
   const float r = fmaf(-m, C, s);
   return isfinite(m) ? fmaf(r, inv, m) : m;
+}
+
+// whether the mean is corrected (see above)
+template <typename T> constexpr bool CORRECT = sizeof(T) == 4;
+// mean square around a number `off` below the mean -> variance; not below zero, and infinite where the squares overflow
+__device__ __forceinline__ float variance(float square, float off) {
+  return isfinite(square) ? fmaxf(fmaf(-off, off, square), 0.f) : square;
 }
 
 template <typename T, int G, int NV, bool TAIL>
@@ -60,26 +71,30 @@ __global__ __launch_bounds__(G <= 256 ? 256 : G) void ln_fwd_kernel(FwdArgs a) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) s += !TAIL || e >= dup[k] ? f[e] : 0.f;
     }
-    const float mean = over(group_sum<G>(s, red), (float)a.C, inv);
-    float q = 0.f;
+    const float near = over(group_sum<G>(s, red), (float)a.C, inv);
+    float q = 0.f, r = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float f[VEC];
       unpack(v[k], f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = f[e] - mean;
+        const float d = f[e] - near;
         q += !TAIL || e >= dup[k] ? d * d : 0.f;
+        if (CORRECT<T>) r += !TAIL || e >= dup[k] ? d : 0.f;
       }
     }
-    const float rstd = 1.f / sqrtf(group_sum<G>(q, red) * inv + a.eps);
+    if (CORRECT<T>) group_sum2<G>(q, r, red);
+    else q = group_sum<G>(q, red);
+    const float off = r * inv;
+    const float rstd = 1.f / sqrtf(variance(q * inv, off) + a.eps);
     T* yr = y + row * a.ldy;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float f[VEC];
       unpack(v[k], f);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f[e] = (f[e] - mean) * rstd * w[k][e] + b[k][e];
+      for (int e = 0; e < VEC; ++e) f[e] = (CORRECT<T> ? f[e] - near - off : f[e] - near) * rstd * w[k][e] + b[k][e];
       if (!TAIL || dup[k] == 0) {
         store_raw(yr + col[k], pack(f));
       } else {
@@ -89,7 +104,7 @@ __global__ __launch_bounds__(G <= 256 ? 256 : G) void ln_fwd_kernel(FwdArgs a) {
       }
     }
     if (a.mean && t == 0) {
-      a.mean[row] = mean;
+      a.mean[row] = near + off;
       a.rstd[row] = rstd;
     }
   }
@@ -109,23 +124,30 @@ __global__ __launch_bounds__(256) void ln_fwd_narrow_kernel(FwdArgs a) {
       f[e] = e < a.C ? (float)x[row * a.ldx + e] : 0.f;
       s += f[e];
     }
-    const float mean = over(s, (float)a.C, inv);
+    const float near = over(s, (float)a.C, inv);
+    float r = 0.f;
 #pragma unroll
-    for (int e = 0; e < M; ++e) q += e < a.C ? (f[e] - mean) * (f[e] - mean) : 0.f;
-    const float rstd = 1.f / sqrtf(q * inv + a.eps);
+    for (int e = 0; e < M; ++e) {
+      const float d = e < a.C ? f[e] - near : 0.f;
+      q += d * d;
+      r += d;
+    }
+    const float off = r * inv;
+    const float rstd = 1.f / sqrtf(variance(q * inv, off) + a.eps);
 #pragma unroll
     for (int e = 0; e < M; ++e)
-      if (e < a.C) y[row * a.ldy + e] = (T)((f[e] - mean) * rstd * (a.w ? a.w[e] : 1.f) + (a.b ? a.b[e] : 0.f));
+      if (e < a.C) y[row * a.ldy + e] = (T)((f[e] - near - off) * rstd * (a.w ? a.w[e] : 1.f) + (a.b ? a.b[e] : 0.f));
     if (a.mean) {
-      a.mean[row] = mean;
+      a.mean[row] = near + off;
       a.rstd[row] = rstd;
     }
   }
 }
 
 // Longer rows: the first 8 chunks of each of 1024 threads stay in registers, what lies behind them is read for each sweep, out
-// of the caches.  4096 x 20000 float32 175 us (3.7 TB/s; three sweeps over memory with 4-byte loads: 249), 1000 x 33000 bfloat16
-// 39 us (71).  A row is one workgroup's, however long: 1 x 100000 takes as long as 8.
+// of the caches.  4096 x 20000 float32 184 us (3.6 TB/s; three sweeps over memory with 4-byte loads: 249), 1000 x 33000 bfloat16
+// 40 us (71).  A row is one workgroup's, however long: 1 x 100000 takes as long as 8.  A thread adds up to 2^18 elements: the sum
+// of a chunk is float32, the thread's float64.
 template <typename T>
 __global__ __launch_bounds__(WIDE) void ln_fwd_wide_kernel(FwdArgs a) {
   constexpr int VEC = Geo<T>::VEC, KEEP = 8;
@@ -135,33 +157,40 @@ __global__ __launch_bounds__(WIDE) void ln_fwd_wide_kernel(FwdArgs a) {
   uint4 v[KEEP];
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) v[i] = make_uint4(0, 0, 0, 0);
-  float s = 0.f, q = 0.f;
+  double s = 0.0, q = 0.0, r = 0.0;
   wide_row<VEC, KEEP>(a.C, [&](int kept, int c, int dup) {
     const uint4 raw = load_raw(x + c);
     if (kept >= 0) v[kept] = raw;
-    float f[VEC];
+    float f[VEC], sc = 0.f;
     unpack(raw, f);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) s += e >= dup ? f[e] : 0.f;
+    for (int e = 0; e < VEC; ++e) sc += e >= dup ? f[e] : 0.f;
+    s += (double)sc;
   });
-  const float mean = over(group_sum<WIDE>(s, red), (float)a.C, 1.f / (float)a.C);
+  const float near = over(group_sum<WIDE>((float)s, red), (float)a.C, 1.f / (float)a.C);
   wide_row<VEC, KEEP>(a.C, [&](int kept, int c, int dup) {
-    float f[VEC];
+    float f[VEC], qc = 0.f, rc = 0.f;
     unpack(kept >= 0 ? v[kept] : load_raw(x + c), f);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const float d = f[e] - mean;
-      q += e >= dup ? d * d : 0.f;
+      const float d = e >= dup ? f[e] - near : 0.f;
+      qc += d * d;
+      rc += d;
     }
+    q += (double)qc;
+    if (CORRECT<T>) r += (double)rc;
   });
-  const float rstd = 1.f / sqrtf(group_sum<WIDE>(q, red) / (float)a.C + a.eps);
+  float square = (float)q, off = (float)r;
+  group_sum2<WIDE>(square, off, red);
+  off /= (float)a.C;
+  const float rstd = 1.f / sqrtf(variance(square / (float)a.C, off) + a.eps);
   wide_row<VEC, KEEP>(a.C, [&](int kept, int c, int dup) {
     float f[VEC], w[VEC], b[VEC];
     unpack(kept >= 0 ? v[kept] : load_raw(x + c), f);
     load_param<VEC>(a.w, c, 1.f, w);
     load_param<VEC>(a.b, c, 0.f, b);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = (f[e] - mean) * rstd * w[e] + b[e];
+    for (int e = 0; e < VEC; ++e) f[e] = (CORRECT<T> ? f[e] - near - off : f[e] - near) * rstd * w[e] + b[e];
     if (dup == 0) {
       store_raw(y + c, pack(f));
     } else {
@@ -171,7 +200,7 @@ __global__ __launch_bounds__(WIDE) void ln_fwd_wide_kernel(FwdArgs a) {
     }
   });
   if (a.mean && threadIdx.x == 0) {
-    a.mean[blockIdx.x] = mean;
+    a.mean[blockIdx.x] = near + off;
     a.rstd[blockIdx.x] = rstd;
   }
 }

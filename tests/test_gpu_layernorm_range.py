@@ -23,3 +23,37 @@ def test_parameter_gradients_of_the_longest_rows(rows):
     assert dw.shape == db.shape == (C,)
     assert not bool(dw.any())
     assert torch.equal(db, rows * column)
+
+
+LENGTHS = [2, 3, 30, 100, 512, 1283, 2049, 9216, 16384, 20000, 300001]
+
+
+@gpu
+@pytest.mark.parametrize("C", LENGTHS)
+def test_constant_rows_far_from_zero(C):
+    """They give the bias.  The first mean is a float32 sum in a tree of at most 73 roundings, so off by less than 146 half
+    steps u with the division's; the corrected one by that share of the distance that is left; rstd is 1 / sqrt(eps)."""
+    gen = torch.Generator(device=DEV).manual_seed(C)
+    w, b = (torch.randn(C, generator=gen, device=DEV) for _ in range(2))
+    for value in (1000.1, -77.7, 30000.3, 0.1):
+        x = torch.full((3, C), value, device=DEV)
+        slack = 316.3 * abs(value) * (146 * U) ** 2
+        y = ops.layer_norm(x, w, b, 1e-5)
+        assert bool(((y - b).abs() <= slack * w.abs() + 2 * U * b.abs()).all()), (value, float((y - b).abs().max()))
+
+
+@gpu
+@pytest.mark.parametrize("C", LENGTHS)
+def test_rows_far_from_zero(C):
+    """The mean's size is not in the bound: an element's distance to it is exact (they lie within a factor of two), its
+    correction off by at most 73 roundings of the mean distance, which is at most the spread; rstd by as many.  256 u of z
+    and of one covers them and the single roundings behind."""
+    gen = torch.Generator(device=DEV).manual_seed(C)
+    x = 1e4 * (1 + torch.rand(20, 1, generator=gen, device=DEV)) + torch.randn(20, C, generator=gen, device=DEV)
+    w, b = (torch.randn(C, generator=gen, device=DEV) for _ in range(2))
+    y = ops.layer_norm(x, w, b, 1e-5)
+    xd = x.double()
+    z = (xd - xd.mean(1, keepdim=True)) / (xd.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+    want = z * w + b
+    assert bool(((y - want).abs() <= 256 * U * (z.abs() + 1) * w.abs() + 4 * U * (want.abs() + b.abs())).all()), \
+        float((y - want).abs().max())
