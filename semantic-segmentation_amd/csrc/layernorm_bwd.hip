@@ -225,7 +225,8 @@ __global__ __launch_bounds__(256) void ln_bwd_narrow_kernel(BwdArgs a) {
   }
 }
 
-// rows beyond what the kernel above holds: 4 chunks of x and dy of each of 1024 threads stay in registers
+// rows beyond what the kernel above holds: 4 chunks of x and dy of each of 1024 threads stay in registers; the sum
+// of a chunk is float32, a thread's, of up to 2^18 elements, float64
 template <typename T>
 __global__ __launch_bounds__(WIDE) void ln_bwd_wide_kernel(BwdArgs a) {
   constexpr int VEC = Geo<T>::VEC, KEEP = 4;
@@ -238,26 +239,30 @@ __global__ __launch_bounds__(WIDE) void ln_bwd_wide_kernel(BwdArgs a) {
   uint4 vx[KEEP], vg[KEEP];
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) vx[i] = vg[i] = make_uint4(0, 0, 0, 0);
-  float s1 = 0.f, s2 = 0.f;
+  double s1 = 0.0, s2 = 0.0;
   wide_row<VEC, KEEP>(a.C, [&](int kept, int c, int dup) {
     const uint4 rx = load_raw(x + c), rg = load_raw(dy + c);
     if (kept >= 0) {
       vx[kept] = rx;
       vg[kept] = rg;
     }
-    float f[VEC], g[VEC], w[VEC];
+    float f[VEC], g[VEC], w[VEC], c1 = 0.f, c2 = 0.f;
     unpack(rx, f);
     unpack(rg, g);
     load_param<VEC>(a.w, c, 1.f, w);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       const float d = e >= dup ? g[e] * w[e] : 0.f;
-      s1 += d;
-      s2 += e >= dup ? d * ((f[e] - mean) * rstd) : 0.f;
+      c1 += d;
+      c2 += e >= dup ? d * ((f[e] - mean) * rstd) : 0.f;
     }
+    s1 += (double)c1;
+    s2 += (double)c2;
   });
-  group_sum2<WIDE>(s1, s2, red);
-  const float m1 = s1 / (float)a.C, m2 = s2 / (float)a.C;
+  float m1 = (float)s1, m2 = (float)s2;
+  group_sum2<WIDE>(m1, m2, red);
+  m1 /= (float)a.C;
+  m2 /= (float)a.C;
   wide_row<VEC, KEEP>(a.C, [&](int kept, int c, int dup) {
     float f[VEC], g[VEC], w[VEC];
     unpack(kept >= 0 ? vx[kept] : load_raw(x + c), f);
@@ -275,27 +280,28 @@ __global__ __launch_bounds__(WIDE) void ln_bwd_wide_kernel(BwdArgs a) {
   });
 }
 
-// parameter gradients of such rows: a thread per column, rows dealt to gridDim.y slices
+// Parameter gradients of such rows: a thread per column, rows dealt to gridDim.y slices.  The slices get fewer as rows get longer,
+// and a thread's rows many, so it adds them in float64.
 template <typename T>
 __global__ __launch_bounds__(256) void ln_bwd_wide_param_kernel(BwdArgs a) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= a.C) return;
   const T* x = static_cast<const T*>(a.x);
   const T* dy = static_cast<const T*>(a.dy);
-  float dw = 0.f, db = 0.f;
+  double dw = 0.0, db = 0.0;
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const float g = (float)dy[row * a.lddy + c];
-    db += g;
-    dw += g * ((float)x[row * a.ldx + c] - a.mean[row]) * a.rstd[row];
+    db += (double)g;
+    dw += (double)(g * (((float)x[row * a.ldx + c] - a.mean[row]) * a.rstd[row]));
   }
   if (!a.part) {               // one slice: no partial rows
-    if (a.dw) a.dw[c] = dw;
-    if (a.db) a.db[c] = db;
+    if (a.dw) a.dw[c] = (float)dw;
+    if (a.db) a.db[c] = (float)db;
     return;
   }
   float* part = a.part + (int64_t)blockIdx.y * 2 * a.C;
-  part[c] = dw;
-  part[a.C + c] = db;
+  part[c] = (float)dw;
+  part[a.C + c] = (float)db;
 }
 
 // dweight[c] / dbias[c] = sum over the partial rows, in float64 and a fixed order: 32 columns x 32 row lanes at a time

@@ -57,3 +57,25 @@ def test_rows_far_from_zero(C):
     want = z * w + b
     assert bool(((y - want).abs() <= 256 * U * (z.abs() + 1) * w.abs() + 4 * U * (want.abs() + b.abs())).all()), \
         float((y - want).abs().max())
+
+
+@gpu
+@pytest.mark.parametrize("rows,C,dtype", [(3000, 16640, torch.float32), (2000, 262160, torch.float32), (700, 40001, torch.bfloat16)])
+def test_parameter_gradients_of_many_long_rows(rows, C, dtype):
+    """Positive terms, so that nothing hides an error: a float32 sum of a thread's rows would be off by up to 50 roundings.
+    dbias: a partial sum and the total are rounded once each.  dweight: x lies in [1, 2] with a spread of 0.29, so the mean's
+    rounding is 4 half steps of z and the distance to it exact; rstd, the product and the term itself make 6 of z's own."""
+    gen = torch.Generator(device=DEV).manual_seed(rows)
+    x = (1 + torch.rand(rows, C, generator=gen, device=DEV)).to(dtype)
+    dy = (0.5 + torch.rand(rows, C, generator=gen, device=DEV)).to(dtype)
+    w, b = (torch.ones(C, device=DEV, requires_grad=True) for _ in range(2))
+    dw, db = torch.autograd.grad(ops.layer_norm(x, w, b, 1e-5), (w, b), dy)
+    want_w, want_b, size = (torch.zeros(C, dtype=torch.float64, device=DEV) for _ in range(3))
+    for r in range(0, rows, 100):
+        xs, ds = x[r:r + 100].double(), dy[r:r + 100].double()
+        z = (xs - xs.mean(1, keepdim=True)) / (xs.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+        want_w += (ds * z).sum(0)
+        want_b += ds.sum(0)
+        size += (ds * (z.abs() + 1)).sum(0)
+    assert bool(((db.double() - want_b).abs() <= 2.02 * U * want_b).all()), float(((db.double() - want_b) / want_b).abs().max() / U)
+    assert bool(((dw.double() - want_w).abs() <= 8 * U * size).all()), float(((dw.double() - want_w).abs() / size).max() / U)
