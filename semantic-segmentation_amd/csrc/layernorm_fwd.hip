@@ -4,9 +4,9 @@
 // Bound by memory: x is read once and y written once.  A row stays in registers between the two (ln.h), so the variance is
 // taken around the mean in a second sweep over registers, in float32.  A float32 sum of C elements is off by some roundings of
 // the mean, which for a row far from zero is no small part of its spread: a constant row of 1000.1 came out as up to 0.4
-// instead of 0 (512 to 16384 elements).  So the second sweep also adds up the distances to that mean - exact numbers, where the row is far from zero -
-// and their mean corrects it.  The bfloat16 elements of such a row are multiples of one unit, at most 2^9 of it each: up to 2^15
-// of them add exactly in float32, and there is nothing to correct.
+// instead of 0 (512 to 16384 elements).  So the second sweep also adds up the distances to that mean - exact numbers, where the
+// row is far from zero - and their mean corrects it.  The bfloat16 elements of such a row are multiples of one unit, at most 2^9
+// of it each: up to 2^15 of them, as many as the registers take, add exactly in float32, and there is nothing to correct.
 // Measured: 262144 x 64 bfloat16 11.6 us (5.8 TB/s), 1048576 x 320 bfloat16 222 us (6.0 TB/s), 997 x 9216 float32 17.1 us
 // (4.3 TB/s), 10 x 512 float32 2.2 us (a launch).
 #include "ln.h"
@@ -34,7 +34,7 @@ __device__ __forceinline__ float over(float s, float C, float inv) {
   return isfinite(m) ? fmaf(r, inv, m) : m;
 }
 
-// whether the mean is corrected (see above)
+// whether the mean of a row in registers is corrected (see above)
 template <typename T> constexpr bool CORRECT = sizeof(T) == 4;
 // mean square around a number `off` below the mean -> variance; not below zero, and infinite where the squares overflow
 __device__ __forceinline__ float variance(float square, float off) {
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(WIDE) void ln_fwd_wide_kernel(FwdArgs a) {
       rc += d;
     }
     q += (double)qc;
-    if (CORRECT<T>) r += (double)rc;
+    r += (double)rc;
   });
   float square = (float)q, off = (float)r;
   group_sum2<WIDE>(square, off, red);
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(WIDE) void ln_fwd_wide_kernel(FwdArgs a) {
     load_param<VEC>(a.w, c, 1.f, w);
     load_param<VEC>(a.b, c, 0.f, b);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = (CORRECT<T> ? f[e] - near - off : f[e] - near) * rstd * w[e] + b[e];
+    for (int e = 0; e < VEC; ++e) f[e] = (f[e] - near - off) * rstd * w[e] + b[e];
     if (dup == 0) {
       store_raw(y + c, pack(f));
     } else {

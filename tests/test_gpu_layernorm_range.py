@@ -79,3 +79,16 @@ def test_parameter_gradients_of_many_long_rows(rows, C, dtype):
         size += (ds * (z.abs() + 1)).sum(0)
     assert bool(((db.double() - want_b).abs() <= 2.02 * U * want_b).all()), float(((db.double() - want_b) / want_b).abs().max() / U)
     assert bool(((dw.double() - want_w).abs() <= 8 * U * size).all()), float(((dw.double() - want_w).abs() / size).max() / U)
+
+
+@gpu
+@pytest.mark.parametrize("C", [100, 32768, 40001, 1 << 21, (1 << 22) + 3])
+def test_constant_bfloat16_rows_far_from_zero(C):
+    """Up to 2^15 such elements add exactly; more of them need the correction as float32 rows do.  The result is rounded once."""
+    gen = torch.Generator(device=DEV).manual_seed(C)
+    w, b = (torch.randn(C, generator=gen, device=DEV) for _ in range(2))
+    for value in (1004.0, -77.5, 30080.0, 25559040.0, 0.1):
+        x = torch.full((2, C), value, device=DEV).bfloat16()
+        slack = 316.3 * abs(float(x[0, 0])) * (146 * U) ** 2
+        y = ops.layer_norm(x, w, b, 1e-5).float()
+        assert bool(((y - b).abs() <= 1.01 * (slack * w.abs() + 2.0 ** -8 * b.abs())).all()), (value, float((y - b).abs().max()))
