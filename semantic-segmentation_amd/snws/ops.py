@@ -1383,6 +1383,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     require_gpu(x, "layer_norm")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("layer_norm: a last axis of at least one element expected, got shape %s" % (tuple(x.shape),))
+    if x.shape[-1] >> 31:       # (a longer one than the kernels take is refused there; this one would be cut to 32 bits)
+        raise ValueError("layer_norm: a last axis of %d elements is too long" % x.shape[-1])
     dtype_code(x)
     eps = float(eps)
     w32, b32 = _param32(weight, x.shape[-1], "weight", x), _param32(bias, x.shape[-1], "bias", x)
@@ -2375,6 +2377,8 @@ def _ortho_coefficients(coefficients, steps):
 
 def _ortho_bytes(rows, cols, steps):
     n = len(rows)
+    if max(max(rows), max(cols)) >> 31:      # (smaller ones than that are refused by the library, these would be cut to 32 bits)
+        raise ValueError("orthogonalize: %d rows or columns are too many" % max(max(rows), max(cols)))
     ints = ctypes.c_int * n
     nbytes = L.lib().snws_ortho_workspace_bytes(ints(*rows), ints(*cols), n, steps)
     if nbytes < 0:

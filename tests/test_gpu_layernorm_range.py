@@ -92,3 +92,14 @@ def test_constant_bfloat16_rows_far_from_zero(C):
         slack = 316.3 * abs(float(x[0, 0])) * (146 * U) ** 2
         y = ops.layer_norm(x, w, b, 1e-5).float()
         assert bool(((y - b).abs() <= 1.01 * (slack * w.abs() + 2.0 ** -8 * b.abs())).all()), (value, float((y - b).abs().max()))
+
+
+@gpu
+def test_rows_beyond_32_bits_are_refused():
+    """A length handed to the library is 32 bits wide: 2^32 + 8 must not arrive there as 8.  (Expanded rows: nothing of that size
+    is laid out.)"""
+    x = torch.zeros(1, 1, device=DEV)
+    with pytest.raises(ValueError, match="too long"):
+        ops.layer_norm(x.expand(1, (1 << 32) + 8))
+    with pytest.raises(ValueError, match="too long"):
+        ops.layer_norm(x.expand(1, 1 << 31))

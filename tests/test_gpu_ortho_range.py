@@ -10,6 +10,23 @@ DEV = "cuda:0"
 gpu = pytest.mark.gpu
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    """A size handed to the library is 32 bits wide: 2^32 + 9 must not arrive there as 9."""
+    big = (1 << 32) + 9
+    for rows, cols in (([big], [3]), ([3], [big]), ([4, 3], [9, 1 << 31])):
+        with pytest.raises(ValueError, match="too many"):
+            ops._ortho_bytes(rows, cols, 5)
+    with pytest.raises(ValueError, match="larger"):
+        ops._ortho_bytes([3], [(1 << 31) - 1], 5)
+
+
+@gpu
+def test_long_matrices_are_refused():
+    big = torch.zeros((1 << 32) + 9, 1, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="too many"):
+        ops.orthogonalize(big)
+
+
 @gpu
 @pytest.mark.parametrize("rows,cols", [(1025, 1 << 20), (300000, 4096)])
 def test_more_numbers_than_a_tile_s_offsets_hold(rows, cols):
