@@ -2370,7 +2370,7 @@ def _ortho_coefficients(coefficients, steps):
     if len(rows) != int(steps) or any(len(r) != 3 for r in rows):
         raise ValueError("orthogonalize: three coefficients, or three for each of the %d steps, expected" % int(steps))
     known = (ctypes.c_float * (3 * len(rows)))(*[float(v) for r in rows for v in r])
-    if isinstance(coefficients, tuple) and isinstance(coefficients[0], float) and len(_COEFFICIENTS) < 64:
+    if isinstance(coefficients, tuple) and all(isinstance(v, float) for v in coefficients) and len(_COEFFICIENTS) < 64:
         _COEFFICIENTS[(coefficients, steps)] = known
     return known
 

@@ -1,4 +1,5 @@
-"""Orthogonalisation at the far ends of the sizes it takes: matrices of more than 2^30 numbers."""
+"""Orthogonalisation at the far ends of what it takes: matrices of more than 2^30 numbers, sizes beyond 32 bits, coefficients
+that change."""
 import math
 
 import pytest
@@ -18,6 +19,14 @@ def test_sizes_beyond_32_bits_are_refused():
             ops._ortho_bytes(rows, cols, 5)
     with pytest.raises(ValueError, match="larger"):
         ops._ortho_bytes([3], [(1 << 31) - 1], 5)
+
+
+def test_coefficients_that_change_are_read_again():
+    b = torch.tensor(-4.0)
+    given = (3.0, b, 2.0)
+    assert list(ops._ortho_coefficients(given, 1)) == [3.0, -4.0, 2.0]
+    b.fill_(-5.0)
+    assert list(ops._ortho_coefficients(given, 1)) == [3.0, -5.0, 2.0]
 
 
 @gpu
