@@ -251,6 +251,8 @@ class FlatMuon(FlatAdamW):
             if st is None:
                 continue
             names = ("momentum_buffer",) if self.is_matrix[i] else ("exp_avg", "exp_avg_sq")
+            if not self.is_matrix[i] and "step" not in st:
+                raise ValueError("FlatMuon.load_state_dict: parameter %s has no step count" % key)
             if any(k not in st or st[k].shape != self.params[i].shape for k in names):
                 raise ValueError("FlatMuon.load_state_dict: parameter %s needs %s of shape %s"
                                  % (key, " and ".join(names), tuple(self.params[i].shape)))
