@@ -17,9 +17,9 @@
 //
 // All matrices of a list share each launch: a workgroup finds its matrix and tile from its index.
 //
-// Measured, float32, five steps: 64 x 126 21 us (one launch), 1024 x 9216 355 us (norm 8, start 16, X X^T 31.5 and its join
+// Measured, float32, five steps: 64 x 126 21 us (one launch), 1024 x 9216 354 us (norm 8, start 16, X X^T 31.5 and its join
 // 8 twice, 13 launches of m x m products at 10.8, Q X 53 and 59), the 21 million numbers of 17 filters with their Muon
-// update 700 us (45, 52, 60 and 9.5 twice, 13 x 19, 105 and 125).
+// update 800 us (the nine filters of 128 rows and more in threes, then the eight of 64 in single steps).
 #include "common.h"
 #include <math.h>
 
@@ -69,7 +69,8 @@ struct Op {
   unsigned char kind, sp, sq, sc, sd, last, pad[2];
   float ca, cb, cc;
 };
-constexpr int MAX_OPS = 24;    // of a program that one kernel runs: six steps in groups take at most 22
+constexpr int MAX_OPS = 24;    // of a program that one kernel runs: eight single steps
+constexpr int GROUP_OPS = 12;  // of a group of three: X X^T, nine products of m x m matrices, Q X
 struct Program {
   int n;
   Op op[MAX_OPS];
@@ -916,7 +917,7 @@ static_assert(MAX_OPS <= 64 && sizeof(Op) % 4 == 0, "an operation to a lane");
 
 // Up to 64 rows the m x m matrices stay in LDS, 16 KB each: slot k, 32-column block b, row r, 16-byte chunks as in the
 // stages of product().  A workgroup computes the whole 64 x 64 product, and a lane's four rows of one column are, by
-// symmetry, four columns of one row: they go back without any transposition.  An operation takes 0.9 us this way (1.2 with
+// symmetry (of X X^T and A A^T, up to rounding), four columns of one row: they go back without any transposition.  An operation takes 0.9 us this way (1.2 with
 // four waves), 2.7 us through global memory.
 constexpr int SLOT64 = 64 * 2 * 128;
 
@@ -995,25 +996,25 @@ __device__ __forceinline__ f32x4 product64(const unsigned char* P, const unsigne
   if (b < nb) multiply64(acc, one);
   return acc;
 }
-__device__ __forceinline__ void square64(const Op& op, int m, unsigned char* slots, const Lane64& L) {
+// the polynomial of A in slot 0 into slot 1
+__device__ __forceinline__ void polynomial64(const Op& op, int m, unsigned char* slots, const Lane64& L) {
   Old64 old{};
   if (op.cb != 0.f) {
-    old.hi = *reinterpret_cast<const f16x4*>(slots + op.sc * SLOT64 + L.at[0]);
-    old.lo = *reinterpret_cast<const f16x4*>(slots + op.sc * SLOT64 + L.at[1]);
+    old.hi = *reinterpret_cast<const f16x4*>(slots + L.at[0]);
+    old.lo = *reinterpret_cast<const f16x4*>(slots + L.at[1]);
   }
-  const f32x4 acc = product64(slots + op.sp * SLOT64, slots + op.sq * SLOT64, up32(m) >> 5, L);
-  put64(acc, op.ca, op.cb, op.cc, m, slots + op.sd * SLOT64, old, L);
+  const f32x4 acc = product64(slots, slots, up32(m) >> 5, L);
+  put64(acc, op.ca, op.cb, op.cc, m, slots + SLOT64, old, L);
   lds_done();
 }
 
-// The m x m operations of a group for matrices of up to 64 rows; the last slot written is Q, which goes to global memory.
-__global__ __launch_bounds__(THREADS64) void ortho_chain64_kernel(Work a, float f, Program prog) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const Ops ops(prog);
+// A step's polynomial P = ca I + cb A + cc A^2 for matrices of up to 64 rows, a workgroup each, from the parts of A = X X^T.
+__global__ __launch_bounds__(THREADS64) void ortho_few_kernel(Work a, float f, Op op) {
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * SLOT64];
   const Mat t = a.count > 1 ? uniform(&reinterpret_cast<const Mats*>(a.ws)->mat[blockIdx.x]) : a.only;
   const Lane64 L;
   const int m = t.m, nb = up32(m) >> 5;
-  unsigned char* A = slot_of(t, a.ws, 0);
+  unsigned char* A = slot_of(t, a.ws, op.sp);
   if (t.ks > 1) {
     // the partial tiles of A, in the order of the splits
     const f32x4* part = part_of(t, a.ws) + threadIdx.x;
@@ -1031,24 +1032,20 @@ __global__ __launch_bounds__(THREADS64) void ortho_chain64_kernel(Work a, float 
     }
   }
   __syncthreads();
-  int last = 0;
-  for (int k = 0; k < prog.n; ++k) {
-    const Op op = ops[k];
-    square64(op, m, smem, L);
-    last = op.sd;
-  }
-  unsigned char* Q = slot_of(t, a.ws, last);
+  polynomial64(op, m, smem, L);
+  unsigned char* P = slot_of(t, a.ws, op.sd);
   for (int id = threadIdx.x; id < m * nb * 8; id += THREADS64) {
     const int r = id / (nb * 8), b = (id >> 3) % nb, c = id & 7;
-    *reinterpret_cast<uint4*>(Q + ((int64_t)r * nb + b) * 128 + c * 16) =
-        *reinterpret_cast<const uint4*>(smem + last * SLOT64 + b * 8192 + r * 128 + (c ^ ((r >> 1) & 7)) * 16);
+    *reinterpret_cast<uint4*>(P + ((int64_t)r * nb + b) * 128 + c * 16) =
+        *reinterpret_cast<const uint4*>(smem + SLOT64 + b * 8192 + r * 128 + (c ^ ((r >> 1) & 7)) * 16);
   }
 }
 
 // The whole call for small matrices, a workgroup each and a single launch: here the time of a launch, and of the latencies
 // behind it, is all there is to save.  X lives in LDS too, as 32-column blocks of 64 rows in the layout of the slots; Q X
-// replaces it 64 columns at a time, each depending on themselves only.
-constexpr int SMALL_N = 192, SMALL_LDS = (SLOTS + SMALL_N / 64) * SLOT64;
+// replaces it 64 columns at a time, each depending on themselves only.  As many columns as LDS holds beside A and P: 64 x 256
+// takes 35 us this way and 65 in the launches of FEW, 64 x 448 54 and 65, eight of them 55 and 77.
+constexpr int SMALL_N = 448, SMALL_LDS = (2 + SMALL_N / 64) * SLOT64;
 
 // columns 64 c .. of X <- f Q X, or the result.  The operands trade sides, D[j][i] = sum_k X[k][j] Q[i][k]: a lane then has
 // four columns of one row of the result.
@@ -1114,7 +1111,7 @@ __global__ __launch_bounds__(THREADS64) void ortho_small_kernel(Mats a, MuonArgs
   keep(&mine, a.mat[blockIdx.x]);
   __syncthreads();
   const Mat t = uniform(&mine);
-  unsigned char* X = smem + SLOTS * SLOT64;
+  unsigned char* X = smem + 2 * SLOT64;
   const Lane64 L;
   const int m = t.m, n = t.n, KB = up32(n) >> 5;
   // the matrix, eight elements at a time, stays in registers until its norm is known
@@ -1194,9 +1191,9 @@ __global__ __launch_bounds__(THREADS64) void ortho_small_kernel(Mats a, MuonArgs
       put64(product64(X, X, KB, L), 0.f, 0.f, op.cc, m, smem, Old64{}, L);
       lds_done();
     } else if (op.kind == K_SQUARE) {
-      square64(op, m, smem, L);
+      polynomial64(op, m, smem, L);
     } else {
-      for (int c = 0; c * 64 < n; ++c) apply64<T, MUON>(t, X, smem + op.sq * SLOT64, c, op.cc, op.last, u, L);
+      for (int c = 0; c * 64 < n; ++c) apply64<T, MUON>(t, X, smem + SLOT64, c, op.cc, op.last, u, L);
       lds_done();
     }
   }
@@ -1254,9 +1251,9 @@ bool ortho_scales(const float* coeff, int steps, Scales* s) {
   return true;
 }
 
-// How a call is run.  GENERAL: every product a launch over all its tiles.  CHAIN: one launch for the m x m products of a
-// group, where they fit LDS (m <= 64).  SMALL: one launch for everything.
-enum Mode { GENERAL, CHAIN, SMALL };
+// How a run is done.  GENERAL: every product a launch over all its tiles.  FEW: up to 64 rows, where one workgroup adds the
+// parts of X X^T and makes a step's polynomial of it.  SMALL: one launch for everything.
+enum Mode { GENERAL, FEW, SMALL };
 
 struct Plan {
   Mode mode;
@@ -1277,36 +1274,49 @@ int square_tiles(int m, int T) {
   return n;
 }
 
+// Steps in groups: with A = X X^T a step multiplies X by P = a I + b A + c A^2, and the next A is P A P.  Three steps then cost
+// one product each way with X and nine with m x m matrices instead of three each way and three.  That pays where n >= 2 m:
+// 1024 x 9216 takes 708 us in single steps, 557 in twos, 481 in threes (with the tiles of that time).
+// Its price is rounding: A is not taken anew from X, so directions far below the largest lose digits, the more the fewer there
+// are to share the error.  Largest error against float64, over that of single steps with float32 products, of twelve kinds of
+// spectra: single steps 3.6 (3 x 9), 2.7 (8 x 72), 1.5 to 1.6 (from 36 x 324 to 1024 x 9216); threes 4.0 (65 x 200), 3.1
+// (80 x 170), 2.6 (100 x 300), 2.2 (128 x 300), 2.0 (512 x 1100), 2.2 (1024 x 9216), but 6 to 400 up to 64 rows.  So: threes from
+// m = 128 on, else single steps, whatever the type.  The choice is each matrix's own: a list with both is two runs.
+bool in_threes(const Mat& t) { return t.m >= 128 && t.n >= 2 * t.m; }
+
+// the matrices of a call in one run or two
+struct Parts {
+  int count;
+  Mats list[2];
+  int group[2];      // steps taken together
+};
+void split(const Mats& a, Parts& s) {
+  s.count = 0;
+  for (int threes = 1; threes >= 0; --threes) {
+    Mats& l = s.list[s.count];
+    l.count = 0;
+    for (int i = 0; i < a.count; ++i)
+      if (in_threes(a.mat[i]) == (threes != 0)) l.mat[l.count++] = a.mat[i];
+    if (!l.count) continue;
+    l.ws = a.ws;
+    s.group[s.count++] = threes ? 3 : 1;
+  }
+}
+
 // Places the workspace, chooses mode, tiles and splits, and counts workgroups.
-//
-// Steps in groups: with A = X X^T a step multiplies X by P = a I + b A + c A^2, and the next A is P A P.  Two steps then cost
-// one product each way with X and five with m x m matrices instead of two each way and two; three steps 1 + 1 and nine.
-// That pays where n >= 2 m: 1024 x 9216 takes 708 us in single steps, 557 in twos, 481 in threes (with the tiles of that
-// time).  Its price is rounding: A is not taken anew from X, so directions far below the largest lose digits.  The error
-// against float64, over that of single steps with float32 products (six kinds of spectra, 64 x 126 to 1024 x 9216): single
-// 0.4 to 1.6; groups of two 0.4 to 2.1; of three 1.0 to 3.9 below m = 512, 0.6 to 1.2 from there on, where the long float32
-// sums dominate; of five up to 600.  So: three from m = 512 on and for results that carry less (bfloat16; an update added
-// to a parameter), else two.
-void make_plan(Mats& a, Plan& p, int steps, bool coarse) {
+void make_plan(Mats& a, Plan& p, int steps, int group) {
   int64_t apply = 0, grams = 0;
-  double long_ops = 0.0, square_ops = 0.0;
-  int mmax = 0, mmin = 1 << 30, nmax = 0;
+  int mmax = 0, nmax = 0;
   for (int i = 0; i < a.count; ++i) {
     const Mat& t = a.mat[i];
     grams += tri(t.m, 128) * cdiv64(up32(t.n) >> 5, 8);
     apply += (int64_t)cdiv(t.m, 128) * cdiv(t.n, 128);
     mmax = t.m > mmax ? t.m : mmax;
-    mmin = t.m < mmin ? t.m : mmin;
     nmax = t.n > nmax ? t.n : nmax;
-    square_ops += (double)t.m * t.m * t.m;
-    long_ops += (double)t.m * t.m * t.n;
   }
-  p.group = long_ops < 2.0 * square_ops ? 1 : coarse || mmin >= 512 ? 3 : 2;
+  p.group = group;
   p.mode = GENERAL;
-  if (steps <= 6) {
-    if (mmax <= 64 && nmax <= SMALL_N) p.mode = SMALL;
-    else if (mmax <= 64) p.mode = CHAIN;
-  }
+  if (mmax <= 64) p.mode = nmax <= SMALL_N && 3 * steps <= MAX_OPS ? SMALL : FEW;
   // Few tiles: 64 x 64, to occupy CUs; fewer than 256 of 128 x 128 are few (Q X of 333 x 1000, 24: 13.5 us against 6.6).
   // X X^T splits its contraction, at least eight blocks to a workgroup: 512 x 4608, 180 workgroups of 128 x 128, 12.1 us
   // against 9.8, but 1024 x 9216, 512 of them, 32 against 41.  From 256 on 128 rows, and for Q X the width whose rounds of 512
@@ -1426,9 +1436,8 @@ struct Run {
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
   }
-  int chain(float f, const Program& prog) const {
-    ORTHO_TRY((ready<&ortho_chain64_kernel>(SLOTS * SLOT64, what)));
-    ortho_chain64_kernel<<<(unsigned)a.count, THREADS64, SLOTS * SLOT64, st>>>(work(), f, prog);
+  int few(float f, const Op& op) const {
+    ortho_few_kernel<<<(unsigned)a.count, THREADS64, 0, st>>>(work(), f, op);
     SNWS_LAUNCH_CHECK(what);
     return SNWS_OK;
   }
@@ -1482,7 +1491,9 @@ int group_ops(const float* coeff, const Scales& s, int k, int g, bool last, Op* 
       spare[1] = old;
       qs = to;
     }
-    if (more) {                                                                   // A <- P (P A), the next X X^T
+    // A <- P (P A)^T, the next X X^T.  Rows by rows, so that it is P A P^T of the rounded P: with (P A) P^T in its place the
+    // error grows tens of times.
+    if (more) {
       square(P, spare[2], spare[3], 0.0, 0.0, s.a[j + 1] / (s.p[j] * s.pa[j]));
       const int old = A;
       A = spare[3];
@@ -1514,13 +1525,11 @@ int run_all(const Mats& a, const Plan& p, const MuonArgs& u, const float* coeff,
   int odd = 0;
   for (int k = 0; k < steps;) {
     const int g = p.group < steps - k ? p.group : steps - k;
-    Op op[MAX_OPS];
+    Op op[GROUP_OPS];
     const int n = group_ops(coeff, s, k, g, k + g == steps, op);
     ORTHO_TRY(p.wg == 128 ? run.gram<Big>(op[0].cc, odd) : run.gram<Fine>(op[0].cc, odd));
-    if (p.mode == CHAIN) {
-      Program prog{};
-      for (int i = 1; i + 1 < n; ++i) prog.op[prog.n++] = op[i];
-      ORTHO_TRY(run.chain(op[0].cc, prog));
+    if (p.mode == FEW) {
+      ORTHO_TRY(run.few(op[0].cc, op[1]));
     } else {
       for (int i = 1; i + 1 < n; ++i) {
         // P A and P Q read the same matrices and write different ones: one launch for both
@@ -1560,6 +1569,36 @@ int check_common(const float* coeff, int steps, float eps, Scales* s, const char
   return SNWS_OK;
 }
 
+// runs use the workspace one after the other
+int64_t bytes_of(const Mats& a, int steps) {
+  Parts s;
+  split(a, s);
+  int64_t most = 0;
+  for (int i = 0; i < s.count; ++i) {
+    Plan p;
+    make_plan(s.list[i], p, steps, s.group[i]);
+    most = p.bytes > most ? p.bytes : most;
+  }
+  return most;
+}
+
+template <typename T, bool MUON>
+int run_parts(Mats& a, const MuonArgs& u, const float* coeff, int steps, float eps, const Scales& scales, void* workspace,
+              int64_t workspace_bytes, const char* what, hipStream_t st) {
+  const int64_t need = bytes_of(a, steps);
+  SNWS_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0,
+                 "%s: workspace of %lld bytes, 256-byte aligned, needed", what, (long long)need);
+  a.ws = static_cast<unsigned char*>(workspace);
+  Parts s;
+  split(a, s);
+  for (int i = 0; i < s.count; ++i) {
+    Plan p;
+    make_plan(s.list[i], p, steps, s.group[i]);
+    ORTHO_TRY((run_all<T, MUON>(s.list[i], p, u, coeff, steps, eps, scales, what, st)));
+  }
+  return SNWS_OK;
+}
+
 }  // namespace
 
 extern "C" int64_t snws_ortho_workspace_bytes(const int* rows, const int* cols, int count, int steps) {
@@ -1568,14 +1607,12 @@ extern "C" int64_t snws_ortho_workspace_bytes(const int* rows, const int* cols, 
     return -1;
   }
   Mats a{};
-  Plan p;
   a.count = count;
   for (int i = 0; i < count; ++i) {
     if (check_size(rows[i], cols[i], "snws_ortho_workspace_bytes") != SNWS_OK) return -1;
     set_shape(a.mat[i], rows[i], cols[i]);
   }
-  make_plan(a, p, steps, false);      // (the group size takes no room)
-  return p.bytes;
+  return bytes_of(a, steps);
 }
 
 extern "C" int snws_orthogonalize(const snws_ortho_item* items, int count, int dtype, const float* coeff, int steps, float eps,
@@ -1586,7 +1623,6 @@ extern "C" int snws_orthogonalize(const snws_ortho_item* items, int count, int d
   Scales s;
   ORTHO_TRY(check_common(coeff, steps, eps, &s, what));
   Mats a{};
-  Plan p;
   a.count = count;
   for (int i = 0; i < count; ++i) {
     const snws_ortho_item& t = items[i];
@@ -1599,13 +1635,10 @@ extern "C" int snws_orthogonalize(const snws_ortho_item* items, int count, int d
     a.mat[i].ldx = t.ldx;
     a.mat[i].ldo = t.ldo;
   }
-  make_plan(a, p, steps, dtype == SNWS_BF16);
-  SNWS_CHECK_ARG(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
-                 "%s: workspace of %lld bytes, 256-byte aligned, needed", what, (long long)p.bytes);
-  a.ws = static_cast<unsigned char*>(workspace);
   const MuonArgs u{};
-  return dtype == SNWS_F32 ? run_all<float, false>(a, p, u, coeff, steps, eps, s, what, (hipStream_t)stream)
-                           : run_all<bf16_t, false>(a, p, u, coeff, steps, eps, s, what, (hipStream_t)stream);
+  return dtype == SNWS_F32
+             ? run_parts<float, false>(a, u, coeff, steps, eps, s, workspace, workspace_bytes, what, (hipStream_t)stream)
+             : run_parts<bf16_t, false>(a, u, coeff, steps, eps, s, workspace, workspace_bytes, what, (hipStream_t)stream);
 }
 
 extern "C" int snws_muon_update(const snws_muon_item* items, int count, float momentum, int nesterov, float grad_scale,
@@ -1617,7 +1650,6 @@ extern "C" int snws_muon_update(const snws_muon_item* items, int count, float mo
   Scales s;
   ORTHO_TRY(check_common(coeff, steps, eps, &s, what));
   Mats a{};
-  Plan p;
   a.count = count;
   for (int i = 0; i < count; ++i) {
     const snws_muon_item& t = items[i];
@@ -1630,10 +1662,6 @@ extern "C" int snws_muon_update(const snws_muon_item* items, int count, float mo
     a.mat[i].ldx = a.mat[i].ldo = t.cols;
     a.mat[i].step = t.lr;
   }
-  make_plan(a, p, steps, true);
-  SNWS_CHECK_ARG(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
-                 "%s: workspace of %lld bytes, 256-byte aligned, needed", what, (long long)p.bytes);
-  a.ws = static_cast<unsigned char*>(workspace);
   const MuonArgs u{momentum, grad_scale, 1.f - weight_decay, nesterov};
-  return run_all<float, true>(a, p, u, coeff, steps, eps, s, what, (hipStream_t)stream);
+  return run_parts<float, true>(a, u, coeff, steps, eps, s, workspace, workspace_bytes, what, (hipStream_t)stream);
 }
