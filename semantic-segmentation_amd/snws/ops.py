@@ -2404,9 +2404,9 @@ def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
     device; returns new contiguous tensors in the same arrangement.  coefficients: (a, b, c), or one such triple per
     step.  A matrix that holds a NaN or an infinity comes out as NaN; the others of the call are not touched by it.
 
-    The error is about that of single steps with float32 products (up to twice it, four times for matrices of a few rows).  The
-    same call gives the same bits; what else is in a list may change a matrix's last digits, as it decides how sums are
-    split.  Not differentiable."""
+    With the default coefficients the error is about that of single steps with float32 products: up to about twice it, four times for
+    matrices of a few rows.  The same call gives the same bits; what else is in a list may change a matrix's last digits, as
+    it decides how sums are split.  Not differentiable."""
     if isinstance(g, torch.Tensor):
         if g.dim() == 2:
             return _orthogonalize([g], steps, coefficients, eps)[0]
