@@ -17,9 +17,10 @@
 //
 // All matrices of a list share each launch: a workgroup finds its matrix and tile from its index.
 //
-// Measured, float32, five steps: 64 x 126 21 us (one launch), 1024 x 9216 354 us (norm 8, start 16, X X^T 31.5 and its join
+// Measured, float32, five steps: 64 x 126 21 us (one launch), 1024 x 9216 361 us (norm 8, start 16, X X^T 31.5 and its join
 // 8 twice, 13 launches of m x m products at 10.8, Q X 53 and 59), the 21 million numbers of 17 filters with their Muon
-// update 800 us (the nine filters of 128 rows and more in threes, then the eight of 64 in single steps).
+// update 807 us (nine of 128 rows and more in threes: 44, 50, 56 and 9 twice, 13 x 19, 103 and 124; eight of 64 in single
+// steps: 125).
 #include "common.h"
 #include <math.h>
 
@@ -1280,7 +1281,7 @@ int square_tiles(int m, int T) {
 // Its price is rounding: A is not taken anew from X, so directions far below the largest lose digits, the more the fewer there
 // are to share the error.  Largest error against float64, over that of single steps with float32 products, of twelve kinds of
 // spectra: single steps 3.6 (3 x 9), 2.7 (8 x 72), 1.5 to 1.6 (from 36 x 324 to 1024 x 9216); threes 4.0 (65 x 200), 3.1
-// (80 x 170), 2.6 (100 x 300), 2.2 (128 x 300), 2.0 (512 x 1100), 2.2 (1024 x 9216), but 6 to 400 up to 64 rows.  So: threes from
+// (80 x 170), 2.6 (100 x 300), 2.2 (128 x 300), 2.0 (512 x 1100), 2.2 (1024 x 9216), but 6 to 33 up to 64 rows (emulated).  So: threes from
 // m = 128 on, else single steps, whatever the type.  The choice is each matrix's own: a list with both is two runs.
 bool in_threes(const Mat& t) { return t.m >= 128 && t.n >= 2 * t.m; }
 
