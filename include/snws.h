@@ -452,7 +452,7 @@ int snws_bn_bwd_pack_post(const float* part, int T, int N, int C, const float* p
  *
  * x (rows, C) with row stride ldx, y with row stride ldy (elements; >= C), any alignment; dtype SNWS_F32 | SNWS_BF16;
  * weight / bias f32 (C) or NULL (ones / zeros).  mean, rstd: f32 (rows), what the backward pass needs of each row, or both
- * NULL.  1 <= C <= 2^28, any rows >= 0; no workspace. */
+ * NULL.  1 <= C <= 2^28, rows >= 0 (below 2^22 where a row is longer than 64 KB); no workspace. */
 int snws_ln_fwd(const void* x, int64_t ldx, const float* weight, const float* bias, void* y, int64_t ldy, int dtype,
                 int64_t rows, int C, float eps, float* mean, float* rstd, void* stream);
 /* With z = (x - mean) rstd and g = dy weight: dx = rstd (g - sum(g)/C - z sum(g z)/C) in dtype (NULL: not wanted);
