@@ -1282,7 +1282,7 @@ int square_tiles(int m, int T) {
 // are to share the error.  Largest error against float64, over that of single steps with float32 products, of twelve kinds of
 // spectra: single steps 3.6 (3 x 9), 2.7 (8 x 72), 1.5 to 1.6 (from 36 x 324 to 1024 x 9216); threes 4.0 (65 x 200), 3.1
 // (80 x 170), 2.6 (100 x 300), 2.2 (128 x 300), 2.0 (512 x 1100), 2.2 (1024 x 9216), but 6 to 33 up to 64 rows (emulated).  So: threes from
-// m = 128 on, else single steps, whatever the type.  The choice is each matrix's own: a list with both is two runs.
+// m = 128 on, else single steps, whatever the type.
 bool in_threes(const Mat& t) { return t.m >= 128 && t.n >= 2 * t.m; }
 
 // the matrices of a call in one run or two
@@ -1291,16 +1291,30 @@ struct Parts {
   Mats list[2];
   int group[2];      // steps taken together
 };
+// A list with both kinds is two runs where the threes save more than the twenty launches of a second run cost, in multiplications
+// of halves; else all go in single steps.  Muon for the 17 filters of a model, two runs and one (us): 0.6e10 saved 228 and 138,
+// 3.3e10 299 and 247, 7.0e10 350 and 348, 9.6e10 381 and 400, 4.0e11 798 and 1017.
+constexpr double RUN_PRODUCTS = 7e10;
 void split(const Mats& a, Parts& s) {
-  s.count = 0;
-  for (int threes = 1; threes >= 0; --threes) {
-    Mats& l = s.list[s.count];
+  double saved = 0.0;
+  int threes = 0;
+  for (int i = 0; i < a.count; ++i) {
+    const double m = a.mat[i].m, n = a.mat[i].n;
+    if (in_threes(a.mat[i])) {
+      ++threes;
+      saved += 3.0 * m * m * (9.0 * n - 8.0 * m);
+    }
+  }
+  const bool both = threes && threes < a.count && saved >= RUN_PRODUCTS;
+  s.count = both ? 2 : 1;
+  s.group[0] = both || threes == a.count ? 3 : 1;
+  s.group[1] = 1;
+  for (int k = 0; k < s.count; ++k) {
+    Mats& l = s.list[k];
     l.count = 0;
-    for (int i = 0; i < a.count; ++i)
-      if (in_threes(a.mat[i]) == (threes != 0)) l.mat[l.count++] = a.mat[i];
-    if (!l.count) continue;
     l.ws = a.ws;
-    s.group[s.count++] = threes ? 3 : 1;
+    for (int i = 0; i < a.count; ++i)
+      if (!both || in_threes(a.mat[i]) == (k == 0)) l.mat[l.count++] = a.mat[i];
   }
 }
 

@@ -2406,7 +2406,7 @@ def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
 
     With the default coefficients the error is about that of single steps with float32 products: up to about twice it, four times for
     matrices of a few rows.  The same call gives the same bits; what else is in a list may change a matrix's last digits, as
-    it decides how sums are split.  Not differentiable."""
+    it decides how sums are split and steps are grouped.  Not differentiable."""
     if isinstance(g, torch.Tensor):
         if g.dim() == 2:
             return _orthogonalize([g], steps, coefficients, eps)[0]
